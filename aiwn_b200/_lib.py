@@ -73,6 +73,17 @@ def load():
         lib.il_attention_backward.restype = ci
         lib.il_attention_dropout_mask.argtypes = [vp, i64, i64, i64, f64, vp, vp]
         lib.il_attention_dropout_mask.restype = ci
+        lib.il_token_logprobs.argtypes = [vp, ci, i64, i64, i64, i64, i64, vp, i64, i64, i64, i64, f64, vp, vp, vp,
+                                          vp, vp, vp]
+        lib.il_token_logprobs.restype = ci
+        lib.il_token_logprobs_backward.argtypes = [vp, ci, i64, i64, i64, i64, i64, vp, i64, i64, i64, i64, f64, vp,
+                                                   vp, vp, vp, vp, vp, vp, i64, i64, vp]
+        lib.il_token_logprobs_backward.restype = ci
+        lib.il_distill_workspace_bytes.argtypes = [i64]
+        lib.il_distill_workspace_bytes.restype = i64
+        lib.il_distill.argtypes = [vp, ci, i64, i64, i64, i64, i64, vp, vp, i64, vp, i64, i64, i64, f64, f64, ci, ci,
+                                   vp, ci, vp, vp, i64, i64, vp, i64, vp]
+        lib.il_distill.restype = ci
         lib.il_bin_counts.argtypes = [vp, ci, i64, i64, i64, f64, vp, vp]
         lib.il_bin_counts.restype = ci
         lib.il_allreduce_scratch_bytes.argtypes = [i64, ci]
@@ -367,6 +378,134 @@ def attention_dropout_mask(keep, B: int, T: int, H: int, p: float, seed):
     with _on_device(keep.device):
         _check(lib.il_attention_dropout_mask(_p(keep), B, T, H, float(p), _p(seed), _stream(keep.device)),
                "il_attention_dropout_mask")
+
+
+MAX_TOP = 128        # alternatives, or a teacher's slots, of a row of logits
+MAX_VOCAB = 1 << 21
+
+
+def _logit_rows(name: str, t):
+    """(B, T, V, stride_b, stride_t) of logits [B, T, V] whose last dimension is contiguous."""
+    if t.dim() != 3 or t.shape[2] < 1:
+        raise ILError(f"{name} must be [B, T, V] with V >= 1, got shape {tuple(t.shape)}")
+    x_dtype_code(t)
+    if t.shape[2] > MAX_VOCAB:
+        raise ILError(f"{name}: {t.shape[2]} logits a row, at most {MAX_VOCAB}")
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        raise ILError(f"{name}: the last dimension must be contiguous, got strides {tuple(t.stride())}")
+    return (*t.shape, t.stride(0), t.stride(1))
+
+
+def _token_strides(name: str, t, B: int, T: int):
+    if t is None:
+        return 0, 0
+    _expect(name, t, (B, T), torch.int64)
+    return t.stride()
+
+
+def _on_cuda(*ts):
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise ILError("aiwn_b200 kernels need CUDA tensors; there is no CPU path")
+
+
+def token_logprobs(logits, tokens, ignore_index: int, temperature: float, logprob, entropy, stats, top_index,
+                   top_logprob):
+    """logprob, entropy [B, T] and top_index, top_logprob [B, T, k] <- logits [B, T, V] (rows with any strides) and
+    tokens [B, T] (or None, with logprob None); stats [B, T, 2] for the backward, or None."""
+    _same_device(logits, tokens, logprob, entropy, stats, top_index, top_logprob)
+    B, T, V, sb, st = _logit_rows("logits", logits)
+    k = top_index.shape[-1]
+    if k > min(V, MAX_TOP):
+        raise ILError(f"top_k {k}: at most {MAX_TOP}, and no more than the {V} logits of a row")
+    tb, tt = _token_strides("tokens", tokens, B, T)
+    _expect("logprob", logprob, (B, T))
+    if tokens is not None and logprob is None:
+        raise ILError("tokens without an output for their log probabilities")
+    _expect("entropy", entropy, (B, T))
+    _expect("stats", stats, (B, T, 2))
+    _expect("top_index", top_index, (B, T, k), torch.int64)
+    _expect("top_logprob", top_logprob, (B, T, k))
+    _on_cuda(logits, tokens)
+    _need_cuda(logprob, entropy, stats, top_index, top_logprob)
+    lib = load()
+    with _on_device(logits.device):
+        _check(lib.il_token_logprobs(_p(logits), x_dtype_code(logits), B, T, V, sb, st, _p(tokens), tb, tt,
+                                     int(ignore_index), k, float(temperature), _p(logprob), _p(entropy), _p(stats),
+                                     _p(top_index), _p(top_logprob), _stream(logits.device)), "il_token_logprobs")
+
+
+def token_logprobs_backward(logits, tokens, ignore_index: int, temperature: float, entropy, stats, top_index,
+                            g_logprob, g_entropy, g_top, dlogits):
+    """dlogits [B, T, V] <- gradient of token_logprobs from g_logprob, g_entropy [B, T] and g_top [B, T, k] (each may
+    be None)."""
+    _same_device(logits, tokens, entropy, stats, top_index, g_logprob, g_entropy, g_top, dlogits)
+    B, T, V, sb, st = _logit_rows("logits", logits)
+    k = top_index.shape[-1]
+    if k > min(V, MAX_TOP):
+        raise ILError(f"top_k {k}: at most {MAX_TOP}, and no more than the {V} logits of a row")
+    tb, tt = _token_strides("tokens", tokens, B, T)
+    _expect("dlogits", dlogits, (B, T, V), logits.dtype)
+    *_, db, dt = _logit_rows("dlogits", dlogits)
+    for name, t in (("entropy", entropy), ("g_logprob", g_logprob), ("g_entropy", g_entropy)):
+        _expect(name, t, (B, T))
+    if g_logprob is not None and tokens is None:
+        raise ILError("g_logprob without tokens")
+    _expect("stats", stats, (B, T, 2))
+    _expect("top_index", top_index, (B, T, k), torch.int64)
+    _expect("g_top", g_top, (B, T, k))
+    _on_cuda(logits, tokens, dlogits)
+    _need_cuda(entropy, stats, top_index, g_logprob, g_entropy, g_top)
+    lib = load()
+    with _on_device(logits.device):
+        _check(lib.il_token_logprobs_backward(
+            _p(logits), x_dtype_code(logits), B, T, V, sb, st, _p(tokens), tb, tt, int(ignore_index), k,
+            float(temperature), _p(entropy), _p(stats), _p(top_index), _p(g_logprob), _p(g_entropy), _p(g_top),
+            _p(dlogits), db, dt, _stream(logits.device)), "il_token_logprobs_backward")
+
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def distill_workspace_bytes(N: int) -> int:
+    return int(load().il_distill_workspace_bytes(int(N)))
+
+
+def distill(logits, top_index, top_logprob, targets, ignore_index: int, alpha: float, temperature: float, tail: bool,
+            reduction: str, loss, dlogits, workspace, g=None, only_if_not_one: bool = False):
+    """loss ([B, T] for reduction "none", else []) and dlogits [B, T, V] (either may be None) <- distillation of
+    logits [B, T, V] from the teacher's top_index (int64) and top_logprob [B, T, k]; the gradient is multiplied by g
+    (like loss, on the device; None: 1), and nothing is written where only_if_not_one is set and g is 1."""
+    _same_device(logits, top_index, top_logprob, targets, loss, dlogits, workspace, g)
+    B, T, V, sb, st = _logit_rows("logits", logits)
+    if reduction not in REDUCTIONS:
+        raise ILError(f"reduction {reduction!r}: one of {sorted(REDUCTIONS)}")
+    if top_index.dim() != 3 or top_index.shape[2] > MAX_TOP:
+        raise ILError(f"top_index must be [B, T, k] with k <= {MAX_TOP}, got shape {tuple(top_index.shape)}")
+    k = top_index.shape[2]
+    _expect("top_index", top_index, (B, T, k), torch.int64)
+    _expect("top_logprob", top_logprob, (B, T, k))
+    tb, tt = _token_strides("targets", targets, B, T)
+    if alpha < 1.0 and targets is None:
+        raise ILError(f"alpha {alpha} < 1 needs targets")
+    shape = (B, T) if reduction == "none" else ()
+    _expect("loss", loss, shape)
+    _expect("g", g, shape)
+    db = dt = 0
+    if dlogits is not None:
+        _expect("dlogits", dlogits, (B, T, V), logits.dtype)
+        *_, db, dt = _logit_rows("dlogits", dlogits)
+    if workspace is not None and workspace.dtype != torch.uint8:
+        raise ILError("workspace must be a uint8 tensor")
+    _on_cuda(logits, targets, dlogits)
+    _need_cuda(top_index, top_logprob, loss, workspace, g)
+    lib = load()
+    with _on_device(logits.device):
+        _check(lib.il_distill(
+            _p(logits), x_dtype_code(logits), B, T, V, sb, st, _p(top_index), _p(top_logprob), k, _p(targets), tb, tt,
+            int(ignore_index), float(alpha), float(temperature), int(bool(tail)), REDUCTIONS[reduction], _p(g),
+            int(bool(only_if_not_one)), _p(loss), _p(dlogits), db, dt, _p(workspace),
+            0 if workspace is None else workspace.numel(), _stream(logits.device)), "il_distill")
 
 
 def bin_counts(x, K: int, bw: float, counts):

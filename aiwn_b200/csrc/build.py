@@ -15,6 +15,8 @@ import glob
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -22,19 +24,23 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libaiwn_il.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
+ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a",
+    *ARCH,
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-    "--shared", "-cudart", "static",
     "-prec-div=true", "-prec-sqrt=true", "-ftz=false", "-fmad=true",
     "-Xptxas", "-warn-spills",
 ]
 
 
 def sources():
-    return sorted(glob.glob(os.path.join(HERE, "*.cu"))) + sorted(glob.glob(os.path.join(HERE, "*.cuh"))) + [
+    return units() + sorted(glob.glob(os.path.join(HERE, "*.cuh"))) + sorted(glob.glob(os.path.join(HERE, "*.h"))) + [
         os.path.join(ROOT, "include", "aiwn_il.h")]
+
+
+def units():
+    return sorted(glob.glob(os.path.join(HERE, "*.cu")))
 
 
 def up_to_date() -> bool:
@@ -47,11 +53,16 @@ def up_to_date() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB
-    cmd = [NVCC, *FLAGS, "-I", os.path.join(ROOT, "include"), "-o", LIB + ".tmp",
-           os.path.join(HERE, "il_capi.cu")]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(u) + ".o") for u in units()]
+        cmds = [[NVCC, *FLAGS, "-I", os.path.join(ROOT, "include"), "-c", "-o", o, u] for o, u in zip(objs, units())]
+        link = [NVCC, *ARCH, "--shared", "-cudart", "static", "-o", LIB + ".tmp", *objs]
+        if verbose:
+            print(*(" ".join(c) for c in (*cmds, link)), sep="\n")
+        with ThreadPoolExecutor() as pool:  # the units are compiled side by side
+            for _ in pool.map(lambda c: subprocess.run(c, check=True), cmds):
+                pass
+        subprocess.run(link, check=True)
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

@@ -14,6 +14,7 @@
 #include <mutex>
 
 #include "../../include/aiwn_il.h"
+#include "il_host.h"
 #include "il_common.cuh"
 #include "il_simple.cuh"
 #include "il_fast.cuh"
@@ -349,6 +350,13 @@ int noalloc_cross_wait(int world, void* const* streams, bool summed) {
 }
 
 }  // namespace
+
+namespace il {
+
+int host_check_device(int* num_sms) { return check_device(num_sms); }
+int host_launch_status(int kernels) { return launch_status(kernels); }
+
+}  // namespace il
 
 extern "C" {
 

@@ -1,0 +1,242 @@
+// il_logits.cu -- entry points of the operators on a language model's logits:
+// il_token_logprobs, il_distill and their gradients (include/aiwn_il.h).
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/aiwn_il.h"
+#include "il_host.h"
+#include "il_distill.cuh"
+#include "il_score.cuh"
+
+namespace {
+
+using namespace il;
+
+constexpr double kLog2e = 1.4426950408889634074;
+
+// how a [B, T, V] operand is cut up
+struct Plan {
+    int regs;       // logits a lane holds, rows of one warp; 0: CTAs
+    uint32_t ctas;  // CTAs of a row
+    unsigned grid;
+};
+
+int check_rows(int dtype, int64_t B, int64_t T, int64_t V, double temperature) {
+    if (dtype != IL_F32 && dtype != IL_BF16) return IL_ERR_DTYPE;
+    if (B < 0 || T < 0 || V < 1 || V > kMaxVocab) return IL_ERR_SHAPE;
+    if (B > 0 && T > (int64_t(1) << 30) / B) return IL_ERR_SHAPE;
+    const float tau = (float)temperature;
+    if (!(tau > 0.0f) || isinf(tau) || isinf(1.0f / tau)) return IL_ERR_VALUE;
+    return IL_OK;
+}
+
+// the row stride of the operands and their element size: natural alignment of the base is all that is asked
+int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_BF16 ? 1u : 3u)) ? IL_ERR_ALIGN : IL_OK; }
+
+Plan plan_rows(int64_t N, int64_t V, int sms) {
+    Plan p{0, 1, 0};
+    if (V <= kWarpVocab) {
+        p.regs = (int)((V + 31) / 32);
+        const int64_t blocks = (N + 7) / 8, most = (int64_t)sms * 8;
+        p.grid = (unsigned)(blocks < most ? blocks : most);
+        return p;
+    }
+    while (p.ctas < kMaxCluster && ((int64_t)N * p.ctas < sms && V / (2 * p.ctas) >= 4096)) p.ctas *= 2;
+    while (p.ctas < kMaxCluster && V / p.ctas > (1 << 18)) p.ctas *= 2;
+    const int64_t rows = N < (1 << 20) ? N : (1 << 20);
+    p.grid = (unsigned)(rows * p.ctas);
+    return p;
+}
+
+template <class... P, class... A>
+int launch(void (*kern)(P...), unsigned grid, int threads, uint32_t ctas, size_t smem, cudaStream_t s, A... args) {
+    if (smem > 40 * 1024 &&  // beyond 48 KB with the static arrays
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+        cudaGetLastError();
+        return IL_ERR_LAUNCH;
+    }
+    if (ctas > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaGetLastError();
+        return IL_ERR_LAUNCH;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = ctas;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = ctas > 1 ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kern, P(args)...) != cudaSuccess) {
+        cudaGetLastError();
+        return IL_ERR_LAUNCH;
+    }
+    return host_launch_status(1);
+}
+
+// f(integral constant E) for the smallest instantiated E >= regs
+template <class F>
+int with_regs(int regs, F f) {
+#define IL_REGS(E) \
+    if (regs <= E) return f(std::integral_constant<int, E>());
+    IL_REGS(1) IL_REGS(2) IL_REGS(3) IL_REGS(4) IL_REGS(8) IL_REGS(16) IL_REGS(32)
+#undef IL_REGS
+    return IL_ERR_SHAPE;
+}
+template <class F>
+int with_dtype(int dtype, F f) {
+    return dtype == IL_BF16 ? f(std::integral_constant<int, kBF16>()) : f(std::integral_constant<int, kF32>());
+}
+template <class F>
+int with_bool(bool b, F f) {
+    return b ? f(std::true_type()) : f(std::false_type());
+}
+
+}  // namespace
+
+extern "C" {
+
+int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t stride_b,
+                      int64_t stride_t, const int64_t* tokens, int64_t tokens_b, int64_t tokens_t,
+                      int64_t ignore_index, int64_t k, double temperature, float* logprob, float* entropy,
+                      float* stats, int64_t* top_index, float* top_logprob, void* stream) {
+    int st = check_rows(dtype, B, T, V, temperature);
+    if (st) return st;
+    if (k < 0 || k > kMaxTop || k > V) return IL_ERR_SHAPE;
+    if (B * T == 0) return IL_OK;
+    if (!logits || !entropy || (tokens && !logprob) || (k > 0 && (!top_index || !top_logprob))) return IL_ERR_NULL;
+    if ((st = check_align(logits, dtype))) return st;
+    if ((uintptr_t)stats & 7u) return IL_ERR_ALIGN;
+    int sms = 0;
+    if ((st = host_check_device(&sms))) return st;
+    ScoreArgs a{};
+    a.z = RowsIn{logits, stride_b, stride_t, (uint32_t)T};
+    a.tok = Tokens{tokens, tokens_b, tokens_t, ignore_index};
+    a.N = (uint32_t)(B * T), a.V = (int)V, a.k = (int)k;
+    a.tau = (float)temperature, a.c = (float)(kLog2e / temperature);
+    a.logprob = tokens ? logprob : nullptr, a.entropy = entropy, a.stats = reinterpret_cast<float2*>(stats);
+    a.top_index = top_index, a.top_logprob = top_logprob;
+    const Plan p = plan_rows(a.N, V, sms);
+    cudaStream_t s = (cudaStream_t)stream;
+    return with_dtype(dtype, [&](auto dt) {
+        if (p.regs)
+            return with_regs(p.regs, [&](auto e) {
+                return launch(score_warp_kernel<dt.value, e.value>, p.grid, 256, 1, 0, s, a);
+            });
+        return with_bool(k > 0, [&](auto top) {
+            const size_t smem = top.value ? 8 * (size_t)(top_list(a.k) + (p.ctas > 1 ? top_merge(a.k) : 0)) : 0;
+            return launch(score_row_kernel<dt.value, top.value>, p.grid, kRowThreads, p.ctas, smem, s, a, p.ctas);
+        });
+    });
+}
+
+int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t stride_b,
+                               int64_t stride_t, const int64_t* tokens, int64_t tokens_b, int64_t tokens_t,
+                               int64_t ignore_index, int64_t k, double temperature, const float* entropy,
+                               const float* stats, const int64_t* top_index, const float* g_logprob,
+                               const float* g_entropy, const float* g_top, void* dlogits, int64_t dstride_b,
+                               int64_t dstride_t, void* stream) {
+    int st = check_rows(dtype, B, T, V, temperature);
+    if (st) return st;
+    if (k < 0 || k > kMaxTop || k > V) return IL_ERR_SHAPE;
+    if (B * T == 0) return IL_OK;
+    if (!logits || !entropy || !stats || !dlogits || (g_logprob && !tokens) || (k > 0 && g_top && !top_index))
+        return IL_ERR_NULL;
+    if ((st = check_align(logits, dtype)) || (st = check_align(dlogits, dtype))) return st;
+    if ((uintptr_t)stats & 7u) return IL_ERR_ALIGN;
+    int sms = 0;
+    if ((st = host_check_device(&sms))) return st;
+    ScoreGradArgs a{};
+    a.z = RowsIn{logits, stride_b, stride_t, (uint32_t)T};
+    a.tok = Tokens{tokens, tokens_b, tokens_t, ignore_index};
+    a.d = RowsOut{dlogits, dstride_b, dstride_t, (uint32_t)T};
+    a.N = (uint32_t)(B * T), a.V = (int)V, a.k = (int)k;
+    a.tau = (float)temperature, a.c = (float)(kLog2e / temperature);
+    a.stats = reinterpret_cast<const float2*>(stats), a.entropy = entropy, a.top_index = top_index;
+    a.g_logprob = g_logprob, a.g_entropy = g_entropy, a.g_top = k > 0 ? g_top : nullptr;
+    const Plan p = plan_rows(a.N, V, sms);
+    cudaStream_t s = (cudaStream_t)stream;
+    return with_dtype(dtype, [&](auto dt) {
+        if (p.regs)
+            return with_regs(p.regs, [&](auto e) {
+                return launch(score_grad_warp_kernel<dt.value, e.value>, p.grid, 256, 1, 0, s, a);
+            });
+        const uint32_t parts = (uint32_t)((V + 32767) / 32768);
+        const int64_t grid = (int64_t)a.N * parts;
+        if (grid > 0x7fffffff) return (int)IL_ERR_SHAPE;
+        return launch(score_grad_row_kernel<dt.value>, (unsigned)grid, kRowThreads, 1, 0, s, a, parts);
+    });
+}
+
+int64_t il_distill_workspace_bytes(int64_t N) { return N < 0 ? -1 : (N + 4) * 4; }
+
+int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t stride_b, int64_t stride_t,
+               const int64_t* top_index, const float* top_logprob, int64_t k, const int64_t* targets,
+               int64_t targets_b, int64_t targets_t, int64_t ignore_index, double alpha, double temperature, int tail,
+               int reduction, const float* g, int only_if_not_one, float* loss, void* dlogits, int64_t dstride_b,
+               int64_t dstride_t, void* workspace, int64_t workspace_bytes, void* stream) {
+    int st = check_rows(dtype, B, T, V, temperature);
+    if (st) return st;
+    if (k < 0 || k > kMaxTop || reduction < 0 || reduction > 2) return IL_ERR_SHAPE;
+    if (!(alpha >= 0.0 && alpha <= 1.0)) return IL_ERR_VALUE;
+    const int64_t N = B * T;
+    if (N == 0 && (reduction == 0 || !loss)) return IL_OK;
+    if (!loss && !dlogits) return IL_ERR_NULL;
+    if (N > 0 && (!logits || (k > 0 && (!top_index || !top_logprob)) || (alpha < 1.0 && !targets))) return IL_ERR_NULL;
+    if (only_if_not_one && (!g || reduction == 0)) return IL_ERR_NULL;
+    if ((st = check_align(logits, dtype)) || (st = check_align(dlogits, dtype))) return st;
+    const bool whole = reduction != 0;
+    if (whole && (!workspace || workspace_bytes < il_distill_workspace_bytes(N))) return IL_ERR_WORKSPACE;
+    if ((uintptr_t)workspace & 15u) return IL_ERR_ALIGN;
+    int sms = 0;
+    if ((st = host_check_device(&sms))) return st;
+    cudaStream_t s = (cudaStream_t)stream;
+    float* ws = reinterpret_cast<float*>(workspace);
+    DistillArgs a{};
+    a.z = RowsIn{logits, stride_b, stride_t, (uint32_t)T};
+    a.tok = Tokens{targets, targets_b, targets_t, ignore_index};
+    a.d = RowsOut{dlogits, dstride_b, dstride_t, (uint32_t)T};
+    a.N = (uint32_t)N, a.V = (int)V, a.k = (int)k;
+    a.index = top_index, a.logprob = top_logprob;
+    a.tau = (float)temperature, a.c = (float)(kLog2e / temperature), a.alpha = (float)alpha;
+    a.tail = tail != 0, a.hard = alpha < 1.0;
+    a.scale = 1.0f;
+    a.g = g, a.g_rows = reduction == 0, a.skip_if_one = only_if_not_one;
+    a.loss = loss ? (whole ? ws + 4 : loss) : nullptr;
+    if (reduction == kMean) {
+        if (targets && N > 0) {
+            a.scale_p = ws;
+            if ((st = launch(distill_count_kernel, 1, 1024, 1, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
+        } else {
+            a.scale = 1.0f / (float)(N > 1 ? N : 1);
+        }
+    }
+    if (N > 0) {
+        const Plan p = plan_rows(N, V, sms);
+        const bool two = a.hard && a.tau != 1.0f;
+        st = with_dtype(dtype, [&](auto dt) {
+            return with_bool(a.tail, [&](auto tl) {
+                return with_bool(two, [&](auto s1) {
+                    if (p.regs)
+                        return with_regs(p.regs, [&](auto e) {
+                            return launch(distill_warp_kernel<dt.value, e.value, tl.value, s1.value>, p.grid, 256, 1, 0,
+                                          s, a);
+                        });
+                    const size_t smem = tl.value ? 4 * (size_t)distill_words(a.V, p.ctas) : 0;
+                    return launch(distill_row_kernel<dt.value, tl.value, s1.value>, p.grid, kRowThreads, p.ctas, smem, s,
+                                  a, p.ctas);
+                });
+            });
+        });
+        if (st) return st;
+    }
+    if (whole && loss)
+        return launch(distill_total_kernel, 1, 1024, 1, 0, s, (const float*)(ws + 4), a.N, a.scale, a.scale_p, loss);
+    return IL_OK;
+}
+
+}  // extern "C"

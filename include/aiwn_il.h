@@ -207,6 +207,69 @@ IL_API int il_attention_dropout_mask(uint8_t* keep, int64_t B, int64_t T, int64_
                               const uint64_t* seed, void* stream);
 
 /*
+ * Log probabilities of given tokens under softmax(logits / temperature), the
+ * entropy of that distribution, and its k largest logits (no counterpart in
+ * the reference, whose IndexedGPT returns a mean cross-entropy,
+ * transformer_validation.py:365-370).  logits [B, T, V] (IL_F32 / IL_BF16),
+ * the last dimension contiguous, the others stride_b and stride_t elements
+ * apart; any alignment of the rows.  tokens [B, T] with its strides, or NULL
+ * (then logprob may be NULL).  Outputs over N = B*T rows: logprob [N],
+ * entropy [N], stats [N, 2] for the backward (8-byte aligned, or NULL),
+ * top_index and top_logprob [N, k] (largest first, equal logits by index).
+ * V <= 2^21, k <= 128 and <= V.
+ *   A row whose token is ignore_index is padding: its logits are not read,
+ * logprob and entropy are 0, its indices -1 and their log probabilities -inf.
+ * A token outside [0, V) gets NaN.  Where every logit is -inf, logprob is
+ * -inf and the entropy 0; a NaN or +inf logit makes a row's results NaN (a NaN
+ * counts as -inf among the alternatives).
+ */
+IL_API int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t stride_b,
+                             int64_t stride_t, const int64_t* tokens, int64_t tokens_b, int64_t tokens_t,
+                             int64_t ignore_index, int64_t k, double temperature, float* logprob, float* entropy,
+                             float* stats, int64_t* top_index, float* top_logprob, void* stream);
+
+/*
+ * Gradient of il_token_logprobs: dlogits [B, T, V] (the type of logits, its
+ * own strides; overwritten, 0 in padded rows) from g_logprob [N], g_entropy
+ * [N] and g_top [N, k] (each may be NULL), with the forward's entropy, stats
+ * and top_index.
+ */
+IL_API int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t T, int64_t V,
+                                      int64_t stride_b, int64_t stride_t, const int64_t* tokens, int64_t tokens_b,
+                                      int64_t tokens_t, int64_t ignore_index, int64_t k, double temperature,
+                                      const float* entropy, const float* stats, const int64_t* top_index,
+                                      const float* g_logprob, const float* g_entropy, const float* g_top,
+                                      void* dlogits, int64_t dstride_b, int64_t dstride_t, void* stream);
+
+/*
+ * Distillation from a teacher's k <= 128 log probabilities a row, and the
+ * gradient of the logits in the same call (no counterpart in the reference).
+ * With p = softmax(logits / temperature), slots (top_index, top_logprob)
+ * [N, k] (an index < 0 is an empty slot; one that occurs twice counts twice),
+ *   tail == 0:  q = softmax(top_logprob) over the slots
+ *   tail != 0:  q = exp(top_logprob), the rest q_r = max(0, 1 - sum q) is one
+ *               bucket against p_r, the student's mass outside the slots
+ *   KL = sum q (ln q - ln p) [+ q_r (ln q_r - ln p_r)]
+ *   row loss = alpha temperature^2 KL - (1 - alpha) ln softmax(logits)[target]
+ * targets [B, T] may be NULL when alpha == 1; rows whose target is
+ * ignore_index are left out (loss 0, gradient 0).  reduction 0: loss [N];
+ * 1: the mean over the rows that are not left out (0 if there are none);
+ * 2: their sum.  loss may be NULL (gradient only), dlogits may be NULL.
+ * The gradient is that of loss times g (device memory: one value, or [N] with
+ * reduction 0; NULL: 1).  With only_if_not_one, nothing is written to loss or
+ * dlogits when *g == 1.  A slot index >= V or, with alpha < 1, a target
+ * outside [0, V) makes the row NaN.  workspace: il_distill_workspace_bytes(N)
+ * (reduction 1 and 2), 16-byte aligned, used until the call's kernels end.
+ */
+IL_API int64_t il_distill_workspace_bytes(int64_t N);
+IL_API int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t stride_b,
+                      int64_t stride_t, const int64_t* top_index, const float* top_logprob, int64_t k,
+                      const int64_t* targets, int64_t targets_b, int64_t targets_t, int64_t ignore_index,
+                      double alpha, double temperature, int tail, int reduction, const float* g,
+                      int only_if_not_one, float* loss, void* dlogits, int64_t dstride_b, int64_t dstride_t,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Backward of the GaussianCDFNorm prologue: given gxn = dL/dxn (from
  * il_backward run on xn), writes dx [N, IN] and overwrites dgamma, dbeta [IN].
  * Any of dx / dgamma / dbeta may be NULL.  IN <= 16384.  PyTorch autograd's
