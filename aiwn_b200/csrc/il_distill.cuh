@@ -38,210 +38,224 @@ struct DistillArgs {
     const int64_t* index;  // [N, k], < 0: empty slot
     const float* logprob;  // [N, k]
     float tau, c, alpha;
-    int tail, hard;        // hard: the target's term is wanted (alpha < 1)
-    float scale;           // of the gradient
+    int hard;              // the target's term is wanted (alpha < 1)
+    float scale;           // of the gradient and of a whole loss
     const float* scale_p;  // times *scale_p, or null
-    const float* g;        // times g[0], or g[row] with g_rows, or null
+    const float* g;        // gradient: times g[0], or g[row] with g_rows, or null
     int g_rows;
     int skip_if_one;       // nothing is left to do where g[0] == 1
-    float* loss;           // [N] or null
+    float* loss;           // [N] (each), [1], or null
+    int each;
+    uint32_t* ticket;      // 0 before the call, and partial sums of a whole loss, one a CTA
+    float* partial;
 };
 
-struct DistillRow {  // what a warp found out about a row's slots, in shared memory
-    int index[kMaxTop + 1];  // the last of the k + 1: the target; -1: none
-    float q[kMaxTop];
-    Sums slots;              // of the slots' logits, each token once (with tail)
-    float Q, rest;           // rest: q_r
-    float own;               // sum q_i (ln q_i - (z_i - m0) / tau), m0 = base
-    float base, used;        // used: sum of q_i over the slots
-    float z_target;
-    int bad;
-    // gradient: e_j coef + e1_j coef1 with e_j = 2^((z_j - h) c), e1_j = 2^((z_j - h1) log2 e)
-    float h, coef, h1, coef1;
-    // at a slot: 2^((z - h1) c) inside - w q
-    float inside, w, w_hard;
+struct Slot {  // a teacher's value, of one lane
+    int j;     // -1: none
+    float l, z;
 };
 
-// One warp.  Reads the slots of a row.
-template <int DT>
-__device__ __forceinline__ void distill_slots(const DistillArgs& a, uint32_t row, const typename Elem<DT>::type* zr,
-                                              int64_t t, DistillRow& r) {
-    constexpr int kPer = kMaxTop / 32;
-    const int lane = threadIdx.x & 31;
-    bool bad = false;
-    int j[kPer];
-    float l[kPer], z[kPer], q[kPer];
-#pragma unroll
-    for (int n = 0; n < kPer; ++n) {
-        const int i = lane + 32 * n;
-        j[n] = -1;
-        l[n] = -INFINITY;
-        z[n] = -INFINITY;
-        if (i < a.k) {
-            const int64_t x = a.index[(int64_t)row * a.k + i];
-            bad |= x >= a.V;
-            if (x >= 0 && x < a.V) {
-                j[n] = (int)x;
-                l[n] = a.logprob[(int64_t)row * a.k + i];
-                z[n] = to_float(zr[x]);
-            }
-            r.index[i] = j[n];
-        }
-    }
-    // weights
-    float Q, rest = 0.0f, shift = 0.0f, log_sum = 0.0f;
-    if (a.tail) {
-        double sum = 0.0;
-#pragma unroll
-        for (int n = 0; n < kPer; ++n) {
-            const double e = j[n] >= 0 ? exp((double)l[n]) : 0.0;
-            q[n] = (float)e;
-            sum += e;
-        }
-        sum = warp_sum(sum);
-        const double left = 1.0 - sum;
-        rest = left > 0.0 || left != left ? (float)left : 0.0f;
-        Q = (float)(left > 0.0 ? 1.0 : sum);
-    } else {
-        float m = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int n = 0; n < kPer; ++n) m = fmaxf(m, l[n]);
-        shift = shift_of(warp_max(m));
-#pragma unroll
-        for (int n = 0; n < kPer; ++n) {
-            q[n] = j[n] >= 0 ? expf(l[n] - shift) : 0.0f;
-            sum += q[n];
-        }
-        sum = warp_sum(sum);
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        log_sum = sum == 0.0f ? 0.0f : logf(sum);
-#pragma unroll
-        for (int n = 0; n < kPer; ++n) q[n] *= inv;
-        Q = sum == 0.0f ? 0.0f : 1.0f;
-    }
-    // sums over the slots; base: their largest logit
-    float base = -INFINITY, own = 0.0f, used = 0.0f;
-#pragma unroll
-    for (int n = 0; n < kPer; ++n) base = fmaxf(base, z[n]);
-    base = shift_of(warp_max(base));
-#pragma unroll
-    for (int n = 0; n < kPer; ++n) {
-        const int i = lane + 32 * n;
-        if (i < a.k) r.q[i] = q[n];
-        used += q[n];
-        own += q[n] == 0.0f ? 0.0f : q[n] * ((l[n] - shift - log_sum) - (z[n] - base) / a.tau);
-    }
-    used = warp_sum(used);
-    own = warp_sum(own);
-    __syncwarp();
-    if (a.tail) {
-        Sums s = no_sums();
-#pragma unroll
-        for (int n = 0; n < kPer; ++n) {
-            if (j[n] < 0) continue;
-            bool first = true;  // a token that several slots name counts once
-            for (int i = 0; i < lane + 32 * n; ++i) first &= r.index[i] != j[n];
-            const float x[1] = {z[n]};
-            if (first) add_values<1, false, true>(s, x, z[n], a.c, 1.44269504088896341f);
-        }
-        s = warp_join<false, true>(s, a.c, 1.44269504088896341f);
-        if (lane == 0) r.slots = s;
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) {
-        r.Q = Q, r.rest = rest, r.own = own, r.base = base, r.used = used;
-        r.index[a.k] = -1;
-        r.z_target = 0.0f;
-        if (a.hard) {
-            if (t >= 0 && t < a.V) {
-                r.index[a.k] = (int)t;
-                r.z_target = to_float(zr[t]);
-            } else {
-                bad = true;
-            }
-        }
-        r.bad = bad;
-    }
-    __syncwarp();
+// What a warp's lanes found out about their slots: with w_i = exp(l_i - top)
+// (tail: exp(l_i)), mass = sum w, cross = sum w ((l_i - top) - (z_i - base) / tau)
+struct SlotSums {
+    float top, mass, cross, base;
+    double left;  // sum of exp(l_i) in 64 bits (tail)
+    Sums s;       // of the slots' logits, each token once (tail)
+    int bad, pad;
+};
+
+template <bool TAIL>
+__device__ __forceinline__ float slot_weight(float l, float top) {
+    return TAIL ? expf(l) : expf(l - top);
 }
 
-// One thread.  The row's loss, and what its gradient is made of.  s: the sums of
-// the row, or of what no slot names (tail)
-__device__ __forceinline__ float distill_row(const DistillArgs& a, uint32_t row, Sums s, DistillRow& r) {
-    const float c1 = 1.44269504088896341f;
-    const bool two = a.hard && a.tau != 1.0f;
+// n: slots of this lane; first: whether slot q is the first to name its token (tail)
+template <bool TAIL, bool S1, int n, class First>
+__device__ __forceinline__ SlotSums slot_sums(const DistillArgs& a, const Slot (&x)[n], int used, bool bad, First first) {
+    SlotSums r;
+    float top = -INFINITY, base = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < n; ++q)
+        if (q < used) top = fmaxf(top, x[q].l), base = fmaxf(base, x[q].z);
+    r.top = TAIL ? 0.0f : shift_of(warp_max(top));
+    r.base = shift_of(warp_max(base));
+    float mass = 0.0f, cross = 0.0f;
+    double left = 0.0;
+    r.s = no_sums();
+#pragma unroll
+    for (int q = 0; q < n; ++q) {
+        if (q >= used) continue;
+        const bool is = x[q].j >= 0;
+        const float w = is ? slot_weight<TAIL>(x[q].l, r.top) : 0.0f;
+        mass += w;
+        if (w != 0.0f) cross += w * ((x[q].l - r.top) - (x[q].z - r.base) / a.tau);
+        if constexpr (TAIL) {
+            if (is) left += exp((double)x[q].l);
+            if (is && first(q)) {
+                const float y[1] = {x[q].z};
+                add_values<1, false, S1>(r.s, y, x[q].z, a.c);
+            }
+        }
+    }
+    r.mass = warp_sum(mass);
+    r.cross = warp_sum(cross);
+    if constexpr (TAIL) {
+        r.left = warp_sum(left);
+        r.s = warp_join<false, S1>(r.s, a.c);
+    }
+    r.bad = __any_sync(0xffffffffu, bad);
+    return r;
+}
+
+// A row's gradient at a logit that no slot names: 2^((z - h) c) coef + 2^((z - h1) log2 e) coef1;
+// at one that slots name: 2^((z - h1) c) inside + 2^((z - h1) log2 e) coef1 - soft sum of the slots' weights;
+// less `hard` at the target.
+struct DistillRow {
+    float loss, h, coef, h1, coef1, inside, soft, hard, top, c;
+    template <bool S1>
+    __device__ __forceinline__ float at(float z) const {
+        float y = exp2_approx((z - h) * c) * coef;
+        if constexpr (S1) y = fmaf(exp2_approx((z - h1) * kLog2e), coef1, y);
+        return y;
+    }
+    template <bool S1>
+    __device__ __forceinline__ float at_slot(float z, float weight) const {
+        float y = fmaf(exp2_approx((z - h1) * c), inside, -soft * weight);
+        if constexpr (S1) y = fmaf(exp2_approx((z - h1) * kLog2e), coef1, y);
+        return y;
+    }
+};
+
+// s: the sums of the row, or of what no slot names (tail); part: the slots' of `parts` warps;
+// z_t: the target's logit, NaN for one outside the vocabulary
+template <bool TAIL, bool S1>
+__device__ __forceinline__ DistillRow distill_row(const DistillArgs& a, uint32_t row, Sums s, const SlotSums* part,
+                                                  int parts, float z_t, bool gradient) {
+    DistillRow r;
+    float top = 0.0f, mass = 0.0f;
+    bool bad = false;
+    if constexpr (!TAIL) {
+        top = -INFINITY;
+        for (int n = 0; n < parts; ++n)
+            if (part[n].mass != 0.0f) top = fmaxf(top, part[n].top);
+        top = shift_of(top);
+    }
     const Sums rest = s;
-    if (a.tail) s = two ? join<false, true>(s, r.slots, a.c, c1) : join<false, false>(s, r.slots, a.c, c1);
-    const float h = shift_of(s.m), log_s = logf(s.s);
-    float kl = r.own;
-    // - ln p_i = ln s - (z_i - h) / tau, and own holds - (z_i - base) / tau
-    if (r.used != 0.0f) kl += r.used * (s.s == 0.0f ? INFINITY : log_s - (r.base - h) / a.tau);
-    const float hr = shift_of(rest.m);
-    if (a.tail && r.rest != 0.0f)
-        kl += rest.s == 0.0f ? (r.rest != r.rest ? NAN : INFINITY)
-                             : r.rest * (logf(r.rest) - ((hr - h) / a.tau + logf(rest.s) - log_s));
-    float loss = a.alpha == 0.0f ? 0.0f : a.alpha * a.tau * a.tau * kl;
-    const float s1 = two ? s.s1 : s.s;
-    if (a.hard) loss -= (1.0f - a.alpha) * (s1 == 0.0f ? -INFINITY : r.z_target - h - logf(s1));
-    if (r.bad) loss = NAN;
-    if (a.d.p) {
+    double left = 0.0;
+    for (int n = 0; n < parts; ++n) {
+        bad |= part[n].bad != 0;
+        const float f = TAIL ? 1.0f : part[n].mass != 0.0f ? expf(part[n].top - top) : 0.0f;
+        mass = fmaf(part[n].mass, f, mass);
+        if constexpr (TAIL) {
+            s = join<false, S1>(s, part[n].s, a.c);
+            left += part[n].left;
+        }
+    }
+    const float h = shift_of(s.m);
+    const float inv_mass = TAIL ? 1.0f : mass != 0.0f ? 1.0f / mass : 0.0f;  // NaN stays
+    left = 1.0 - left;
+    const float q_rest = !TAIL || left < 0.0 ? 0.0f : (float)left;  // NaN stays
+    const float Q = TAIL ? (left < 0.0 ? mass : 1.0f + 0.0f * q_rest) : mass != 0.0f ? 1.0f + 0.0f * mass : 0.0f;
+    r.c = a.c;
+    r.h1 = h;
+    r.top = top;
+    const float s1 = S1 ? s.s1 : s.s;
+    {
+        const float log_s = logf(s.s);
+        // sum q (ln q - (z - h) / tau), then + sum q (ln s)
+        float kl = 0.0f, used = 0.0f;
+        for (int n = 0; n < parts; ++n) {
+            if (part[n].mass == 0.0f) continue;
+            const float f = TAIL ? 1.0f : expf(part[n].top - top);
+            if (f == 0.0f) continue;
+            const float q = part[n].mass * f * inv_mass;
+            kl += part[n].cross * f * inv_mass + q * ((TAIL ? 0.0f : part[n].top - top) - (part[n].base - h) / a.tau);
+            used += q;
+        }
+        if (used != 0.0f) kl += used * (s.s == 0.0f ? INFINITY : log_s - (TAIL ? 0.0f : logf(mass)));
+        const float hr = shift_of(rest.m);
+        if (TAIL && q_rest != 0.0f)
+            kl += rest.s == 0.0f ? (q_rest != q_rest ? NAN : INFINITY)
+                                 : q_rest * (logf(q_rest) - ((hr - h) / a.tau + logf(rest.s) - log_s));
+        r.loss = a.alpha == 0.0f ? 0.0f : a.alpha * a.tau * a.tau * kl;
+        if (a.hard) {
+            r.loss -= (1.0f - a.alpha) * (s1 == 0.0f ? -INFINITY : z_t - h - logf(s1));
+            bad |= z_t != z_t;
+        }
+        if (bad) r.loss = NAN;
+    }
+    if (gradient) {
         float w = a.scale * (a.scale_p ? *a.scale_p : 1.0f) * (a.g ? a.g[a.g_rows ? row : 0] : 1.0f);
-        if (r.bad) w = NAN;
+        if (bad) w = NAN;
         const float soft = w * a.alpha * a.tau, hard = a.hard ? w * (1.0f - a.alpha) : 0.0f;
         const float inv = s.s == 0.0f ? 0.0f : 1.0f / s.s, inv1 = s1 == 0.0f ? 0.0f : 1.0f / s1;
-        r.w = soft;
-        r.w_hard = hard;
-        r.h1 = h;
-        r.coef1 = two ? hard * inv1 : 0.0f;
-        r.inside = soft * r.Q * inv + (two ? 0.0f : hard * inv);
-        if (a.tail) {
+        r.soft = soft * inv_mass;
+        r.hard = hard;
+        r.coef1 = S1 ? hard * inv1 : 0.0f;
+        r.inside = soft * Q * inv + (S1 ? 0.0f : hard * inv);
+        if constexpr (TAIL) {
             const float f = exp2_approx(exponent(rest.m, h, a.c));
-            r.h = hr;
-            r.coef = rest.s == 0.0f ? 0.0f * w : f * r.inside - soft * r.rest / rest.s;
+            r.h = shift_of(rest.m);
+            r.coef = rest.s == 0.0f ? 0.0f * w : f * r.inside - soft * q_rest / rest.s;
         } else {
             r.h = h;
             r.coef = r.inside;
         }
     }
-    return loss;
+    return r;
 }
 
-struct DistillGrad {
-    float h, coef, h1, coef1, c;
-    __device__ __forceinline__ explicit DistillGrad(const DistillRow& r, float c_)
-        : h(r.h), coef(r.coef), h1(r.h1), coef1(r.coef1), c(c_) {}
-    template <bool S1>
-    __device__ __forceinline__ float at(float z) const {
-        float y = exp2_approx((z - h) * c) * coef;
-        if constexpr (S1) y = fmaf(exp2_approx((z - h1) * 1.44269504088896341f), coef1, y);
-        return y;
+// The gradient at slot q's token (q == k: at the target) of logit z, written by the first slot
+// that names it.  index, logprob: the row's k slots, index[k] the target or -1.
+template <class T, bool TAIL, bool S1>
+__device__ __forceinline__ void distill_grad_slot(const DistillRow& r, const int* index, const float* logprob, int k,
+                                                  int q, const T* zr, T* dr) {
+    const int j = index[q];
+    bool first = true;
+    for (int n = 0; n < q; ++n) first &= index[n] != j;
+    if (!first) return;
+    const float z = to_float(zr[j]);
+    float y;
+    if (q < k) {
+        float weight = 0.0f;
+        for (int n = q; n < k; ++n)
+            if (index[n] == j) weight += slot_weight<TAIL>(logprob[n], r.top);
+        y = r.template at_slot<S1>(z, weight);
+    } else {
+        y = r.template at<S1>(z);
     }
-};
+    if (index[k] == j) y -= r.hard;
+    dr[j] = from_float<T>(y);
+}
 
-// the slots and the target in logits j0 .. j1 - 1, after the others' gradient was written
-template <class T, bool S1>
-__device__ __forceinline__ void distill_grad_slots(const DistillArgs& a, const DistillRow& r, const T* zr, T* dr, int j0,
-                                                   int j1, int tid, int threads) {
-    const DistillGrad g(r, a.c);
-    for (int i = tid; i <= a.k; i += threads) {
-        const int j = r.index[i];
-        if (j < j0 || j >= j1) continue;
-        bool first = true;
-        for (int n = 0; n < i; ++n) first &= r.index[n] != j;
-        if (!first) continue;
-        float q = 0.0f;  // all that is taken off at j, in the order of the slots
-        for (int n = i; n < a.k; ++n)
-            if (r.index[n] == j) q += r.q[n];
-        const float z = to_float(zr[j]);
-        float y;
-        if (i < a.k) {
-            y = fmaf(exp2_approx((z - r.h1) * a.c), r.inside, -r.w * q);
-            if constexpr (S1) y = fmaf(exp2_approx((z - r.h1) * 1.44269504088896341f), r.coef1, y);
-        } else {
-            y = g.template at<S1>(z);
-        }
-        if (r.index[a.k] == j) y -= r.w_hard;
-        dr[j] = from_float<T>(y);
+// A slot as it stands in memory; false: its index is beyond the vocabulary
+__device__ __forceinline__ bool read_slot(const DistillArgs& a, int64_t at, int& j, float& l) {
+    const int64_t x = a.index[at];
+    j = x >= 0 && x < a.V ? (int)x : -1;
+    l = j >= 0 ? a.logprob[at] : -INFINITY;
+    return x < a.V;
+}
+
+// The rows' losses of a CTA are added up; the last CTA adds up the CTAs', in their order.
+__device__ __forceinline__ void distill_total(const DistillArgs& a, float sum, float* shared, int threads) {
+    if (!a.loss || a.each) return;
+    __shared__ bool last;
+    if (threadIdx.x == 0) {
+        a.partial[blockIdx.x] = sum;
+        __threadfence();
+        last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    float v = 0.0f;
+    for (uint32_t i = threadIdx.x; i < gridDim.x; i += threads) v += __ldcg(a.partial + i);
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        v = warp_sum(threadIdx.x < (threads >> 5) ? shared[threadIdx.x] : 0.0f);
+        if (threadIdx.x == 0) *a.loss = v * a.scale * (a.scale_p ? *a.scale_p : 1.0f);
     }
 }
 
@@ -250,39 +264,64 @@ __device__ __forceinline__ void distill_grad_slots(const DistillArgs& a, const D
 template <int DT, int E, bool TAIL, bool S1>
 __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
     using T = typename Elem<DT>::type;
+    constexpr int kPer = kMaxTop / 32;
     if (a.skip_if_one && *a.g == 1.0f) return;
-    __shared__ DistillRow rows[8];
+    __shared__ int index[8][kMaxTop + 1];
+    __shared__ float logprob[8][kMaxTop], total[8];
     __shared__ uint32_t named[8][TAIL ? 32 : 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float c1 = 1.44269504088896341f;
-    DistillRow& r = rows[warp];
+    const int used = (a.k + 31) / 32;
+    int* idx = index[warp];
+    float sum = 0.0f;
     for (uint32_t row = blockIdx.x * 8 + warp; row < a.N; row += gridDim.x * 8) {
         const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : 0;
-        T* dr = a.d.p ? reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row) : nullptr;
-        if (a.tok.p && t == a.tok.ignore) {
-            if (dr)
-                for (int j = lane; j < a.V; j += 32) dr[j] = from_float<T>(0.0f);
-            if (a.loss && lane == 0) a.loss[row] = 0.0f;
-            continue;
-        }
         const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
+        T* dr = a.d.p ? reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row) : nullptr;
         float x[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int j = lane + 32 * e;
             x[e] = j < a.V ? to_float(zr[j]) : -INFINITY;
         }
-        distill_slots<DT>(a, row, zr, t, r);
+        Slot slot[kPer];
+        bool bad = false;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+            slot[q] = Slot{-1, -INFINITY, -INFINITY};
+            if (lane + 32 * q < a.k)
+                bad |= !read_slot(a, (int64_t)row * a.k + lane + 32 * q, slot[q].j, slot[q].l);
+        }
+        if (a.tok.p && t == a.tok.ignore) {
+            if (dr)
+                for (int j = lane; j < a.V; j += 32) dr[j] = from_float<T>(0.0f);
+            if (a.loss && a.each && lane == 0) a.loss[row] = 0.0f;
+            continue;
+        }
+        const bool in = a.hard && t >= 0 && t < a.V;
+        const float z_t = in ? to_float(zr[t]) : NAN;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+            if (slot[q].j >= 0) slot[q].z = to_float(zr[slot[q].j]);
+            const int i = lane + 32 * q;
+            if (i < a.k) idx[i] = slot[q].j, logprob[warp][i] = slot[q].l;
+        }
+        if (lane == 0) idx[a.k] = in ? (int)t : -1;
+        if constexpr (TAIL) named[warp][lane] = 0;
+        __syncwarp();
+        bool firsts[kPer];
+        if constexpr (TAIL) {
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) {
+                const uint32_t bit = 1u << (slot[q].j & 31);
+                firsts[q] = slot[q].j >= 0 && !(atomicOr(&named[warp][slot[q].j >> 5], bit) & bit);
+            }
+            __syncwarp();
+        }
+        const SlotSums slots =
+            slot_sums<TAIL, S1, kPer>(a, slot, used, bad, [&](int q) { return TAIL ? firsts[q] : true; });
         Sums s = no_sums();
         {
             float y[E], cm = -INFINITY;
-            if constexpr (TAIL) {
-                named[warp][lane] = 0;
-                __syncwarp();
-                for (int i = lane; i < a.k; i += 32)
-                    if (r.index[i] >= 0) atomicOr(&named[warp][r.index[i] >> 5], 1u << (r.index[i] & 31));
-                __syncwarp();
-            }
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 y[e] = x[e];
@@ -290,25 +329,34 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
                     if (named[warp][e] >> lane & 1u) y[e] = -INFINITY;
                 cm = fmaxf(cm, y[e]);
             }
-            add_values<E, false, S1>(s, y, cm, a.c, c1);
+            s.m = warp_max(cm);
+            add_values<E, false, S1>(s, y, s.m, a.c);
+            s.s = warp_sum(s.s);
+            if constexpr (S1) s.s1 = warp_sum(s.s1);
         }
-        s = warp_join<false, S1>(s, a.c, c1);
-        if (lane == 0) {
-            const float loss = distill_row(a, row, s, r);
-            if (a.loss) a.loss[row] = loss;
-        }
-        __syncwarp();
+        const DistillRow r = distill_row<TAIL, S1>(a, row, s, &slots, 1, z_t, dr != nullptr);
+        sum += r.loss;
+        if (a.loss && a.each && lane == 0) a.loss[row] = r.loss;
         if (dr) {
-            const DistillGrad g(r, a.c);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int j = lane + 32 * e;
-                if (j < a.V) dr[j] = from_float<T>(g.template at<S1>(x[e]));
+                if (j < a.V) dr[j] = from_float<T>(r.template at<S1>(x[e]));
             }
             __syncwarp();
-            distill_grad_slots<T, S1>(a, r, zr, dr, 0, a.V, lane, 32);
+            for (int q = lane; q <= a.k; q += 32)
+                if (idx[q] >= 0) distill_grad_slot<T, TAIL, S1>(r, idx, logprob[warp], a.k, q, zr, dr);
         }
         __syncwarp();
+    }
+    if (a.loss && !a.each) {
+        __syncthreads();
+        if (lane == 0) total[warp] = sum;
+        __syncthreads();
+        float v = 0.0f;
+        for (int w = 0; w < 8; ++w) v += total[w];
+        __syncthreads();
+        distill_total(a, v, total, 256);
     }
 }
 
@@ -317,157 +365,193 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
 // words of the bitmap of a part of a row: its vectors' logits, 8 of the head, 8 of the tail
 __host__ __device__ constexpr int distill_words(int V, int ctas) { return (V / ctas + 8 + 31) / 32 + 2; }
 
-template <int DT, bool TAIL, bool S1>
+constexpr int kDistillStages = 5;
+
+template <int DT, bool TAIL, bool S1, bool GRAD>
 __global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs a, uint32_t ctas) {
     using T = typename Elem<DT>::type;
-    constexpr int kVec = Elem<DT>::kVec, kU = kRowElems / kVec;
+    using Stream = RowStream<DT, GRAD ? 2 : 1, kDistillStages>;
+    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems;
     if (a.skip_if_one && *a.g == 1.0f) return;
-    extern __shared__ uint32_t named[];  // [distill_words]
-    __shared__ DistillRow r;
-    __shared__ Sums part[kRowThreads / 32];
-    __shared__ __align__(16) Sums mine[2];
+    extern __shared__ __align__(16) unsigned char sm[];  // the stream's places, the bitmap
+    uint32_t* named = reinterpret_cast<uint32_t*>(sm + Stream::kBytes);
+    __shared__ float4 part[2][kRowWarps], mine[2];
+    __shared__ SlotSums slots[2][kMaxTop / 32];
+    __shared__ int index[2][kMaxTop + 1];
+    __shared__ float logprob[2][kMaxTop], total[kRowWarps];
     const int tid = threadIdx.x;
     const uint32_t rank = blockIdx.x % ctas;
-    const float c1 = 1.44269504088896341f;
+    const int slot_warps = (a.k + 31) / 32;
     if constexpr (TAIL) {
         for (int i = tid; i < distill_words(a.V, ctas); i += kRowThreads) named[i] = 0;
         __syncthreads();
     }
+    RowList list(a.tok, a.z.T, a.N, blockIdx.x / ctas, gridDim.x / ctas);
+    Stream stream(a.z, a.V, list, rank, ctas, sm);
     int parity = 0;
-    for (uint32_t row = blockIdx.x / ctas; row < a.N; row += gridDim.x / ctas) {
-        const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : 0;
-        const bool live = !(a.tok.p && t == a.tok.ignore);
+    float sum = 0.0f;
+    // a slot of the next row, read while this one's logits go by
+    Slot next{-1, -INFINITY, -INFINITY};
+    bool next_ok = true;
+    auto read_ahead = [&](uint32_t i) {
+        if (tid < a.k && i < list.count) next_ok = read_slot(a, (int64_t)list.row(i) * a.k + tid, next.j, next.l);
+    };
+    read_ahead(0);
+    for (uint32_t i = 0; i < list.count; ++i) {
+        if ((i & 31) == 0) list.window(i);
+        const uint32_t row = list.row(i);
+        const bool live = list.live(i);
         const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
-        T* dr = a.d.p ? reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row) : nullptr;
+        T* dr = GRAD ? reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row) : nullptr;
         const Segment g = segment_of<DT>(zr, a.V, rank, ctas);
-        const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
         const bool wide = (((uintptr_t)zr ^ (uintptr_t)dr) & 15u) == 0;  // 16-byte stores
-        if (live) {
-            // bit of a logit of this part: vectors first, then head and tail
-            auto bit_of = [&](int j) {
-                const int body_bits = (g.v1 - g.v0) * kVec;
-                return j < g.h0 ? body_bits + j : j >= g.t0 ? body_bits + 8 + (j - g.t0) : j - g.h0 - g.v0 * kVec;
-            };
-            if (tid < 32) {
-                distill_slots<DT>(a, row, zr, t, r);
-                if constexpr (TAIL) {
-                    for (int i = tid; i < a.k; i += 32)
-                        if (r.index[i] >= g.j0 && r.index[i] < g.j1) {
-                            const int b = bit_of(r.index[i]);
-                            atomicOr(&named[b >> 5], 1u << (b & 31));
-                        }
+        const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
+        Slot slot[1] = {next};
+        const bool ok = next_ok;
+        read_ahead(i + 1);
+        if (!live) {
+            if (a.loss && a.each && rank == 0 && tid == 0) a.loss[row] = 0.0f;
+            if constexpr (GRAD) {
+                if (wide) {
+                    uint4* to = reinterpret_cast<uint4*>(dr + g.h0);
+                    for (int v = g.v0 + tid; v < g.v1; v += kRowThreads) __stcs(to + v, make_uint4(0, 0, 0, 0));
+                    if (tid < ends) dr[end_at] = from_float<T>(0.0f);
+                } else {
+                    for (int j = g.j0 + tid; j < g.j1; j += kRowThreads) dr[j] = from_float<T>(0.0f);
                 }
             }
-            if constexpr (TAIL) __syncthreads();
-            auto is_named = [&](int b) { return (named[b >> 5] >> (b & 31) & 1u) != 0; };
-            Sums s = no_sums();
-            for (int v = g.v0; v < g.v1; v += kU * kRowThreads) {
-                float x[kRowElems];
+            continue;
+        }
+        int64_t t = -1;
+        float z_t = 0.0f;
+        if (a.hard) {
+            t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
+            z_t = t >= 0 && t < a.V ? to_float(zr[t]) : NAN;
+        }
+        const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
+        int* idx = index[parity];
+        if (tid < a.k) {
+            if (slot[0].j >= 0) slot[0].z = to_float(zr[slot[0].j]);
+            idx[tid] = slot[0].j;
+            logprob[parity][tid] = slot[0].l;
+        }
+        if (tid == 0) idx[a.k] = z_t == z_t && a.hard ? (int)t : -1;
+        // bit of a logit of this part: vectors first, then head and tail
+        auto bit_of = [&](int j) {
+            const int body = (g.v1 - g.v0) * kVec;
+            return j < g.h0 ? body + j : j >= g.t0 ? body + 8 + (j - g.t0) : j - g.h0 - g.v0 * kVec;
+        };
+        if constexpr (TAIL) {
+            if (tid < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) {
+                const int b = bit_of(slot[0].j);
+                atomicOr(&named[b >> 5], 1u << (b & 31));
+            }
+            __syncthreads();
+        }
+        if (tid < 32 * slot_warps) {
+            const SlotSums x = slot_sums<TAIL, S1, 1>(a, slot, 1, tid < a.k && !ok, [&](int) {
+                bool first = true;
+                for (int n = 0; n < tid; ++n) first &= idx[n] != slot[0].j;
+                return first;
+            });
+            if ((tid & 31) == 0) slots[parity][tid >> 5] = x;
+        }
+        Sums s = no_sums();
+        for (int v = g.v0; v < g.v1; v += Stream::kStep) {
+            uint4 raw[kU];
+            stream.take(raw, v, g.v1);
+            float x[kElems];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                unpack16<DT>(raw[u], x + u * kVec);
+                if constexpr (TAIL) {
+                    const int w = v + tid + u * kRowThreads;
+                    const int b = w < g.v1 ? (w - g.v0) * kVec : 0;
+                    const uint32_t bits = named[b >> 5] >> (b & 31) & ((1u << kVec) - 1u);
+                    if (bits) {
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e)
+                            if (bits >> e & 1u) x[u * kVec + e] = -INFINITY;
+                    }
+                }
+            }
+            stream.issue();
+            float cm = x[0];
+#pragma unroll
+            for (int e = 1; e < kElems; ++e) cm = fmaxf(cm, x[e]);
+            cm = fmaxf(cm, -INFINITY);  // all NaN
+            add_values<kElems, false, S1>(s, x, cm, a.c);
+        }
+        if (tid < ends) {
+            float x[1] = {end};
+            if constexpr (TAIL) {
+                const int b = bit_of(end_at);
+                if (named[b >> 5] >> (b & 31) & 1u) x[0] = -INFINITY;
+            }
+            add_values<1, false, S1>(s, x, x[0], a.c);
+        }
+        s = cta_join<false, S1>(s, part[parity], a.c);
+        if constexpr (TAIL) {
+            // all of the CTA have read the bitmap
+            if (tid < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) named[bit_of(slot[0].j) >> 5] = 0;
+        }
+        if (ctas > 1) s = cluster_join<false, S1>(s, &mine[parity], ctas, a.c);
+        const DistillRow r = distill_row<TAIL, S1>(a, row, s, slots[parity], slot_warps, z_t, GRAD);
+        if (rank == 0) sum += r.loss;
+        if (a.loss && a.each && rank == 0 && tid == 0) a.loss[row] = r.loss;
+        if constexpr (GRAD) {
+            for (int v = g.v0; v < g.v1; v += Stream::kStep) {
+                uint4 raw[kU];
+                stream.take(raw, v, g.v1);
+                float x[kElems];
+#pragma unroll
+                for (int u = 0; u < kU; ++u) unpack16<DT>(raw[u], x + u * kVec);
+                stream.issue();
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) x[e] = r.template at<S1>(x[e]);
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
                     const int w = v + tid + u * kRowThreads;
-                    unpack16<DT>(w < g.v1 ? __ldg(body + w) : neg_inf16<DT>(), x + u * kVec);
-                    if constexpr (TAIL) {
-                        if (w < g.v1) {
-                            const int b = (w - g.v0) * kVec;
-                            const uint32_t bits = named[b >> 5] >> (b & 31) & ((1u << kVec) - 1u);
-                            if (bits) {
+                    if (w >= g.v1) continue;
+                    T* to = dr + g.h0 + (int64_t)w * kVec;
+                    if (wide) {
+                        __stcs(reinterpret_cast<uint4*>(to), pack16<DT>(x + u * kVec));
+                    } else {
 #pragma unroll
-                                for (int e = 0; e < kVec; ++e)
-                                    if (bits >> e & 1u) x[u * kVec + e] = -INFINITY;
-                            }
-                        }
+                        for (int e = 0; e < kVec; ++e) to[e] = from_float<T>(x[u * kVec + e]);
                     }
                 }
-                float cm = x[0];
-#pragma unroll
-                for (int i = 1; i < kRowElems; ++i) cm = fmaxf(cm, x[i]);
-                add_values<kRowElems, false, S1>(s, x, cm, a.c, c1);
             }
-            if (tid < g.head + g.tail) {
-                const int j = tid < g.head ? tid : g.t0 + (tid - g.head);
-                float x[1] = {to_float(zr[j])};
-                if constexpr (TAIL)
-                    if (is_named(bit_of(j))) x[0] = -INFINITY;
-                add_values<1, false, S1>(s, x, x[0], a.c, c1);
-            }
-            s = cta_join<kRowThreads, false, S1>(s, part, a.c, c1);
-            if (ctas > 1) {
-                s = cluster_join<false, S1>(s, &mine[parity], ctas, a.c, c1);
-                parity ^= 1;
-            }
-            if (tid == 0) {
-                const float loss = distill_row(a, row, s, r);
-                if (a.loss && rank == 0) a.loss[row] = loss;
-            }
-            if constexpr (TAIL) {
-                if (tid < 32)
-                    for (int i = tid; i < a.k; i += 32)
-                        if (r.index[i] >= g.j0 && r.index[i] < g.j1) named[bit_of(r.index[i]) >> 5] = 0;
-            }
+            if (tid < ends) dr[end_at] = from_float<T>(r.template at<S1>(end));
             __syncthreads();
-        } else if (a.loss && rank == 0 && tid == 0) {
-            a.loss[row] = 0.0f;
+            if (tid <= a.k && idx[tid] >= g.j0 && idx[tid] < g.j1)
+                distill_grad_slot<T, TAIL, S1>(r, idx, logprob[parity], a.k, tid, zr, dr);
+        } else if constexpr (TAIL) {
+            __syncthreads();  // the bitmap is clear
         }
-        if (dr) {
-            const DistillGrad gr(r, a.c);
-            for (int v = g.v0 + tid; v < g.v1; v += kRowThreads) {
-                float y[kVec];
-                if (live) {
-                    float x[kVec];
-                    unpack16<DT>(__ldg(body + v), x);
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) y[e] = gr.template at<S1>(x[e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) y[e] = 0.0f;
-                }
-                T* to = dr + g.h0 + (int64_t)v * kVec;
-                if (wide) {
-                    __stcs(reinterpret_cast<uint4*>(to), pack16<DT>(y));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) to[e] = from_float<T>(y[e]);
-                }
-            }
-            if (tid < g.head + g.tail) {
-                const int j = tid < g.head ? tid : g.t0 + (tid - g.head);
-                dr[j] = from_float<T>(live ? gr.template at<S1>(to_float(zr[j])) : 0.0f);
-            }
-            __syncthreads();
-            if (live) distill_grad_slots<T, S1>(a, r, zr, dr, g.j0, g.j1, tid, kRowThreads);
-        }
-        __syncthreads();  // r is written again for the next row
+        parity ^= 1;
     }
     if (ctas > 1) cluster_sync();  // no CTA ends while another may still read its shared memory
+    __syncthreads();
+    distill_total(a, sum, total, kRowThreads);
 }
 
-// ws[0] = 1 / (rows that are not padding, at least 1); one CTA of 1024 threads
-__global__ void __launch_bounds__(1024) distill_count_kernel(Tokens tok, uint32_t T, uint32_t N, float* ws) {
+// ws[0] = 1 / (rows that are not padding, at least 1), ws[1]: the ticket, 0; one CTA of 1024 threads
+__global__ void __launch_bounds__(1024) distill_begin_kernel(Tokens tok, uint32_t T, uint32_t N, float* ws) {
     __shared__ int part[32];
     int n = 0;
-    for (uint32_t row = threadIdx.x; row < N; row += 1024) n += tok.p[row_offset(tok.sb, tok.st, T, row)] != tok.ignore;
+    if (tok.p)
+        for (uint32_t row = threadIdx.x; row < N; row += 1024)
+            n += tok.p[row_offset(tok.sb, tok.st, T, row)] != tok.ignore;
     n = __reduce_add_sync(0xffffffffu, n);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = n;
     __syncthreads();
     if (threadIdx.x < 32) {
         n = __reduce_add_sync(0xffffffffu, part[threadIdx.x]);
-        if (threadIdx.x == 0) ws[0] = 1.0f / (float)(n > 1 ? n : 1);
-    }
-}
-
-// loss = scale * (*scale_p) * sum of the rows' losses, in a fixed order; one CTA of 1024 threads
-__global__ void __launch_bounds__(1024) distill_total_kernel(const float* rows, uint32_t N, float scale,
-                                                             const float* scale_p, float* loss) {
-    __shared__ float part[32];
-    float v = 0.0f;
-    for (uint32_t row = threadIdx.x; row < N; row += 1024) v += rows[row];
-    v = warp_sum(v);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        v = warp_sum(part[threadIdx.x]);
-        if (threadIdx.x == 0) *loss = v * scale * (scale_p ? *scale_p : 1.0f);
+        if (threadIdx.x == 0) {
+            ws[0] = 1.0f / (float)(n > 1 ? n : 1);
+            reinterpret_cast<uint32_t*>(ws)[1] = 0;
+        }
     }
 }
 

@@ -13,7 +13,9 @@ namespace {
 
 using namespace il;
 
-constexpr double kLog2e = 1.4426950408889634074;
+constexpr double kLog2e64 = 1.4426950408889634074;
+constexpr double kRowCost = 16384;
+constexpr int64_t kMaxGrid = 8192;  // CTAs of a kernel that adds up a whole loss
 
 // how a [B, T, V] operand is cut up
 struct Plan {
@@ -34,7 +36,11 @@ int check_rows(int dtype, int64_t B, int64_t T, int64_t V, double temperature) {
 // the row stride of the operands and their element size: natural alignment of the base is all that is asked
 int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_BF16 ? 1u : 3u)) ? IL_ERR_ALIGN : IL_OK; }
 
-Plan plan_rows(int64_t N, int64_t V, int sms) {
+// The CTAs of a row: those that take the shortest time by a simple count, in which a
+// cluster of c CTAs has 1/c of a row to load and what a row costs beside its logits
+// (its slots, joining its sums, its list of alternatives) counts as kRowCost bytes,
+// more in a cluster.
+Plan plan_rows(int64_t N, int64_t V, int dtype, int sms) {
     Plan p{0, 1, 0};
     if (V <= kWarpVocab) {
         p.regs = (int)((V + 31) / 32);
@@ -42,10 +48,18 @@ Plan plan_rows(int64_t N, int64_t V, int sms) {
         p.grid = (unsigned)(blocks < most ? blocks : most);
         return p;
     }
-    while (p.ctas < kMaxCluster && ((int64_t)N * p.ctas < sms && V / (2 * p.ctas) >= 4096)) p.ctas *= 2;
-    while (p.ctas < kMaxCluster && V / p.ctas > (1 << 18)) p.ctas *= 2;
-    const int64_t rows = N < (1 << 20) ? N : (1 << 20);
-    p.grid = (unsigned)(rows * p.ctas);
+    const double bytes = (double)V * (dtype == IL_BF16 ? 2 : 4);
+    double best = 0.0;
+    for (int c = 1; c <= kMaxCluster; c *= 2) {
+        const int64_t clusters = 2 * (int64_t)sms / c;
+        if (c > 1 && bytes / c < 8192) break;  // less than half a step of the CTA's threads
+        const double time = (double)((N + clusters - 1) / clusters) * (bytes / c + (c > 1 ? 2.0 : 1.0) * kRowCost);
+        if (V / c <= (1 << 18) && (best == 0.0 || time < best)) {
+            best = time;
+            p.ctas = c;
+            p.grid = (unsigned)((N < clusters ? N : clusters) * c);
+        }
+    }
     return p;
 }
 
@@ -117,10 +131,10 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
     a.z = RowsIn{logits, stride_b, stride_t, (uint32_t)T};
     a.tok = Tokens{tokens, tokens_b, tokens_t, ignore_index};
     a.N = (uint32_t)(B * T), a.V = (int)V, a.k = (int)k;
-    a.tau = (float)temperature, a.c = (float)(kLog2e / temperature);
+    a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.logprob = tokens ? logprob : nullptr, a.entropy = entropy, a.stats = reinterpret_cast<float2*>(stats);
     a.top_index = top_index, a.top_logprob = top_logprob;
-    const Plan p = plan_rows(a.N, V, sms);
+    const Plan p = plan_rows(a.N, V, dtype, sms);
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
@@ -128,7 +142,8 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
                 return launch(score_warp_kernel<dt.value, e.value>, p.grid, 256, 1, 0, s, a);
             });
         return with_bool(k > 0, [&](auto top) {
-            const size_t smem = top.value ? 8 * (size_t)(top_list(a.k) + (p.ctas > 1 ? top_merge(a.k) : 0)) : 0;
+            const size_t smem = RowStream<dt.value, 1, kScoreStages<top.value>>::kBytes +
+                                (top.value ? 8 * (size_t)top_list(a.k) : 0);
             return launch(score_row_kernel<dt.value, top.value>, p.grid, kRowThreads, p.ctas, smem, s, a, p.ctas);
         });
     });
@@ -155,10 +170,10 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
     a.tok = Tokens{tokens, tokens_b, tokens_t, ignore_index};
     a.d = RowsOut{dlogits, dstride_b, dstride_t, (uint32_t)T};
     a.N = (uint32_t)(B * T), a.V = (int)V, a.k = (int)k;
-    a.tau = (float)temperature, a.c = (float)(kLog2e / temperature);
+    a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.stats = reinterpret_cast<const float2*>(stats), a.entropy = entropy, a.top_index = top_index;
     a.g_logprob = g_logprob, a.g_entropy = g_entropy, a.g_top = k > 0 ? g_top : nullptr;
-    const Plan p = plan_rows(a.N, V, sms);
+    const Plan p = plan_rows(a.N, V, dtype, sms);
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
@@ -172,7 +187,7 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
     });
 }
 
-int64_t il_distill_workspace_bytes(int64_t N) { return N < 0 ? -1 : (N + 4) * 4; }
+int64_t il_distill_workspace_bytes(int64_t N) { return N < 0 ? -1 : (kMaxGrid + 4) * 4; }
 
 int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t stride_b, int64_t stride_t,
                const int64_t* top_index, const float* top_logprob, int64_t k, const int64_t* targets,
@@ -202,41 +217,38 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
     a.d = RowsOut{dlogits, dstride_b, dstride_t, (uint32_t)T};
     a.N = (uint32_t)N, a.V = (int)V, a.k = (int)k;
     a.index = top_index, a.logprob = top_logprob;
-    a.tau = (float)temperature, a.c = (float)(kLog2e / temperature), a.alpha = (float)alpha;
-    a.tail = tail != 0, a.hard = alpha < 1.0;
+    a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature), a.alpha = (float)alpha;
+    a.hard = alpha < 1.0;
     a.scale = 1.0f;
     a.g = g, a.g_rows = reduction == 0, a.skip_if_one = only_if_not_one;
-    a.loss = loss ? (whole ? ws + 4 : loss) : nullptr;
-    if (reduction == kMean) {
-        if (targets && N > 0) {
-            a.scale_p = ws;
-            if ((st = launch(distill_count_kernel, 1, 1024, 1, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
-        } else {
-            a.scale = 1.0f / (float)(N > 1 ? N : 1);
+    a.loss = loss, a.each = !whole;
+    if (whole) {
+        a.ticket = reinterpret_cast<uint32_t*>(ws) + 1, a.partial = ws + 4;
+        if (reduction == kMean) {
+            if (targets) a.scale_p = ws;
+            else a.scale = 1.0f / (float)(N > 1 ? N : 1);
         }
+        if (loss || a.scale_p)
+            if ((st = launch(distill_begin_kernel, 1, 1024, 1, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
     }
-    if (N > 0) {
-        const Plan p = plan_rows(N, V, sms);
-        const bool two = a.hard && a.tau != 1.0f;
-        st = with_dtype(dtype, [&](auto dt) {
-            return with_bool(a.tail, [&](auto tl) {
-                return with_bool(two, [&](auto s1) {
-                    if (p.regs)
-                        return with_regs(p.regs, [&](auto e) {
-                            return launch(distill_warp_kernel<dt.value, e.value, tl.value, s1.value>, p.grid, 256, 1, 0,
-                                          s, a);
-                        });
-                    const size_t smem = tl.value ? 4 * (size_t)distill_words(a.V, p.ctas) : 0;
-                    return launch(distill_row_kernel<dt.value, tl.value, s1.value>, p.grid, kRowThreads, p.ctas, smem, s,
-                                  a, p.ctas);
+    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms) : Plan{1, 1, 1};
+    const bool two = a.hard && a.tau != 1.0f;
+    return with_dtype(dtype, [&](auto dt) {
+        return with_bool(tail != 0, [&](auto tl) {
+            return with_bool(two, [&](auto s1) {
+                if (p.regs)
+                    return with_regs(p.regs, [&](auto e) {
+                        return launch(distill_warp_kernel<dt.value, e.value, tl.value, s1.value>, p.grid, 256, 1, 0, s, a);
+                    });
+                return with_bool(dlogits != nullptr, [&](auto gr) {
+                    const size_t smem = RowStream<dt.value, 1, kDistillStages>::kBytes +
+                                        (tl.value ? 4 * (size_t)distill_words(a.V, p.ctas) : 0);
+                    return launch(distill_row_kernel<dt.value, tl.value, s1.value, gr.value>, p.grid, kRowThreads, p.ctas,
+                                  smem, s, a, p.ctas);
                 });
             });
         });
-        if (st) return st;
-    }
-    if (whole && loss)
-        return launch(distill_total_kernel, 1, 1024, 1, 0, s, (const float*)(ws + 4), a.N, a.scale, a.scale_p, loss);
-    return IL_OK;
+    });
 }
 
 }  // extern "C"

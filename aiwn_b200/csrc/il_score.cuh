@@ -65,12 +65,10 @@ __device__ __forceinline__ float log_prob(float z, float m, float s, float log_s
     return s == 0.0f ? -INFINITY : (z - shift_of(m)) / tau - log_s;
 }
 
-template <int DT>
-__device__ __forceinline__ void score_write(const ScoreArgs& a, uint32_t row, const typename Elem<DT>::type* zr,
-                                            int64_t t, const Sums& r) {
+// z_t: the token's logit, NaN for a token outside the vocabulary
+__device__ __forceinline__ void score_write(const ScoreArgs& a, uint32_t row, float z_t, const Sums& r) {
     const float log_s = logf(r.s);
-    if (a.logprob)
-        a.logprob[row] = t >= 0 && t < a.V ? log_prob(to_float(zr[t]), r.m, r.s, log_s, a.tau) : NAN;
+    if (a.logprob) a.logprob[row] = z_t != z_t ? NAN : log_prob(z_t, r.m, r.s, log_s, a.tau);
     a.entropy[row] = r.s == 0.0f ? 0.0f : fmaxf(log_s - kLn2 * r.u / r.s, 0.0f) + 0.0f * r.s;
     if (a.stats) a.stats[row] = make_float2(r.m, r.s);
 }
@@ -83,59 +81,62 @@ __global__ void __launch_bounds__(256) score_warp_kernel(ScoreArgs a) {
     const int lane = threadIdx.x & 31;
     const uint32_t warps = gridDim.x * 8;
     for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < a.N; row += warps) {
-        int64_t t = 0;
-        if (a.tok.p) {
-            t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
-            if (t == a.tok.ignore) {
-                score_padding(a, row, lane, 32);
-                continue;
-            }
-        }
+        const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : 0;
         const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
         float x[E];
-        float cm = -INFINITY;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int j = lane + 32 * e;
             x[e] = j < a.V ? to_float(zr[j]) : -INFINITY;
-            cm = fmaxf(cm, x[e]);
         }
+        if (a.tok.p && t == a.tok.ignore) {
+            score_padding(a, row, lane, 32);
+            continue;
+        }
+        float best = x[0];
+#pragma unroll
+        for (int e = 1; e < E; ++e) best = fmaxf(best, x[e]);
         Sums r = no_sums();
-        add_values<E, true, false>(r, x, cm, a.c, 0.0f);
-        r = warp_join<true, false>(r, a.c, 0.0f);
-        if (lane == 0) score_write<DT>(a, row, zr, t, r);
+        r.m = warp_max(fmaxf(best, -INFINITY));
+        add_values<E, true, false>(r, x, r.m, a.c);
+        r.s = warp_sum(r.s);
+        r.u = warp_sum(r.u);
+        if (lane == 0) score_write(a, row, a.logprob && t >= 0 && t < a.V ? to_float(zr[t]) : NAN, r);
         if (a.k == 0) continue;
-        // k times the largest of the lanes' largest; keys are 0 where nothing is left
-        uint32_t key[E];
-        uint32_t best = 0;
-        int at = 0;
+        // k times the largest of the lanes' largest; what is not left is NaN, which no maximum takes
+        const float log_s = logf(r.s);
+        best = NAN;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            key[e] = lane + 32 * e < a.V ? order_key(x[e]) : 0u;
-            if (key[e] > best) best = key[e], at = e;
+            x[e] = lane + 32 * e >= a.V ? NAN : fmaxf(x[e], -INFINITY);
+            best = fmaxf(best, x[e]);
         }
-        const float log_s = logf(r.s);
-        uint32_t my_key = 0, my_index = 0;
+        float my_value = 0.0f;
+        uint32_t my_index = 0;
         for (int i = 0; i < a.k; ++i) {
-            const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-            const uint32_t mine = best == top ? (uint32_t)(lane + 32 * at) : 0xffffffffu;
+            const float top = warp_max(best);
+            uint32_t mine = 0xffffffffu;
+            if (best == top) {
+#pragma unroll
+                for (int e = E - 1; e >= 0; --e)
+                    if (x[e] == top) mine = lane + 32 * e;
+            }
             const uint32_t index = __reduce_min_sync(0xffffffffu, mine);
-            if (lane == (i & 31)) my_key = top, my_index = index;
+            if (lane == (i & 31)) my_value = top, my_index = index;
             if ((i & 31) == 31 || i == a.k - 1) {
                 const int o = (i & ~31) + lane;
                 if (o <= i) {
                     a.top_index[(int64_t)row * a.k + o] = my_index;
-                    a.top_logprob[(int64_t)row * a.k + o] = log_prob(key_value(my_key), r.m, r.s, log_s, a.tau);
+                    a.top_logprob[(int64_t)row * a.k + o] = log_prob(my_value, r.m, r.s, log_s, a.tau);
                 }
             }
             if (mine == index) {
+                best = NAN;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (e == at) key[e] = 0;
-                best = 0;
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (key[e] > best) best = key[e], at = e;
+                for (int e = 0; e < E; ++e) {
+                    if (lane + 32 * e == index) x[e] = NAN;
+                    best = fmaxf(best, x[e]);
+                }
             }
         }
     }
@@ -144,14 +145,15 @@ __global__ void __launch_bounds__(256) score_warp_kernel(ScoreArgs a) {
 // ---- longer rows: a CTA, or a cluster of CTAs, a row --------------------------------
 
 // entries of the list of candidates: k kept, 16 of each of k - 1 threads, k equal ones
-__host__ __device__ constexpr int top_list(int k) {
-    int n = 2;
-    while (n < 18 * k || n < 512) n <<= 1;
-    return n;
-}
+// and 16 of a row's ends; or k and those of 16 CTAs, sorted
 __host__ __device__ constexpr int top_merge(int k) {
     int n = 2;
     while (n < kMaxCluster * k) n <<= 1;
+    return n;
+}
+__host__ __device__ constexpr int top_list(int k) {
+    int n = 512;
+    while (n < 18 * k + 16 || n < k + top_merge(k)) n <<= 1;
     return n;
 }
 
@@ -176,7 +178,7 @@ struct Top {
     uint64_t* list;  // shared
     int* count;      // shared
     int* scan;       // shared, one entry a warp
-    int k, cap;
+    int k, cap;      // cap: 16 less than the list has room for
     float bound;     // only logits above it are candidates, once `have`
     bool have;       // k logits at or above `bound`, of lower index than any to come, are listed
     int upper;       // at least *count
@@ -282,6 +284,12 @@ struct Top {
         have = upper >= k;
     }
 
+    // a logit of the row's ends, after all others: of lower index than all of them, or of higher
+    __device__ __forceinline__ void add_end(float z, int index, bool lower) {
+        const float v = z != z ? -INFINITY : z;
+        if (!have || v > bound || (lower && v == bound)) put(v, index);
+    }
+
     // list[0 .. k - 1]: the largest, sorted; 0 where the part of the row has fewer
     __device__ __forceinline__ void finish() {
         __syncthreads();
@@ -296,96 +304,94 @@ struct Top {
     }
 };
 
+template <bool TOP>
+constexpr int kScoreStages = TOP ? 4 : 6;
+
 template <int DT, bool TOP>
 __global__ void __launch_bounds__(kRowThreads, 2) score_row_kernel(ScoreArgs a, uint32_t ctas) {
     using T = typename Elem<DT>::type;
-    constexpr int kVec = Elem<DT>::kVec, kU = kRowElems / kVec;
-    extern __shared__ uint64_t sm_list[];
-    __shared__ Sums part[kRowThreads / 32];
-    __shared__ __align__(16) Sums mine[2];
-    __shared__ int count, scan[kRowThreads / 32];
+    using Stream = RowStream<DT, 1, kScoreStages<TOP>>;
+    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems;
+    extern __shared__ __align__(16) unsigned char sm[];  // the stream's places, the list
+    __shared__ float4 part[2][kRowWarps], mine[2];
+    __shared__ int count, scan[kRowWarps];
     const int tid = threadIdx.x;
     const uint32_t rank = blockIdx.x % ctas;
     Top top;
-    top.list = sm_list, top.count = &count, top.scan = scan, top.k = a.k, top.cap = top_list(a.k);
+    top.list = reinterpret_cast<uint64_t*>(sm + Stream::kBytes);
+    top.count = &count, top.scan = scan, top.k = a.k, top.cap = top_list(a.k) - 16;
+    RowList list(a.tok, a.z.T, a.N, blockIdx.x / ctas, gridDim.x / ctas);
+    Stream stream(a.z, a.V, list, rank, ctas, sm);
     int parity = 0;
-    for (uint32_t row = blockIdx.x / ctas; row < a.N; row += gridDim.x / ctas) {
-        int64_t t = 0;
-        if (a.tok.p) {
-            t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
-            if (t == a.tok.ignore) {
-                if (rank == 0) score_padding(a, row, tid, kRowThreads);
-                continue;
-            }
+    for (uint32_t i = 0; i < list.count; ++i) {
+        if ((i & 31) == 0) list.window(i);
+        const uint32_t row = list.row(i);
+        if (!list.live(i)) {
+            if (rank == 0) score_padding(a, row, tid, kRowThreads);
+            continue;
         }
         const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
         const Segment g = segment_of<DT>(zr, a.V, rank, ctas);
-        const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
+        const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
+        const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
+        int64_t t = 0;
+        float z_t = 0.0f;
+        if (tid == 0 && a.logprob) {
+            t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
+            z_t = t >= 0 && t < a.V ? to_float(zr[t]) : NAN;
+        }
         if constexpr (TOP) {
             top.begin();
             __syncthreads();
         }
         Sums r = no_sums();
-        uint4 next[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int v = g.v0 + tid + u * kRowThreads;
-            next[u] = v < g.v1 ? __ldcs(body + v) : neg_inf16<DT>();
-        }
-        if (g.head) {
-            const float x[1] = {tid < g.head ? to_float(zr[tid]) : -INFINITY};
-            add_values<1, true, false>(r, x, x[0], a.c, 0.0f);
-            if constexpr (TOP) top.template add<1, 1>(x, x[0], tid < g.head, tid, 0);
-        }
-        for (int v = g.v0; v < g.v1; v += kU * kRowThreads) {
-            float x[kRowElems];
+        for (int v = g.v0; v < g.v1; v += Stream::kStep) {
+            uint4 raw[kU];
+            stream.take(raw, v, g.v1);
+            float x[kElems];
             uint32_t valid = 0;
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
-                unpack16<DT>(next[u], x + u * kVec);
-                const int w = v + tid + u * kRowThreads;
-                valid |= (w < g.v1 ? 1u : 0u) << u;
-                const int y = w + kU * kRowThreads;
-                next[u] = y < g.v1 ? __ldcs(body + y) : neg_inf16<DT>();
+                unpack16<DT>(raw[u], x + u * kVec);
+                valid |= (v + tid + u * kRowThreads < g.v1 ? 1u : 0u) << u;
             }
+            stream.issue();
             float cm = x[0];
 #pragma unroll
-            for (int i = 1; i < kRowElems; ++i) cm = fmaxf(cm, x[i]);
+            for (int e = 1; e < kElems; ++e) cm = fmaxf(cm, x[e]);
             cm = fmaxf(cm, -INFINITY);  // all NaN
-            add_values<kRowElems, true, false>(r, x, cm, a.c, 0.0f);
+            add_values<kElems, true, false>(r, x, cm, a.c);
             if constexpr (TOP)
                 top.template add<kU, kVec>(x, cm, valid, g.h0 + (v + tid) * kVec, kRowThreads * kVec);
         }
-        if (g.tail) {
-            const float x[1] = {tid < g.tail ? to_float(zr[g.t0 + tid]) : -INFINITY};
-            add_values<1, true, false>(r, x, x[0], a.c, 0.0f);
-            if constexpr (TOP) top.template add<1, 1>(x, x[0], tid < g.tail, g.t0 + tid, 0);
+        if (tid < ends) {
+            const float x[1] = {end};
+            add_values<1, true, false>(r, x, end, a.c);
+            if constexpr (TOP) top.add_end(end, end_at, tid < g.head);
         }
-        r = cta_join<kRowThreads, true, false>(r, part, a.c, 0.0f);
-        if (ctas > 1) {
-            r = cluster_join<true, false>(r, &mine[parity], ctas, a.c, 0.0f);
-            parity ^= 1;
-        }
-        if (rank == 0 && tid == 0) score_write<DT>(a, row, zr, t, r);
+        r = cta_join<true, false>(r, part[parity], a.c);
+        if (ctas > 1) r = cluster_join<true, false>(r, &mine[parity], ctas, a.c);
+        parity ^= 1;
+        if (rank == 0 && tid == 0) score_write(a, row, z_t, r);
         if constexpr (TOP) {
             top.finish();
-            uint64_t* best = sm_list;
+            uint64_t* best = top.list;
             if (ctas > 1) {
                 cluster_sync();
                 if (rank == 0) {
-                    best = sm_list + top.cap;
-                    for (int i = tid; i < (int)ctas * a.k; i += kRowThreads)
-                        best[i] = ld_dsmem_u64(map_to_rank(smem_addr(sm_list + i % a.k), i / a.k));
+                    best = top.list + a.k;
+                    for (int n = tid; n < (int)ctas * a.k; n += kRowThreads)
+                        best[n] = ld_dsmem_u64(map_to_rank(smem_addr(top.list + n % a.k), n / a.k));
                 }
                 cluster_sync();
                 if (rank == 0) sort_list(best, (int)ctas * a.k);
             }
             if (rank == 0) {
                 const float log_s = logf(r.s);
-                for (int i = tid; i < a.k; i += kRowThreads) {
-                    a.top_index[(int64_t)row * a.k + i] = (uint32_t)~best[i];
-                    a.top_logprob[(int64_t)row * a.k + i] =
-                        log_prob(key_value((uint32_t)(best[i] >> 32)), r.m, r.s, log_s, a.tau);
+                for (int n = tid; n < a.k; n += kRowThreads) {
+                    a.top_index[(int64_t)row * a.k + n] = (uint32_t)~best[n];
+                    a.top_logprob[(int64_t)row * a.k + n] =
+                        log_prob(key_value((uint32_t)(best[n] >> 32)), r.m, r.s, log_s, a.tau);
                 }
             }
             __syncthreads();
