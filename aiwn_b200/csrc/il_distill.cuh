@@ -118,6 +118,24 @@ struct DistillRow {
         if constexpr (S1) y = fmaf(exp2_approx((z - h1) * kLog2e), coef1, y);
         return y;
     }
+    // at() of n values, in place
+    template <bool S1, int n>
+    __device__ __forceinline__ void at_all(float (&x)[n]) const {
+        const uint64_t hh = pack2(-h, -h), cc = pack2(c, c), co = pack2(coef, coef);
+        const uint64_t hh1 = pack2(-h1, -h1), cc1 = pack2(kLog2e, kLog2e), co1 = pack2(coef1, coef1);
+#pragma unroll
+        for (int i = 0; i < n; i += 2) {
+            const uint64_t z = pack2(x[i], x[i + 1]);
+            float d, f;
+            unpack2(mul2(add2(z, hh), cc), d, f);
+            uint64_t y = mul2(pack2(exp2_approx(d), exp2_approx(f)), co);
+            if constexpr (S1) {
+                unpack2(mul2(add2(z, hh1), cc1), d, f);
+                y = fma2(pack2(exp2_approx(d), exp2_approx(f)), co1, y);
+            }
+            unpack2(y, x[i], x[i + 1]);
+        }
+    }
     template <bool S1>
     __device__ __forceinline__ float at_slot(float z, float weight) const {
         float y = fmaf(exp2_approx((z - h1) * c), inside, -soft * weight);
@@ -365,29 +383,49 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
 // words of the bitmap of a part of a row: its vectors' logits, 8 of the head, 8 of the tail
 __host__ __device__ constexpr int distill_words(int V, int ctas) { return (V / ctas + 8 + 31) / 32 + 2; }
 
-constexpr int kDistillStages = 5;
+// a vector with -inf in place of the logits whose bits are set
+template <int DT>
+__device__ __forceinline__ uint4 without(const uint4& r, uint32_t bits) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == kF32) {
+            if (bits >> i & 1u) w[i] = 0xff800000u;
+        } else {
+            if (bits >> (2 * i) & 1u) w[i] = (w[i] & 0xffff0000u) | 0xff80u;
+            if (bits >> (2 * i + 1) & 1u) w[i] = (w[i] & 0xffffu) | 0xff800000u;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
-template <int DT, bool TAIL, bool S1, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs a, uint32_t ctas) {
+constexpr int kDistillStages = 5;  // steps that are loaded ahead
+
+template <int DT, int kThreads, bool TAIL, bool S1, bool GRAD>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_row_kernel(DistillArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
-    using Stream = RowStream<DT, GRAD ? 2 : 1, kDistillStages>;
-    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems;
+    using Stream = RowStream<DT, kThreads, GRAD ? 2 : 1, kDistillStages>;
+    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems, kWarps = kThreads / 32;
     if (a.skip_if_one && *a.g == 1.0f) return;
     extern __shared__ __align__(16) unsigned char sm[];  // the stream's places, the bitmap
     uint32_t* named = reinterpret_cast<uint32_t*>(sm + Stream::kBytes);
-    __shared__ float4 part[2][kRowWarps], mine[2];
+    __shared__ float4 part[2][kWarps], mine[2];
     __shared__ SlotSums slots[2][kMaxTop / 32];
     __shared__ int index[2][kMaxTop + 1];
-    __shared__ float logprob[2][kMaxTop], total[kRowWarps];
+    __shared__ float logprob[2][kMaxTop], total[kWarps];
+    __shared__ DistillRow shared_row[2];
     const int tid = threadIdx.x;
-    const uint32_t rank = blockIdx.x % ctas;
+    const uint32_t ctas = 1u << lg, rank = blockIdx.x & (ctas - 1);
     const int slot_warps = (a.k + 31) / 32;
     if constexpr (TAIL) {
-        for (int i = tid; i < distill_words(a.V, ctas); i += kRowThreads) named[i] = 0;
+        for (int i = tid; i < distill_words(a.V, ctas); i += kThreads) named[i] = 0;
         __syncthreads();
     }
-    RowList list(a.tok, a.z.T, a.N, blockIdx.x / ctas, gridDim.x / ctas);
-    Stream stream(a.z, a.V, list, rank, ctas, sm);
+    const RowList list(a.tok, a.z.T, a.N, blockIdx.x >> lg, gridDim.x >> lg);
+    const RowStep step(a.z, gridDim.x >> lg);
+    Stream stream(a.z, a.V, list, step, rank, lg, sm);
+    RowAt at(a.z, list.first);
+    uint32_t window = 0;
     int parity = 0;
     float sum = 0.0f;
     // a slot of the next row, read while this one's logits go by
@@ -397,13 +435,13 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs
         if (tid < a.k && i < list.count) next_ok = read_slot(a, (int64_t)list.row(i) * a.k + tid, next.j, next.l);
     };
     read_ahead(0);
-    for (uint32_t i = 0; i < list.count; ++i) {
-        if ((i & 31) == 0) list.window(i);
+    for (uint32_t i = 0; i < list.count; ++i, step.move(at, a.z.T)) {
+        if ((i & 31) == 0) window = list.window(i);
         const uint32_t row = list.row(i);
-        const bool live = list.live(i);
-        const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
+        const bool live = window >> (i & 31) & 1u;
+        const T* zr = reinterpret_cast<const T*>(a.z.p) + at.off;
         T* dr = GRAD ? reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row) : nullptr;
-        const Segment g = segment_of<DT>(zr, a.V, rank, ctas);
+        const Segment g = segment_of<DT>(zr, a.V, rank, lg);
         const bool wide = (((uintptr_t)zr ^ (uintptr_t)dr) & 15u) == 0;  // 16-byte stores
         const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
         Slot slot[1] = {next};
@@ -414,10 +452,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs
             if constexpr (GRAD) {
                 if (wide) {
                     uint4* to = reinterpret_cast<uint4*>(dr + g.h0);
-                    for (int v = g.v0 + tid; v < g.v1; v += kRowThreads) __stcs(to + v, make_uint4(0, 0, 0, 0));
+                    for (int v = g.v0 + tid; v < g.v1; v += kThreads) __stcs(to + v, make_uint4(0, 0, 0, 0));
                     if (tid < ends) dr[end_at] = from_float<T>(0.0f);
                 } else {
-                    for (int j = g.j0 + tid; j < g.j1; j += kRowThreads) dr[j] = from_float<T>(0.0f);
+                    for (int j = g.j0 + tid; j < g.j1; j += kThreads) dr[j] = from_float<T>(0.0f);
                 }
             }
             continue;
@@ -460,26 +498,20 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs
         for (int v = g.v0; v < g.v1; v += Stream::kStep) {
             uint4 raw[kU];
             stream.take(raw, v, g.v1);
-            float x[kElems];
+            if constexpr (TAIL) {
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                unpack16<DT>(raw[u], x + u * kVec);
-                if constexpr (TAIL) {
-                    const int w = v + tid + u * kRowThreads;
+                for (int u = 0; u < kU; ++u) {
+                    const int w = v + tid + u * kThreads;
                     const int b = w < g.v1 ? (w - g.v0) * kVec : 0;
                     const uint32_t bits = named[b >> 5] >> (b & 31) & ((1u << kVec) - 1u);
-                    if (bits) {
-#pragma unroll
-                        for (int e = 0; e < kVec; ++e)
-                            if (bits >> e & 1u) x[u * kVec + e] = -INFINITY;
-                    }
+                    if (bits) raw[u] = without<DT>(raw[u], bits);
                 }
             }
-            stream.issue();
-            float cm = x[0];
+            float x[kElems];
 #pragma unroll
-            for (int e = 1; e < kElems; ++e) cm = fmaxf(cm, x[e]);
-            cm = fmaxf(cm, -INFINITY);  // all NaN
+            for (int u = 0; u < kU; ++u) unpack16<DT>(raw[u], x + u * kVec);
+            const float cm = max_of<DT>(raw);
+            stream.issue();
             add_values<kElems, false, S1>(s, x, cm, a.c);
         }
         if (tid < ends) {
@@ -490,16 +522,21 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs
             }
             add_values<1, false, S1>(s, x, x[0], a.c);
         }
-        s = cta_join<false, S1>(s, part[parity], a.c);
+        s = cta_join<kThreads, false, S1>(s, part[parity], a.c);
         if constexpr (TAIL) {
             // all of the CTA have read the bitmap
             if (tid < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) named[bit_of(slot[0].j) >> 5] = 0;
         }
         if (ctas > 1) s = cluster_join<false, S1>(s, &mine[parity], ctas, a.c);
-        const DistillRow r = distill_row<TAIL, S1>(a, row, s, slots[parity], slot_warps, z_t, GRAD);
-        if (rank == 0) sum += r.loss;
-        if (a.loss && a.each && rank == 0 && tid == 0) a.loss[row] = r.loss;
+        if (tid < 32) {
+            const DistillRow r = distill_row<TAIL, S1>(a, row, s, slots[parity], slot_warps, z_t, GRAD);
+            if (rank == 0) sum += r.loss;
+            if (a.loss && a.each && rank == 0 && tid == 0) a.loss[row] = r.loss;
+            if (GRAD && tid == 0) shared_row[parity] = r;
+        }
         if constexpr (GRAD) {
+            __syncthreads();
+            const DistillRow r = shared_row[parity];
             for (int v = g.v0; v < g.v1; v += Stream::kStep) {
                 uint4 raw[kU];
                 stream.take(raw, v, g.v1);
@@ -507,11 +544,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs
 #pragma unroll
                 for (int u = 0; u < kU; ++u) unpack16<DT>(raw[u], x + u * kVec);
                 stream.issue();
-#pragma unroll
-                for (int e = 0; e < kElems; ++e) x[e] = r.template at<S1>(x[e]);
+                r.template at_all<S1, kElems>(x);
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    const int w = v + tid + u * kRowThreads;
+                    const int w = v + tid + u * kThreads;
                     if (w >= g.v1) continue;
                     T* to = dr + g.h0 + (int64_t)w * kVec;
                     if (wide) {
@@ -524,8 +560,9 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs
             }
             if (tid < ends) dr[end_at] = from_float<T>(r.template at<S1>(end));
             __syncthreads();
-            if (tid <= a.k && idx[tid] >= g.j0 && idx[tid] < g.j1)
-                distill_grad_slot<T, TAIL, S1>(r, idx, logprob[parity], a.k, tid, zr, dr);
+            for (int q = tid; q <= a.k; q += kThreads)
+                if (idx[q] >= g.j0 && idx[q] < g.j1)
+                    distill_grad_slot<T, TAIL, S1>(r, idx, logprob[parity], a.k, q, zr, dr);
         } else if constexpr (TAIL) {
             __syncthreads();  // the bitmap is clear
         }
@@ -533,7 +570,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_row_kernel(DistillArgs
     }
     if (ctas > 1) cluster_sync();  // no CTA ends while another may still read its shared memory
     __syncthreads();
-    distill_total(a, sum, total, kRowThreads);
+    distill_total(a, sum, total, kThreads);
 }
 
 // ws[0] = 1 / (rows that are not padding, at least 1), ws[1]: the ticket, 0; one CTA of 1024 threads

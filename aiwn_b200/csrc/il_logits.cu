@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <stdio.h>
+#include <stdlib.h>
 
 #include "../../include/aiwn_il.h"
 #include "il_host.h"
@@ -15,12 +17,14 @@ using namespace il;
 
 constexpr double kLog2e64 = 1.4426950408889634074;
 constexpr double kRowCost = 16384;
+constexpr double kResident = 48e6;  // bytes of rows that the L2 keeps from one pass over them to the next
 constexpr int64_t kMaxGrid = 8192;  // CTAs of a kernel that adds up a whole loss
 
 // how a [B, T, V] operand is cut up
 struct Plan {
-    int regs;       // logits a lane holds, rows of one warp; 0: CTAs
-    uint32_t ctas;  // CTAs of a row
+    int regs;     // logits a lane holds, rows of one warp; 0: CTAs
+    int threads;  // of a CTA
+    uint32_t lg;  // 2^lg CTAs a row
     unsigned grid;
 };
 
@@ -36,12 +40,14 @@ int check_rows(int dtype, int64_t B, int64_t T, int64_t V, double temperature) {
 // the row stride of the operands and their element size: natural alignment of the base is all that is asked
 int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_BF16 ? 1u : 3u)) ? IL_ERR_ALIGN : IL_OK; }
 
-// The CTAs of a row: those that take the shortest time by a simple count, in which a
-// cluster of c CTAs has 1/c of a row to load and what a row costs beside its logits
-// (its slots, joining its sums, its list of alternatives) counts as kRowCost bytes,
-// more in a cluster.
-Plan plan_rows(int64_t N, int64_t V, int dtype, int sms) {
-    Plan p{0, 1, 0};
+// Rows of more than kWarpVocab logits.  1024 threads an SM, in CTAs of 512, 256 or 128: a
+// warp's share of what a row costs beside its logits is the same whatever the row's length,
+// so that shorter rows get fewer warps.  Then the CTAs of a row: those that take the
+// shortest time by a simple count, in which a cluster of c CTAs has 1/c of a row to load
+// and the rest costs as much as kRowCost bytes, twice as much in a cluster.
+// AIWN_IL_LOGITS=threads,ctas pins both where they can serve the row (for the tests).
+Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, bool twice) {
+    Plan p{0, 256, 0, 0};
     if (V <= kWarpVocab) {
         p.regs = (int)((V + 31) / 32);
         const int64_t blocks = (N + 7) / 8, most = (int64_t)sms * 8;
@@ -50,30 +56,42 @@ Plan plan_rows(int64_t N, int64_t V, int dtype, int sms) {
     }
     const double bytes = (double)V * (dtype == IL_BF16 ? 2 : 4);
     double best = 0.0;
-    for (int c = 1; c <= kMaxCluster; c *= 2) {
-        const int64_t clusters = 2 * (int64_t)sms / c;
-        if (c > 1 && bytes / c < 8192) break;  // less than half a step of the CTA's threads
-        const double time = (double)((N + clusters - 1) / clusters) * (bytes / c + (c > 1 ? 2.0 : 1.0) * kRowCost);
-        if (V / c <= (1 << 18) && (best == 0.0 || time < best)) {
-            best = time;
-            p.ctas = c;
-            p.grid = (unsigned)((N < clusters ? N : clusters) * c);
+    int threads = 0, ctas = 0;
+    const char* pin = getenv("AIWN_IL_LOGITS");
+    if (pin && sscanf(pin, "%d,%d", &threads, &ctas) != 2) threads = ctas = 0;
+    for (int t = 128; t <= 512; t *= 2)
+        for (int lg = 0; (1 << lg) <= kMaxCluster; ++lg) {
+            const int c = 1 << lg;
+            if (V / c > (1 << 18) || (threads == t && c < ctas) || (threads && threads != t)) continue;
+            if (threads && best != 0.0) break;
+            if (best != 0.0 && bytes / c < 16 * t) break;  // less than half a step of the CTA's threads
+            const int64_t clusters = (int64_t)sms * (1024 / t) / c;
+            const double rounds = (double)((N + clusters - 1) / clusters);
+            const double rate = 1.0 / (1024 / t);  // CTAs of an SM share it
+            double time = rounds * (bytes / c / rate * 1.0 + (c > 1 ? 2.0 : 1.0) * kRowCost * 2);
+            if (twice && (double)(N < clusters ? N : clusters) * bytes > kResident) time *= 1.3;
+            if (best == 0.0 || time < best) {
+                best = time;
+                p.threads = t;
+                p.lg = lg;
+                p.grid = (unsigned)((N < clusters ? N : clusters) * c);
+            }
         }
-    }
     return p;
 }
 
 template <class... P, class... A>
-int launch(void (*kern)(P...), unsigned grid, int threads, uint32_t ctas, size_t smem, cudaStream_t s, A... args) {
+int launch(void (*kern)(P...), unsigned grid, int threads, uint32_t lg, size_t smem, cudaStream_t s, A... args) {
     if (smem > 40 * 1024 &&  // beyond 48 KB with the static arrays
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
         cudaGetLastError();
         return IL_ERR_LAUNCH;
     }
-    if (ctas > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    if (lg > 3 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         cudaGetLastError();
         return IL_ERR_LAUNCH;
     }
+    const uint32_t ctas = 1u << lg;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
@@ -106,6 +124,12 @@ int with_dtype(int dtype, F f) {
     return dtype == IL_BF16 ? f(std::integral_constant<int, kBF16>()) : f(std::integral_constant<int, kF32>());
 }
 template <class F>
+int with_threads(int threads, F f) {
+    if (threads == 128) return f(std::integral_constant<int, 128>());
+    if (threads == 256) return f(std::integral_constant<int, 256>());
+    return f(std::integral_constant<int, 512>());
+}
+template <class F>
 int with_bool(bool b, F f) {
     return b ? f(std::true_type()) : f(std::false_type());
 }
@@ -134,17 +158,19 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.logprob = tokens ? logprob : nullptr, a.entropy = entropy, a.stats = reinterpret_cast<float2*>(stats);
     a.top_index = top_index, a.top_logprob = top_logprob;
-    const Plan p = plan_rows(a.N, V, dtype, sms);
+    const Plan p = plan_rows(a.N, V, dtype, sms, false);
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
             return with_regs(p.regs, [&](auto e) {
-                return launch(score_warp_kernel<dt.value, e.value>, p.grid, 256, 1, 0, s, a);
+                return launch(score_warp_kernel<dt.value, e.value>, p.grid, 256, 0, 0, s, a);
             });
         return with_bool(k > 0, [&](auto top) {
-            const size_t smem = RowStream<dt.value, 1, kScoreStages<top.value>>::kBytes +
-                                (top.value ? 8 * (size_t)top_list(a.k) : 0);
-            return launch(score_row_kernel<dt.value, top.value>, p.grid, kRowThreads, p.ctas, smem, s, a, p.ctas);
+            return with_threads(p.threads, [&](auto th) {
+                const size_t smem = RowStream<dt.value, th.value, 1, kScoreStages<top.value>>::kBytes +
+                                    (top.value ? 8 * (size_t)top_list(a.k) : 0);
+                return launch(score_row_kernel<dt.value, th.value, top.value>, p.grid, th.value, p.lg, smem, s, a, p.lg);
+            });
         });
     });
 }
@@ -173,17 +199,18 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.stats = reinterpret_cast<const float2*>(stats), a.entropy = entropy, a.top_index = top_index;
     a.g_logprob = g_logprob, a.g_entropy = g_entropy, a.g_top = k > 0 ? g_top : nullptr;
-    const Plan p = plan_rows(a.N, V, dtype, sms);
+    const Plan p = plan_rows(a.N, V, dtype, sms, false);
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
             return with_regs(p.regs, [&](auto e) {
-                return launch(score_grad_warp_kernel<dt.value, e.value>, p.grid, 256, 1, 0, s, a);
+                return launch(score_grad_warp_kernel<dt.value, e.value>, p.grid, 256, 0, 0, s, a);
             });
-        const uint32_t parts = (uint32_t)((V + 32767) / 32768);
-        const int64_t grid = (int64_t)a.N * parts;
+        uint32_t lg = 0;
+        while ((V >> lg) > 32768) ++lg;
+        const int64_t grid = (int64_t)a.N << lg;
         if (grid > 0x7fffffff) return (int)IL_ERR_SHAPE;
-        return launch(score_grad_row_kernel<dt.value>, (unsigned)grid, kRowThreads, 1, 0, s, a, parts);
+        return launch(score_grad_row_kernel<dt.value>, (unsigned)grid, kGradThreads, 0, 0, s, a, lg);
     });
 }
 
@@ -229,22 +256,24 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
             else a.scale = 1.0f / (float)(N > 1 ? N : 1);
         }
         if (loss || a.scale_p)
-            if ((st = launch(distill_begin_kernel, 1, 1024, 1, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
+            if ((st = launch(distill_begin_kernel, 1, 1024, 0, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
     }
-    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms) : Plan{1, 1, 1};
+    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits != nullptr) : Plan{1, 256, 0, 1};
     const bool two = a.hard && a.tau != 1.0f;
     return with_dtype(dtype, [&](auto dt) {
         return with_bool(tail != 0, [&](auto tl) {
             return with_bool(two, [&](auto s1) {
                 if (p.regs)
                     return with_regs(p.regs, [&](auto e) {
-                        return launch(distill_warp_kernel<dt.value, e.value, tl.value, s1.value>, p.grid, 256, 1, 0, s, a);
+                        return launch(distill_warp_kernel<dt.value, e.value, tl.value, s1.value>, p.grid, 256, 0, 0, s, a);
                     });
                 return with_bool(dlogits != nullptr, [&](auto gr) {
-                    const size_t smem = RowStream<dt.value, 1, kDistillStages>::kBytes +
-                                        (tl.value ? 4 * (size_t)distill_words(a.V, p.ctas) : 0);
-                    return launch(distill_row_kernel<dt.value, tl.value, s1.value, gr.value>, p.grid, kRowThreads, p.ctas,
-                                  smem, s, a, p.ctas);
+                    return with_threads(p.threads, [&](auto th) {
+                        const size_t smem = RowStream<dt.value, th.value, 1, kDistillStages>::kBytes +
+                                            (tl.value ? 4 * (size_t)distill_words(a.V, 1 << p.lg) : 0);
+                        return launch(distill_row_kernel<dt.value, th.value, tl.value, s1.value, gr.value>, p.grid,
+                                      th.value, p.lg, smem, s, a, p.lg);
+                    });
                 });
             });
         });

@@ -27,8 +27,6 @@ namespace il {
 constexpr int kMaxTop = 128;         // alternatives, or the teacher's slots, of a row
 constexpr int kMaxVocab = 1 << 21;   // a row split over 16 CTAs keeps its bitmap in shared memory
 constexpr int kWarpVocab = 1024;     // rows up to this long are held in one warp's registers
-constexpr int kRowThreads = 512;     // CTA of the longer rows
-constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kMaxCluster = 16;
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -52,6 +50,25 @@ __device__ __forceinline__ int64_t row_offset(int64_t sb, int64_t st, uint32_t T
     const uint32_t b = row / T;
     return (int64_t)b * sb + (int64_t)(row - b * T) * st;
 }
+
+// a row that moves on by a fixed number of rows, without a division for each
+struct RowAt {
+    uint32_t t;
+    int64_t off;
+    __device__ __forceinline__ RowAt(const RowsIn& z, uint32_t row)
+        : t(row % z.T), off(row_offset(z.sb, z.st, z.T, row)) {}
+};
+struct RowStep {
+    uint32_t t;
+    int64_t off, wrap;  // of b and t together; more where t passes T
+    __device__ __forceinline__ RowStep(const RowsIn& z, uint32_t step)
+        : t(step % z.T), off(row_offset(z.sb, z.st, z.T, step)), wrap(z.sb - (int64_t)z.T * z.st) {}
+    __device__ __forceinline__ void move(RowAt& r, uint32_t T) const {
+        r.t += t;
+        r.off += off;
+        if (r.t >= T) r.t -= T, r.off += wrap;
+    }
+};
 
 template <int DT>
 struct Elem;
@@ -128,6 +145,31 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return y;
 }
 
+// two floats in one 64-bit register pair: one instruction for both
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kMinExp = -150.0f;
 
@@ -169,33 +211,60 @@ template <int n, bool U, bool S1>
 __device__ __forceinline__ void add_values(Sums& a, const float (&x)[n], float cm, float c) {
     if (cm > a.m) a = raised<U, S1>(a, cm, c);
     const float h = shift_of(a.m);
-    float s = 0.0f, u = 0.0f, s1 = 0.0f, t = 0.0f, v = 0.0f, t1 = 0.0f;  // even and odd values
+    const uint64_t hh = pack2(-h, -h), cc = pack2(c, c), c1 = pack2(kLog2e, kLog2e);
+    uint64_t s = 0, u = 0, s1 = 0;  // of the even and of the odd values
 #pragma unroll
     for (int i = 0; i < n; i += 2) {
-        const float g = x[i] - h;
-        if constexpr (U) {
-            const float d = max_nan(g * c, kMinExp), e = exp2_approx(d);
-            s += e;
-            u = fmaf(e, d, u);
-        } else {
-            s += exp2_approx(g * c);
-        }
-        if constexpr (S1) s1 += exp2_approx(g * kLog2e);
-        if (i + 1 < n) {
-            const float g2 = x[i + 1] - h;
-            if constexpr (U) {
-                const float d = max_nan(g2 * c, kMinExp), e = exp2_approx(d);
-                t += e;
-                v = fmaf(e, d, v);
-            } else {
-                t += exp2_approx(g2 * c);
-            }
-            if constexpr (S1) t1 += exp2_approx(g2 * kLog2e);
+        const uint64_t g = add2(pack2(x[i], i + 1 < n ? x[i + 1 < n ? i + 1 : i] : -INFINITY), hh);
+        float d, f, e0, e1;
+        unpack2(mul2(g, cc), d, f);
+        if constexpr (U) d = max_nan(d, kMinExp), f = max_nan(f, kMinExp);
+        e0 = exp2_approx(d);
+        e1 = exp2_approx(f);
+        const uint64_t e = pack2(e0, e1);
+        s = i ? add2(s, e) : e;
+        if constexpr (U) u = i ? fma2(e, pack2(d, f), u) : mul2(e, pack2(d, f));
+        if constexpr (S1) {
+            unpack2(mul2(g, c1), d, f);
+            const uint64_t e = pack2(exp2_approx(d), exp2_approx(f));
+            s1 = i ? add2(s1, e) : e;
         }
     }
-    a.s += s + t;
-    if constexpr (U) a.u += u + v;
-    if constexpr (S1) a.s1 += s1 + t1;
+    float lo, hi;
+    unpack2(s, lo, hi);
+    a.s += lo + hi;
+    if constexpr (U) {
+        unpack2(u, lo, hi);
+        a.u += lo + hi;
+    }
+    if constexpr (S1) {
+        unpack2(s1, lo, hi);
+        a.s1 += lo + hi;
+    }
+}
+
+// the largest of kU 16-byte vectors' values, -inf where all are NaN
+template <int DT, int kU>
+__device__ __forceinline__ float max_of(const uint4 (&r)[kU]) {
+    if constexpr (DT == kBF16) {
+        auto word = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+        __nv_bfloat162 m = word(r[0].x);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            if (u) m = __hmax2(m, word(r[u].x));
+            m = __hmax2(m, word(r[u].y));
+            m = __hmax2(m, word(r[u].z));
+            m = __hmax2(m, word(r[u].w));
+        }
+        return fmaxf(fmaxf(__low2float(m), __high2float(m)), -INFINITY);
+    } else {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+            m = fmaxf(fmaxf(fmaxf(m, __uint_as_float(r[u].x)), fmaxf(__uint_as_float(r[u].y), __uint_as_float(r[u].z))),
+                      __uint_as_float(r[u].w));
+        return m;
+    }
 }
 
 // lanes of a warp, all lanes get the result; kLanes = 32 or 16 (lanes 0..15 hold values)
@@ -229,8 +298,9 @@ __device__ __forceinline__ Sums warp_join(Sums a, float c) {
 
 // every thread's sums -> the CTA's, in all threads.  part: shared, one entry a
 // warp, not written again before the CTA's next barrier but one.
-template <bool U, bool S1>
+template <int kThreads, bool U, bool S1>
 __device__ __forceinline__ Sums cta_join(Sums a, float4* part, float c) {
+    constexpr int kRowWarps = kThreads / 32;
     a = warp_join<U, S1>(a, c);
     const int lane = threadIdx.x & 31;
     if (lane == 0) part[threadIdx.x >> 5] = make_float4(a.m, a.s, a.u, a.s1);
@@ -270,7 +340,7 @@ __device__ __forceinline__ Sums cluster_join(Sums a, float4* mine, uint32_t ctas
     return warp_join<U, S1>(a, c);
 }
 
-// the part of a row that one of `ctas` CTAs reads: `head` logits before the
+// the part of a row that one of 2^lg CTAs reads: `head` logits before the
 // first 16-byte boundary (rank 0), 16-byte vectors v0 .. v1 - 1 from there on,
 // and `tail` logits behind the last whole vector (last rank).  Vector v starts
 // at logit h0 + v * kVec, the tail at logit t0; j0 .. j1 - 1 is the whole part.
@@ -279,44 +349,42 @@ struct Segment {
 };
 
 template <int DT>
-__device__ __forceinline__ Segment segment_of(const void* row, int V, uint32_t rank, uint32_t ctas) {
+__device__ __forceinline__ Segment segment_of(const void* row, int V, uint32_t rank, uint32_t lg) {
     constexpr int kVec = Elem<DT>::kVec, kSize = 16 / kVec;
     Segment g;
     const int mis = (int)(((uintptr_t)row & 15u) / kSize);
     g.h0 = min(V, mis ? kVec - mis : 0);
     const int nv = (V - g.h0) / kVec;
     g.t0 = g.h0 + nv * kVec;
-    g.v0 = (int)((int64_t)nv * rank / ctas);
-    g.v1 = (int)((int64_t)nv * (rank + 1) / ctas);
+    const bool last = rank + 1 == 1u << lg;
+    g.v0 = (int)(nv * rank >> lg);  // nv < 2^20, rank <= 16
+    g.v1 = (int)(nv * (rank + 1) >> lg);
     g.head = rank == 0 ? g.h0 : 0;
-    g.tail = rank == ctas - 1 ? V - g.t0 : 0;
+    g.tail = last ? V - g.t0 : 0;
     g.j0 = rank == 0 ? 0 : g.h0 + g.v0 * kVec;
-    g.j1 = rank == ctas - 1 ? V : g.h0 + g.v1 * kVec;
+    g.j1 = last ? V : g.h0 + g.v1 * kVec;
     return g;
 }
 
 // ---- rows a CTA goes through, and their 16-byte vectors ahead of time -----------------
 
-// the i-th row of a cluster (or CTA); which of 32 rows are not padding is found by one
-// load of a lane each
+// which of 32 consecutive rows of a cluster (or CTA) are not padding: a load of a lane each
 struct RowList {
     Tokens tok;
     uint32_t T, N, first, step, count;
-    uint32_t mask;  // of rows 32 (i / 32) ...
 
     __device__ __forceinline__ RowList(const Tokens& tok_, uint32_t T_, uint32_t N_, uint32_t first_, uint32_t step_)
-        : tok(tok_), T(T_), N(N_), first(first_), step(step_), mask(0xffffffffu) {
+        : tok(tok_), T(T_), N(N_), first(first_), step(step_) {
         count = first < N ? (N - first - 1) / step + 1 : 0;
     }
     __device__ __forceinline__ uint32_t row(uint32_t i) const { return first + i * step; }
-    // whole warps; call with i = 0 and then with every multiple of 32
-    __device__ __forceinline__ void window(uint32_t i) {
-        if (!tok.p) return;
+    // whole warps; i: a multiple of 32.  Bit n: row i + n
+    __device__ __forceinline__ uint32_t window(uint32_t i) const {
+        if (!tok.p) return 0xffffffffu;
         const uint32_t n = i + (threadIdx.x & 31);
         const bool live = n < count && tok.p[row_offset(tok.sb, tok.st, T, row(n))] != tok.ignore;
-        mask = __ballot_sync(0xffffffffu, live);
+        return __ballot_sync(0xffffffffu, live);
     }
-    __device__ __forceinline__ bool live(uint32_t i) const { return mask >> (i & 31) & 1u; }
 };
 
 __device__ __forceinline__ uint64_t policy_evict_first() {
@@ -324,10 +392,8 @@ __device__ __forceinline__ uint64_t policy_evict_first() {
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
     return p;
 }
-__device__ __forceinline__ uint64_t policy_evict_last() {
-    uint64_t p;
-    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
-    return p;
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, uint64_t policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
@@ -344,88 +410,96 @@ __device__ __forceinline__ void copy_wait() {
 // row's sums are joined.  Each thread copies what it will read itself into
 // places of its own (cp.async), so that no barrier is involved.  Every row is
 // gone through kPasses times; the last time its lines may leave the L2 first.
-template <int DT, int kPasses, int kStages>
+template <int DT, int kThreads, int kPasses, int kStages>
 struct RowStream {
     static constexpr int kVec = Elem<DT>::kVec, kU = 2, kElems = kU * kVec;
-    static constexpr int kStep = kU * kRowThreads;  // vectors of a step
+    static constexpr int kStep = kU * kThreads;  // vectors of a step
     static constexpr int kBytes = kStages * kStep * 16;
+    using T = typename Elem<DT>::type;
 
-    RowsIn z;
-    int V;
-    uint32_t rank, ctas;
-    RowList list;
-    uint32_t slots;  // shared address of this thread's places
-    uint32_t i;      // row being loaded
-    int pass, v, v0, v1, put, get;
+    const RowsIn& z;
+    const int V;
+    const uint32_t rank, lg;
+    const RowList& list;
+    const RowStep& step;
+    RowAt at;
+    uint32_t slots;      // shared address of this thread's places
+    uint32_t i, live;    // row being loaded, its window
+    int v, v1;           // this thread's next vector, the end
+    int left;            // passes over the row after this one
+    uint32_t put, get;   // bytes
     const uint4* body;
-    uint64_t first_time, last_time;
+    uint64_t policy;
 
-    __device__ __forceinline__ RowStream(const RowsIn& z_, int V_, const RowList& list_, uint32_t rank_, uint32_t ctas_,
-                                         void* shared)
-        : z(z_), V(V_), rank(rank_), ctas(ctas_), list(list_), i(0), pass(0), v(0), v0(0), v1(0), put(0), get(0) {
+    __device__ __forceinline__ RowStream(const RowsIn& z_, int V_, const RowList& list_, const RowStep& step_,
+                                         uint32_t rank_, uint32_t lg_, void* shared)
+        : z(z_), V(V_), rank(rank_), lg(lg_), list(list_), step(step_), at(z_, list_.first), i(0), v(0), v1(0),
+          left(0), put(0), get(0) {
         slots = smem_addr(shared) + threadIdx.x * 16;
-        last_time = policy_evict_first();
-        first_time = kPasses > 1 ? policy_evict_last() : last_time;
-        list.window(0);
+        policy = policy_evict_first();
+        live = list.window(0);
         begin_row();
-#pragma unroll
+#pragma unroll 1
         for (int n = 0; n < kStages; ++n) issue();
+    }
+
+    __device__ __forceinline__ void next_row() {
+        step.move(at, z.T);
+        if ((++i & 31) == 0 && i < list.count) live = list.window(i);
     }
 
     // to the first row from i on that has vectors to load
     __device__ __forceinline__ void begin_row() {
-        for (; i < list.count;) {
-            if (list.live(i)) {
-                const typename Elem<DT>::type* zr = reinterpret_cast<const typename Elem<DT>::type*>(z.p) +
-                                                    row_offset(z.sb, z.st, z.T, list.row(i));
-                const Segment g = segment_of<DT>(zr, V, rank, ctas);
-                if (g.v0 < g.v1) {
-                    body = reinterpret_cast<const uint4*>(zr + g.h0);
-                    v0 = g.v0, v1 = g.v1, v = g.v0;
-                    return;
-                }
-            }
-            if ((++i & 31) == 0) list.window(i);
+        for (; i < list.count; next_row()) {
+            if (!(live >> (i & 31) & 1u)) continue;
+            const T* zr = reinterpret_cast<const T*>(z.p) + at.off;
+            const Segment g = segment_of<DT>(zr, V, rank, lg);
+            if (g.v0 >= g.v1) continue;
+            body = reinterpret_cast<const uint4*>(zr + g.h0);
+            v = g.v0 + threadIdx.x, v1 = g.v1;
+            left = kPasses - 1;
+            return;
         }
     }
 
     __device__ __forceinline__ void issue() {
         if (i < list.count) {
-            const uint64_t policy = pass + 1 == kPasses ? last_time : first_time;
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int w = v + (int)threadIdx.x + u * kRowThreads;
-                if (w < v1) copy_async16(slots + (put * kU + u) * (kRowThreads * 16), body + w, policy);
-            }
+            for (int u = 0; u < kU; ++u)
+                if (v + u * kThreads < v1) {
+                    const uint32_t to = slots + put + u * (kThreads * 16);
+                    if (kPasses == 1 || left == 0) copy_async16(to, body + v + u * kThreads, policy);
+                    else copy_async16(to, body + v + u * kThreads);
+                }
             v += kStep;
-            if (v >= v1) {
-                v = v0;
-                if (++pass == kPasses) {
-                    pass = 0;
-                    if ((++i & 31) == 0) list.window(i);
+            if (v - (int)threadIdx.x >= v1) {
+                if (kPasses > 1 && left > 0) {
+                    --left;
+                    const T* zr = reinterpret_cast<const T*>(z.p) + at.off;
+                    v = segment_of<DT>(zr, V, rank, lg).v0 + threadIdx.x;
+                } else {
+                    next_row();
                     begin_row();
                 }
             }
         }
         copy_commit();
-        put = put + 1 == kStages ? 0 : put + 1;
+        put = put + kStep * 16 == kBytes ? 0 : put + kStep * 16;
     }
 
-    // the next kU vectors; valid(u) tells which of them the row has (the others are -inf)
+    // this thread's next kU vectors, -inf from `end` on; first: the step's first vector
     __device__ __forceinline__ void take(uint4 (&r)[kU], int first, int end) {
         copy_wait<kStages - 1>();
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             r[u] = neg_inf16<DT>();
-            if (first + (int)threadIdx.x + u * kRowThreads < end) {
-                const uint32_t at = slots + (get * kU + u) * (kRowThreads * 16);
+            if (first + (int)threadIdx.x + u * kThreads < end)
                 asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(r[u].x), "=r"(r[u].y), "=r"(r[u].z), "=r"(r[u].w)
-                             : "r"(at)
+                             : "r"(slots + get + u * (kThreads * 16))
                              : "memory");
-            }
         }
-        get = get + 1 == kStages ? 0 : get + 1;
+        get = get + kStep * 16 == kBytes ? 0 : get + kStep * 16;
     }
 };
 

@@ -7,18 +7,20 @@
 // with (m, s, u) of il_logits.cuh.  The forward reads each logit once, the
 // backward reads it once more and writes its gradient.
 //
-// The k largest in the same pass.  Every thread knows the maximum of the 16
-// logits that it holds.  For the row's first logits the k-th largest of the
-// threads' maxima is a lower bound of the k-th largest logit; from then on only
-// logits above the bound are put into a list in shared memory (for logits in no
-// particular order a few times k of them), so that the work on a logit that is
-// not among the largest is the comparison of its thread's maximum.  When the
-// list could run over, it is sorted and cut to k, and the bound rises to its
-// last; when one step alone could overrun it, the bound is first taken from the
-// threads' maxima again: at most (k - 1) threads then hold anything above it,
-// and of the logits equal to it the first ones by index are taken.  No input
-// needs a second pass.  List entries are (order-preserving bits of z) << 32 |
-// ~index, so that all are distinct and equal logits go by their index.
+// The k largest in the same pass.  Every thread knows the maximum of the logits
+// that it holds.  For the row's first logits the k-th largest of the threads'
+// maxima is a lower bound of the k-th largest logit; from then on only logits
+// above the bound are put into a list in shared memory, so that the work on a
+// logit that is not among the largest is the comparison of its step's maximum.
+// After 1, 2, 4, ... steps the bound rises to what the threads' maxima so far
+// say: with j = k / warps (rounded up), the least of the warps' j-th largest.
+// For logits in no particular order the list so gets a few times k entries.
+// When it could run over, it is sorted and cut to k; when one step alone could
+// overrun it, the bound is first taken from that step's maxima: at most k - 1
+// threads then hold anything above it, and of the logits equal to it the first
+// ones by index are taken.  No input needs a second pass.  List entries are
+// (order-preserving bits of z) << 32 | ~index, so that all are distinct and
+// equal logits go by their index.
 #pragma once
 #include "il_logits.cuh"
 
@@ -157,15 +159,49 @@ __host__ __device__ constexpr int top_list(int k) {
     return n;
 }
 
-// descending; n entries are in use, `list` has room up to the next power of two
+// descending; n entries are in use, `list` has room up to the next power of two.  A bitonic network; up to one
+// entry a thread, an entry stays in its thread's register and goes through shuffles where its partner is in the warp.
+template <int kThreads>
 __device__ __forceinline__ void sort_list(uint64_t* list, int n) {
     int p = 2;
     while (p < n) p <<= 1;
-    for (int i = n + threadIdx.x; i < p; i += kRowThreads) list[i] = 0;
+    const int tid = threadIdx.x;
+    if (p <= kThreads) {
+        if (tid < p && p <= 32) {  // one warp
+            const unsigned lanes = p == 32 ? 0xffffffffu : (1u << p) - 1u;
+            uint64_t x = tid < n ? list[tid] : 0;
+            for (int size = 2; size <= p; size <<= 1)
+                for (int d = size >> 1; d > 0; d >>= 1) {
+                    const uint64_t y = __shfl_xor_sync(lanes, x, d);
+                    if ((x < y) == (((tid & size) == 0) == ((tid & d) == 0))) x = y;
+                }
+            list[tid] = x;
+        } else if (p > 32) {
+            uint64_t x = tid < n ? list[tid] : 0;
+            for (int size = 2; size <= p; size <<= 1)
+                for (int d = size >> 1; d > 0; d >>= 1) {
+                    uint64_t y;
+                    if (d >= 32) {
+                        __syncthreads();
+                        if (tid < p) list[tid] = x;
+                        __syncthreads();
+                        y = tid < p ? list[tid ^ d] : x;
+                    } else {
+                        y = __shfl_xor_sync(0xffffffffu, x, d);
+                    }
+                    if ((x < y) == (((tid & size) == 0) == ((tid & d) == 0))) x = y;
+                }
+            __syncthreads();
+            if (tid < p) list[tid] = x;
+        }
+        __syncthreads();
+        return;
+    }
+    for (int i = n + tid; i < p; i += kThreads) list[i] = 0;
     __syncthreads();
     for (int size = 2; size <= p; size <<= 1)
         for (int d = size >> 1; d > 0; d >>= 1) {
-            for (int i = threadIdx.x; i < (p >> 1); i += kRowThreads) {
+            for (int i = tid; i < (p >> 1); i += kThreads) {
                 const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
                 const uint64_t x = list[lo], y = list[hi];
                 if ((x < y) == ((lo & size) == 0)) list[lo] = y, list[hi] = x;
@@ -174,19 +210,27 @@ __device__ __forceinline__ void sort_list(uint64_t* list, int n) {
         }
 }
 
+template <int DT, int kThreads, int kU>
 struct Top {
+    static constexpr int kVec = Elem<DT>::kVec, kElems = kU * kVec, kWarps = kThreads / 32;
     uint64_t* list;  // shared
     int* count;      // shared
     int* scan;       // shared, one entry a warp
+    float* deposit;  // shared, two entries a warp, in turn
     int k, cap;      // cap: 16 less than the list has room for
     float bound;     // only logits above it are candidates, once `have`
     bool have;       // k logits at or above `bound`, of lower index than any to come, are listed
     int upper;       // at least *count
+    int steps, due;  // of the row; where `deposit` is next made or read
+    int turn;
 
     __device__ __forceinline__ void begin() {  // the caller's barrier follows
         have = false;
         upper = 0;
         bound = -INFINITY;
+        steps = 0;
+        due = 1;
+        turn = 0;
         if (threadIdx.x == 0) *count = 0;
     }
 
@@ -194,50 +238,97 @@ struct Top {
         list[atomicAdd(count, 1)] = ((uint64_t)order_key(z) << 32) | (uint32_t)~index;
     }
 
-    // kU x kV values of this thread, x[u * kV + e] being logit first + u * step + e; valid: bits of u
-    template <int kU, int kV>
-    __device__ __forceinline__ void add(const float (&x)[kU * kV], float cm, uint32_t valid, int first, int step) {
-        bool want = !have || cm > bound;
-        int n = __syncthreads_count(want);
-        if (n == 0) return;
-        if (have && upper + n * (kU * kV) <= cap) {
-            upper += n * (kU * kV);
-            if (want) {
-#pragma unroll
-                for (int i = 0; i < kU * kV; ++i)
-                    if (x[i] > bound) put(x[i], first + (i / kV) * step + i % kV);
-            }
-            return;
-        }
-        raise<kU, kV>(x, cm, valid, first, step);
+    __device__ __forceinline__ static float value(const uint4 (&r)[kU], int i) {
+        const uint4& q = r[i / kVec];
+        const int e = i % kVec;
+        if constexpr (DT == kF32) return __uint_as_float(e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w);
+        const uint32_t w = e / 2 == 0 ? q.x : e / 2 == 1 ? q.y : e / 2 == 2 ? q.z : q.w;
+        return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
     }
 
-    template <int kU, int kV>
-    __device__ __forceinline__ void raise(const float (&x)[kU * kV], float cm, uint32_t valid, int first, int step) {
-        int c = *count;
-        if (c > k) {
-            sort_list(list, c);
-            c = k;
-            bound = key_value((uint32_t)(list[k - 1] >> 32));
-            have = true;
+    // this thread's values above the bound
+    __device__ __forceinline__ void put_above(const uint4 (&r)[kU], int first) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            if constexpr (DT == kBF16) {
+                const __nv_bfloat162 b = __float2bfloat162_rn(bound);  // exact: a logit
+                const uint32_t w[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t above = __hgt2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[q]), b);
+                    if (above) {
+                        const int at = first + u * kThreads * kVec + 2 * q;
+                        if (above & 0xffffu) put(__uint_as_float(w[q] << 16), at);
+                        if (above >> 16) put(__uint_as_float(w[q] & 0xffff0000u), at + 1);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const float v = value(r, u * kVec + e);
+                    if (v > bound) put(v, first + u * kThreads * kVec + e);
+                }
+            }
         }
+    }
+
+    // The row's next values: vector u of this thread, being logits first + u * kThreads * kVec + 0, 1, ..., is
+    // there if bit u of `valid` is set.  cm: their maximum, all: that of all of this thread's values so far.
+    __device__ __forceinline__ void add(const uint4 (&r)[kU], float cm, float all, uint32_t valid, int first) {
+        const int n = __syncthreads_count(!have || cm > bound);
+        ++steps;
+        if (have && steps == due + 1) {  // the deposit of the step before
+            const float b = deposit[turn + (threadIdx.x & (kWarps - 1))];
+            bound = fmaxf(bound, -warp_max(-b));
+            due *= 2;
+            turn ^= kWarps;
+        }
+        if (n != 0) {
+            if (have && upper + n * kElems <= cap) {
+                upper += n * kElems;
+                if (cm > bound) put_above(r, first);
+            } else {
+                raise(r, cm, valid, first);
+            }
+        }
+        if (steps == due) {
+            float v = all, t = -INFINITY;
+            for (int j = 0; j < (k + kWarps - 1) / kWarps; ++j) {
+                t = warp_max(v);
+                const unsigned who = __ballot_sync(0xffffffffu, v == t);
+                if ((threadIdx.x & 31) == __ffs(who) - 1) v = NAN;  // no maximum takes it again
+            }
+            if ((threadIdx.x & 31) == 0) deposit[turn + (threadIdx.x >> 5)] = t;
+        }
+    }
+
+    __device__ __forceinline__ void raise(const uint4 (&r)[kU], float cm, uint32_t valid, int first) {
+        int c = *count;
         __syncthreads();
-        if (threadIdx.x == 0) *count = c;
-        const bool want = !have || cm > bound;
-        const int n = __syncthreads_count(want);
+        bool want = !have || cm > bound;
+        int n = __syncthreads_count(want);
+        if (c > k && c + n * kElems > cap) {
+            sort_list<kThreads>(list, c);
+            c = k;
+            bound = fmaxf(bound, key_value((uint32_t)(list[k - 1] >> 32)));
+            have = true;
+            if (threadIdx.x == 0) *count = c;
+            want = cm > bound;
+            n = __syncthreads_count(want);
+        }
         bool equal = false;
-        if (!have || c + n * (kU * kV) > cap) {
+        if (!have || c + n * kElems > cap) {
             const uint32_t mine = valid ? order_key(cm) : 0u;
             uint32_t t = 0;
-            for (int b = 31; b >= 0; --b)
+            // the low 16 bits of a bf16 logit's key follow from its sign
+            for (int b = 31; b >= (DT == kBF16 ? 16 : 0); --b)
                 if (__syncthreads_count(mine >= (t | (1u << b))) >= k) t |= 1u << b;
+            if (DT == kBF16 && t && !(t & 0x80000000u)) t |= 0xffffu;
             const float f = t ? key_value(t) : -INFINITY;
             equal = !have || f > bound;
             if (equal) bound = f;
         }
-#pragma unroll
-        for (int i = 0; i < kU * kV; ++i)
-            if (x[i] > bound) put(x[i], first + (i / kV) * step + i % kV);
+        if (cm > bound) put_above(r, first);
         __syncthreads();
         if (equal) {
             int need = k - (*count - c);
@@ -246,13 +337,15 @@ struct Top {
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
                 if (need <= 0) continue;
-                int eq = 0;
+                uint32_t eq = 0;
+                if (valid >> u & 1u) {
 #pragma unroll
-                for (int e = 0; e < kV; ++e) {
-                    const float v = x[u * kV + e];
-                    eq += (valid >> u & 1u) && !(v > bound) && order_key(v) == order_key(bound);
+                    for (int e = 0; e < kVec; ++e) {
+                        const float v = value(r, u * kVec + e);
+                        eq |= (order_key(v) == order_key(bound) ? 1u : 0u) << e;
+                    }
                 }
-                int at = eq;
+                int at = __popc(eq);
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const int y = __shfl_up_sync(0xffffffffu, at, o);
@@ -261,20 +354,14 @@ struct Top {
                 if (lane == 31) scan[warp] = at;
                 __syncthreads();
                 int before = 0, total = 0;
-                for (int w = 0; w < kRowThreads / 32; ++w) {
+                for (int w = 0; w < kWarps; ++w) {
                     const int y = scan[w];
                     before += w < warp ? y : 0;
                     total += y;
                 }
-                int rank = before + at - eq;
-#pragma unroll
-                for (int e = 0; e < kV; ++e) {
-                    const float v = x[u * kV + e];
-                    if ((valid >> u & 1u) && !(v > bound) && order_key(v) == order_key(bound)) {
-                        if (rank < need) put(v, first + u * step + e);
-                        ++rank;
-                    }
-                }
+                int rank = before + at - __popc(eq);
+                for (; eq && rank < need; eq &= eq - 1, ++rank)
+                    put(bound, first + u * kThreads * kVec + __ffs(eq) - 1);
                 need -= total;
                 __syncthreads();
             }
@@ -294,44 +381,49 @@ struct Top {
     __device__ __forceinline__ void finish() {
         __syncthreads();
         const int c = *count;
-        sort_list(list, c);
+        sort_list<kThreads>(list, c);
         if (c < k) {
             int p = 2;
             while (p < c) p <<= 1;
-            for (int i = p + threadIdx.x; i < k; i += kRowThreads) list[i] = 0;
+            for (int i = p + threadIdx.x; i < k; i += kThreads) list[i] = 0;
             __syncthreads();
         }
     }
 };
 
+// steps that are loaded ahead, for 16 KB of them a CTA of 512 threads
 template <bool TOP>
 constexpr int kScoreStages = TOP ? 4 : 6;
 
-template <int DT, bool TOP>
-__global__ void __launch_bounds__(kRowThreads, 2) score_row_kernel(ScoreArgs a, uint32_t ctas) {
+template <int DT, int kThreads, bool TOP>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) score_row_kernel(ScoreArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
-    using Stream = RowStream<DT, 1, kScoreStages<TOP>>;
-    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems;
+    using Stream = RowStream<DT, kThreads, 1, kScoreStages<TOP>>;
+    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems, kWarps = kThreads / 32;
     extern __shared__ __align__(16) unsigned char sm[];  // the stream's places, the list
-    __shared__ float4 part[2][kRowWarps], mine[2];
-    __shared__ int count, scan[kRowWarps];
+    __shared__ float4 part[2][kWarps], mine[2];
+    __shared__ int count, scan[kWarps];
+    __shared__ float deposit[2 * kWarps];
     const int tid = threadIdx.x;
-    const uint32_t rank = blockIdx.x % ctas;
-    Top top;
+    const uint32_t ctas = 1u << lg, rank = blockIdx.x & (ctas - 1);
+    Top<DT, kThreads, kU> top;
     top.list = reinterpret_cast<uint64_t*>(sm + Stream::kBytes);
-    top.count = &count, top.scan = scan, top.k = a.k, top.cap = top_list(a.k) - 16;
-    RowList list(a.tok, a.z.T, a.N, blockIdx.x / ctas, gridDim.x / ctas);
-    Stream stream(a.z, a.V, list, rank, ctas, sm);
+    top.count = &count, top.scan = scan, top.deposit = deposit, top.k = a.k, top.cap = top_list(a.k) - 16;
+    const RowList list(a.tok, a.z.T, a.N, blockIdx.x >> lg, gridDim.x >> lg);
+    const RowStep step(a.z, gridDim.x >> lg);
+    Stream stream(a.z, a.V, list, step, rank, lg, sm);
+    RowAt at(a.z, list.first);
+    uint32_t live = 0;
     int parity = 0;
-    for (uint32_t i = 0; i < list.count; ++i) {
-        if ((i & 31) == 0) list.window(i);
+    for (uint32_t i = 0; i < list.count; ++i, step.move(at, a.z.T)) {
+        if ((i & 31) == 0) live = list.window(i);
         const uint32_t row = list.row(i);
-        if (!list.live(i)) {
-            if (rank == 0) score_padding(a, row, tid, kRowThreads);
+        if (!(live >> (i & 31) & 1u)) {
+            if (rank == 0) score_padding(a, row, tid, kThreads);
             continue;
         }
-        const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
-        const Segment g = segment_of<DT>(zr, a.V, rank, ctas);
+        const T* zr = reinterpret_cast<const T*>(a.z.p) + at.off;
+        const Segment g = segment_of<DT>(zr, a.V, rank, lg);
         const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
         const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
         int64_t t = 0;
@@ -349,27 +441,24 @@ __global__ void __launch_bounds__(kRowThreads, 2) score_row_kernel(ScoreArgs a, 
             uint4 raw[kU];
             stream.take(raw, v, g.v1);
             float x[kElems];
-            uint32_t valid = 0;
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                unpack16<DT>(raw[u], x + u * kVec);
-                valid |= (v + tid + u * kRowThreads < g.v1 ? 1u : 0u) << u;
-            }
+            for (int u = 0; u < kU; ++u) unpack16<DT>(raw[u], x + u * kVec);
+            const float cm = max_of<DT>(raw);
             stream.issue();
-            float cm = x[0];
-#pragma unroll
-            for (int e = 1; e < kElems; ++e) cm = fmaxf(cm, x[e]);
-            cm = fmaxf(cm, -INFINITY);  // all NaN
             add_values<kElems, true, false>(r, x, cm, a.c);
-            if constexpr (TOP)
-                top.template add<kU, kVec>(x, cm, valid, g.h0 + (v + tid) * kVec, kRowThreads * kVec);
+            if constexpr (TOP) {
+                uint32_t valid = 0;
+#pragma unroll
+                for (int u = 0; u < kU; ++u) valid |= (v + tid + u * kThreads < g.v1 ? 1u : 0u) << u;
+                top.add(raw, cm, r.m, valid, g.h0 + (v + tid) * kVec);
+            }
         }
         if (tid < ends) {
             const float x[1] = {end};
             add_values<1, true, false>(r, x, end, a.c);
             if constexpr (TOP) top.add_end(end, end_at, tid < g.head);
         }
-        r = cta_join<true, false>(r, part[parity], a.c);
+        r = cta_join<kThreads, true, false>(r, part[parity], a.c);
         if (ctas > 1) r = cluster_join<true, false>(r, &mine[parity], ctas, a.c);
         parity ^= 1;
         if (rank == 0 && tid == 0) score_write(a, row, z_t, r);
@@ -380,19 +469,17 @@ __global__ void __launch_bounds__(kRowThreads, 2) score_row_kernel(ScoreArgs a, 
                 cluster_sync();
                 if (rank == 0) {
                     best = top.list + a.k;
-                    for (int n = tid; n < (int)ctas * a.k; n += kRowThreads)
+                    for (int n = tid; n < (int)ctas * a.k; n += kThreads)
                         best[n] = ld_dsmem_u64(map_to_rank(smem_addr(top.list + n % a.k), n / a.k));
                 }
                 cluster_sync();
-                if (rank == 0) sort_list(best, (int)ctas * a.k);
+                if (rank == 0) sort_list<kThreads>(best, (int)ctas * a.k);
             }
-            if (rank == 0) {
+            if (rank == 0 && tid < a.k) {
                 const float log_s = logf(r.s);
-                for (int n = tid; n < a.k; n += kRowThreads) {
-                    a.top_index[(int64_t)row * a.k + n] = (uint32_t)~best[n];
-                    a.top_logprob[(int64_t)row * a.k + n] =
-                        log_prob(key_value((uint32_t)(best[n] >> 32)), r.m, r.s, log_s, a.tau);
-                }
+                a.top_index[(int64_t)row * a.k + tid] = (uint32_t)~best[tid];
+                a.top_logprob[(int64_t)row * a.k + tid] =
+                    log_prob(key_value((uint32_t)(best[tid] >> 32)), r.m, r.s, log_s, a.tau);
             }
             __syncthreads();
         }
@@ -494,22 +581,25 @@ __global__ void __launch_bounds__(256) score_grad_warp_kernel(ScoreGradArgs a) {
     }
 }
 
+constexpr int kGradThreads = 512;
+
+// CTA `part` of 2^lg of a row
 template <int DT>
-__global__ void __launch_bounds__(kRowThreads, 2) score_grad_row_kernel(ScoreGradArgs a, uint32_t parts) {
+__global__ void __launch_bounds__(kGradThreads, 2) score_grad_row_kernel(ScoreGradArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
     constexpr int kVec = Elem<DT>::kVec;
     const int tid = threadIdx.x;
-    const uint32_t row = blockIdx.x / parts;
+    const uint32_t row = blockIdx.x >> lg;
     const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : -1;
     const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
     T* dr = reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row);
-    const Segment g = segment_of<DT>(zr, a.V, blockIdx.x - row * parts, parts);
+    const Segment g = segment_of<DT>(zr, a.V, blockIdx.x & ((1u << lg) - 1u), lg);
     const bool live = !(a.tok.p && t == a.tok.ignore);
     const bool wide = (((uintptr_t)zr ^ (uintptr_t)dr) & 15u) == 0;  // 16-byte stores
     ScoreGrad r;
     if (live) r = score_grad_row(a, row, t);
     const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
-    for (int v = g.v0 + tid; v < g.v1; v += kRowThreads) {
+    for (int v = g.v0 + tid; v < g.v1; v += kGradThreads) {
         float y[kVec];
         if (live) {
             float x[kVec];
@@ -532,7 +622,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) score_grad_row_kernel(ScoreGra
     if (tid < g.tail) dr[g.t0 + tid] = from_float<T>(live ? r.at(to_float(zr[g.t0 + tid])) * r.inv_tau : 0.0f);
     if (!live) return;
     __syncthreads();
-    score_grad_slots<T>(a, r, row, t, zr, dr, g.j0, g.j1, tid, kRowThreads);
+    score_grad_slots<T>(a, r, row, t, zr, dr, g.j0, g.j1, tid, kGradThreads);
 }
 
 }  // namespace il
