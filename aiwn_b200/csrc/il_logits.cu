@@ -167,8 +167,8 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
             });
         return with_bool(k > 0, [&](auto top) {
             return with_threads(p.threads, [&](auto th) {
-                const size_t smem = RowStream<dt.value, th.value, 1, kScoreStages<top.value>>::kBytes +
-                                    (top.value ? 8 * (size_t)top_list(a.k) : 0);
+                const size_t smem = RowStream<dt.value, th.value, 1, kScoreStages>::kBytes +
+                                    (top.value ? 8 * (size_t)top_list(a.k, (int)p.lg) : 0);
                 return launch(score_row_kernel<dt.value, th.value, top.value>, p.grid, th.value, p.lg, smem, s, a, p.lg);
             });
         });

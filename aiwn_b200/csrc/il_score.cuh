@@ -7,21 +7,20 @@
 // with (m, s, u) of il_logits.cuh.  The forward reads each logit once, the
 // backward reads it once more and writes its gradient.
 //
-// The k largest in the same pass.  Every thread knows the maximum of the logits
-// that it holds.  For the row's first logits the k-th largest of the threads'
-// maxima is a lower bound of the k-th largest logit; from then on only logits
-// above the bound are put into a list in shared memory, so that the work on a
-// logit that is not among the largest is the comparison of its step's maximum.
-// After 1, 2, 4, ... steps the bound rises to what the threads' maxima so far
-// say: with j = k / warps (rounded up), the least of the warps' j-th largest.
-// For logits in no particular order the list so gets a few times k entries.
-// When it could run over, it is sorted and cut to k; when one step alone could
-// overrun it, the bound is first taken from that step's maxima: at most k - 1
-// threads then hold anything above it, and of the logits equal to it the first
-// ones by index are taken.  No input needs a second pass.  List entries are
-// (order-preserving bits of z) << 32 | ~index, so that all are distinct and
-// equal logits go by their index.
+// The k largest.  While a row goes by, each thread keeps the maximum of every
+// eighth of what it reads (rounded up to 16 bits, in shared memory), and
+// nothing else is done for them.  Then, with W warps and j = k / W rounded up,
+// the least of the warps' j-th largest thread maxima is a bound that at least k
+// logits reach, and of a row in no particular order not many more; the few
+// eighths that reach it are read again, and their logits that reach it are
+// sorted.  Entries are (order-preserving bits of z) << 32 | ~index, so that all
+// are distinct and equal logits go by their index.  Where more logits reach the
+// bound than the list holds, the k-th largest of those listed is a higher bound
+// for another round; where that is no higher, the list is of the logits above
+// the bound, and of those equal to it the first by index fill it up to k.
 #pragma once
+#include <type_traits>
+
 #include "il_logits.cuh"
 
 namespace il {
@@ -146,16 +145,11 @@ __global__ void __launch_bounds__(256) score_warp_kernel(ScoreArgs a) {
 
 // ---- longer rows: a CTA, or a cluster of CTAs, a row --------------------------------
 
-// entries of the list of candidates: k kept, 16 of each of k - 1 threads, k equal ones
-// and 16 of a row's ends; or k and those of 16 CTAs, sorted
-__host__ __device__ constexpr int top_merge(int k) {
-    int n = 2;
-    while (n < kMaxCluster * k) n <<= 1;
-    return n;
-}
-__host__ __device__ constexpr int top_list(int k) {
-    int n = 512;
-    while (n < 18 * k + 16 || n < k + top_merge(k)) n <<= 1;
+// entries of the list of candidates: some times k; in a cluster k and those of 2^lg CTAs, to be sorted
+__host__ __device__ constexpr int top_list(int k, int lg) {
+    int merge = 1, n = 512;
+    while (merge < k << lg) merge <<= 1;
+    while (lg && n < k + merge) n <<= 1;
     return n;
 }
 
@@ -210,177 +204,143 @@ __device__ __forceinline__ void sort_list(uint64_t* list, int n) {
         }
 }
 
+// 16 bits of a float, not below it
+__device__ __forceinline__ uint16_t upper16(float v) {
+    const uint32_t b = __float_as_uint(v);
+    const uint32_t up = (int32_t)b >= 0 ? b + 0xffffu : b;  // away from, or towards zero
+    return (uint16_t)((v == INFINITY ? b : up) >> 16);
+}
+
+constexpr int kTopGroups = 8;
+
 template <int DT, int kThreads, int kU>
 struct Top {
-    static constexpr int kVec = Elem<DT>::kVec, kElems = kU * kVec, kWarps = kThreads / 32;
-    uint64_t* list;  // shared
-    int* count;      // shared
-    int* scan;       // shared, one entry a warp
-    float* deposit;  // shared, two entries a warp, in turn
-    int k, cap;      // cap: 16 less than the list has room for
-    float bound;     // only logits above it are candidates, once `have`
-    bool have;       // k logits at or above `bound`, of lower index than any to come, are listed
-    int upper;       // at least *count
-    int steps, due;  // of the row; where `deposit` is next made or read
-    int turn;
+    static constexpr int kVec = Elem<DT>::kVec, kWarps = kThreads / 32, kStep = kU * kThreads;
+    struct Shared {
+        uint16_t most[kTopGroups][kThreads];  // maxima of the groups of steps
+        uint16_t hits[kTopGroups * kThreads];
+        float deposit[2][kWarps];
+        int scan[kWarps];
+        int count, hit_count;
+    };
+    using T = typename Elem<DT>::type;
+    Shared* sh;
+    uint64_t* list;  // shared, room for cap entries
+    int k, cap;
 
-    __device__ __forceinline__ void begin() {  // the caller's barrier follows
-        have = false;
-        upper = 0;
-        bound = -INFINITY;
-        steps = 0;
-        due = 1;
-        turn = 0;
-        if (threadIdx.x == 0) *count = 0;
-    }
-
-    __device__ __forceinline__ void put(float z, int index) {
-        list[atomicAdd(count, 1)] = ((uint64_t)order_key(z) << 32) | (uint32_t)~index;
-    }
-
-    __device__ __forceinline__ static float value(const uint4 (&r)[kU], int i) {
-        const uint4& q = r[i / kVec];
-        const int e = i % kVec;
-        if constexpr (DT == kF32) return __uint_as_float(e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w);
-        const uint32_t w = e / 2 == 0 ? q.x : e / 2 == 1 ? q.y : e / 2 == 2 ? q.z : q.w;
-        return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
-    }
-
-    // this thread's values above the bound
-    __device__ __forceinline__ void put_above(const uint4 (&r)[kU], int first) {
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            if constexpr (DT == kBF16) {
-                const __nv_bfloat162 b = __float2bfloat162_rn(bound);  // exact: a logit
-                const uint32_t w[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t above = __hgt2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[q]), b);
-                    if (above) {
-                        const int at = first + u * kThreads * kVec + 2 * q;
-                        if (above & 0xffffu) put(__uint_as_float(w[q] << 16), at);
-                        if (above >> 16) put(__uint_as_float(w[q] & 0xffff0000u), at + 1);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    const float v = value(r, u * kVec + e);
-                    if (v > bound) put(v, first + u * kThreads * kVec + e);
-                }
-            }
+    // the least of the warps' j-th largest of their lanes' values is left by two calls with a barrier between
+    __device__ __forceinline__ void offer(float all, int parity) const {
+        float v = all, t = -INFINITY;
+        for (int j = 0; j < (k + kWarps - 1) / kWarps; ++j) {
+            t = warp_max(v);
+            const unsigned who = __ballot_sync(0xffffffffu, v == t);
+            if ((threadIdx.x & 31) == __ffs(who) - 1) v = NAN;  // no maximum takes it again
         }
+        if ((threadIdx.x & 31) == 0) sh->deposit[parity][threadIdx.x >> 5] = t;
+    }
+    __device__ __forceinline__ float bound(int parity) const {
+        return -warp_max(-sh->deposit[parity][threadIdx.x & (kWarps - 1)]);
     }
 
-    // The row's next values: vector u of this thread, being logits first + u * kThreads * kVec + 0, 1, ..., is
-    // there if bit u of `valid` is set.  cm: their maximum, all: that of all of this thread's values so far.
-    __device__ __forceinline__ void add(const uint4 (&r)[kU], float cm, float all, uint32_t valid, int first) {
-        const int n = __syncthreads_count(!have || cm > bound);
-        ++steps;
-        if (have && steps == due + 1) {  // the deposit of the step before
-            const float b = deposit[turn + (threadIdx.x & (kWarps - 1))];
-            bound = fmaxf(bound, -warp_max(-b));
-            due *= 2;
-            turn ^= kWarps;
-        }
-        if (n != 0) {
-            if (have && upper + n * kElems <= cap) {
-                upper += n * kElems;
-                if (cm > bound) put_above(r, first);
-            } else {
-                raise(r, cm, valid, first);
-            }
-        }
-        if (steps == due) {
-            float v = all, t = -INFINITY;
-            for (int j = 0; j < (k + kWarps - 1) / kWarps; ++j) {
-                t = warp_max(v);
-                const unsigned who = __ballot_sync(0xffffffffu, v == t);
-                if ((threadIdx.x & 31) == __ffs(who) - 1) v = NAN;  // no maximum takes it again
-            }
-            if ((threadIdx.x & 31) == 0) deposit[turn + (threadIdx.x >> 5)] = t;
-        }
+    __device__ __forceinline__ void put(float z, int index) const {
+        const int at = atomicAdd(&sh->count, 1);
+        if (at < cap) list[at] = ((uint64_t)order_key(z) << 32) | (uint32_t)~index;
+    }
+    __device__ __forceinline__ static bool reaches(float z, float bound, bool above) {
+        return above ? z > bound : z >= bound;  // not NaN
     }
 
-    __device__ __forceinline__ void raise(const uint4 (&r)[kU], float cm, uint32_t valid, int first) {
-        int c = *count;
+    // Lists the part's logits that reach the bound (above: that are above it); false: more than the list holds.
+    // lg: log2 of the steps of a group; end, end_at, ends: this thread's logit of the row's ends.
+    __device__ __forceinline__ bool collect(const T* zr, const Segment& g, int lg, float end, int end_at, int ends,
+                                            float bound, bool above) const {
+        const int tid = threadIdx.x;
+        const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
+        if (tid == 0) sh->count = 0, sh->hit_count = 0;
         __syncthreads();
-        bool want = !have || cm > bound;
-        int n = __syncthreads_count(want);
-        if (c > k && c + n * kElems > cap) {
-            sort_list<kThreads>(list, c);
-            c = k;
-            bound = fmaxf(bound, key_value((uint32_t)(list[k - 1] >> 32)));
-            have = true;
-            if (threadIdx.x == 0) *count = c;
-            want = cm > bound;
-            n = __syncthreads_count(want);
-        }
-        bool equal = false;
-        if (!have || c + n * kElems > cap) {
-            const uint32_t mine = valid ? order_key(cm) : 0u;
-            uint32_t t = 0;
-            // the low 16 bits of a bf16 logit's key follow from its sign
-            for (int b = 31; b >= (DT == kBF16 ? 16 : 0); --b)
-                if (__syncthreads_count(mine >= (t | (1u << b))) >= k) t |= 1u << b;
-            if (DT == kBF16 && t && !(t & 0x80000000u)) t |= 0xffffu;
-            const float f = t ? key_value(t) : -INFINITY;
-            equal = !have || f > bound;
-            if (equal) bound = f;
-        }
-        if (cm > bound) put_above(r, first);
+        const int groups = (g.v1 - g.v0 + (kStep << lg) - 1) / (kStep << lg);
+        for (int n = 0; n < groups; ++n)
+            if (reaches(__uint_as_float((uint32_t)sh->most[n][tid] << 16), bound, above))
+                sh->hits[atomicAdd(&sh->hit_count, 1)] = (uint16_t)(n * kThreads + tid);
+        if (tid < ends && reaches(end, bound, above)) put(end, end_at);
         __syncthreads();
-        if (equal) {
-            int need = k - (*count - c);
+        const int hits = sh->hit_count, per = kU << lg;
+        for (int n = tid; n < hits * per; n += kThreads) {
+            const int h = sh->hits[n / per], q = n % per;
+            const int v = g.v0 + ((h / kThreads << lg) + q / kU) * kStep + q % kU * kThreads + h % kThreads;
+            if (v >= g.v1) continue;
+            float x[kVec];
+            unpack16<DT>(__ldg(body + v), x);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e)
+                if (reaches(x[e], bound, above)) put(x[e], g.h0 + v * kVec + e);
+        }
+        __syncthreads();
+        return sh->count <= cap;
+    }
+
+    // the first `need` logits by index that equal the bound (-inf: NaN too)
+    __device__ __forceinline__ void fill(const T* zr, const Segment& g, float bound, int need) const {
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
+        auto equal = [&](float z) { return z == bound || (z != z && bound == -INFINITY); };
+        for (int j = 0; j < g.head; ++j)
+            if (need > 0 && equal(to_float(zr[j]))) {
+                if (tid == 0) put(bound, j);
+                --need;
+            }
+        for (int v = g.v0; need > 0 && v < g.v1; v += kThreads) {
+            uint32_t eq = 0;
+            if (v + tid < g.v1) {
+                float x[kVec];
+                unpack16<DT>(__ldg(body + v + tid), x);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) eq |= (equal(x[e]) ? 1u : 0u) << e;
+            }
+            int at = __popc(eq);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, at, o);
+                if (lane >= o) at += y;
+            }
+            if (lane == 31) sh->scan[warp] = at;
             __syncthreads();
-            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                if (need <= 0) continue;
-                uint32_t eq = 0;
-                if (valid >> u & 1u) {
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) {
-                        const float v = value(r, u * kVec + e);
-                        eq |= (order_key(v) == order_key(bound) ? 1u : 0u) << e;
-                    }
-                }
-                int at = __popc(eq);
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, at, o);
-                    if (lane >= o) at += y;
-                }
-                if (lane == 31) scan[warp] = at;
-                __syncthreads();
-                int before = 0, total = 0;
-                for (int w = 0; w < kWarps; ++w) {
-                    const int y = scan[w];
-                    before += w < warp ? y : 0;
-                    total += y;
-                }
-                int rank = before + at - __popc(eq);
-                for (; eq && rank < need; eq &= eq - 1, ++rank)
-                    put(bound, first + u * kThreads * kVec + __ffs(eq) - 1);
-                need -= total;
-                __syncthreads();
+            int before = 0, total = 0;
+            for (int w = 0; w < kWarps; ++w) {
+                const int y = sh->scan[w];
+                before += w < warp ? y : 0;
+                total += y;
             }
+            int rank = before + at - __popc(eq);
+            for (; eq && rank < need; eq &= eq - 1, ++rank) put(bound, g.h0 + (v + tid) * kVec + __ffs(eq) - 1);
+            need -= total;
+            __syncthreads();
         }
-        upper = *count;
+        for (int j = g.t0; j < g.t0 + g.tail; ++j)
+            if (need > 0 && equal(to_float(zr[j]))) {
+                if (tid == 0) put(bound, j);
+                --need;
+            }
         __syncthreads();
-        have = upper >= k;
     }
 
-    // a logit of the row's ends, after all others: of lower index than all of them, or of higher
-    __device__ __forceinline__ void add_end(float z, int index, bool lower) {
-        const float v = z != z ? -INFINITY : z;
-        if (!have || v > bound || (lower && v == bound)) put(v, index);
-    }
-
-    // list[0 .. k - 1]: the largest, sorted; 0 where the part of the row has fewer
-    __device__ __forceinline__ void finish() {
-        __syncthreads();
-        const int c = *count;
+    // list[0 .. k - 1]: the largest of the part, sorted; 0 where it has fewer
+    __device__ __forceinline__ void find(const T* zr, const Segment& g, int lg, float end, int end_at, int ends,
+                                         float bound) const {
+        bool above = bound == -INFINITY;
+        while (!collect(zr, g, lg, end, end_at, ends, bound, above)) {
+            sort_list<kThreads>(list, cap);
+            const float b = key_value((uint32_t)(list[k - 1] >> 32));
+            above = !(b > bound);
+            bound = b;
+            __syncthreads();
+        }
+        if (above && sh->count < k) {
+            const int need = k - sh->count;
+            __syncthreads();
+            fill(zr, g, bound, need);
+        }
+        const int c = sh->count;
         sort_list<kThreads>(list, c);
         if (c < k) {
             int p = 2;
@@ -391,24 +351,23 @@ struct Top {
     }
 };
 
-// steps that are loaded ahead, for 16 KB of them a CTA of 512 threads
-template <bool TOP>
-constexpr int kScoreStages = TOP ? 4 : 6;
+constexpr int kScoreStages = 5;  // steps that are loaded ahead
 
 template <int DT, int kThreads, bool TOP>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) score_row_kernel(ScoreArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
-    using Stream = RowStream<DT, kThreads, 1, kScoreStages<TOP>>;
+    using Stream = RowStream<DT, kThreads, 1, kScoreStages>;
     constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems, kWarps = kThreads / 32;
+    using TopOf = Top<DT, kThreads, kU>;
     extern __shared__ __align__(16) unsigned char sm[];  // the stream's places, the list
     __shared__ float4 part[2][kWarps], mine[2];
-    __shared__ int count, scan[kWarps];
-    __shared__ float deposit[2 * kWarps];
+    __shared__ typename std::conditional<TOP, typename TopOf::Shared, int>::type top_shared;
     const int tid = threadIdx.x;
     const uint32_t ctas = 1u << lg, rank = blockIdx.x & (ctas - 1);
-    Top<DT, kThreads, kU> top;
-    top.list = reinterpret_cast<uint64_t*>(sm + Stream::kBytes);
-    top.count = &count, top.scan = scan, top.deposit = deposit, top.k = a.k, top.cap = top_list(a.k) - 16;
+    TopOf top;
+    if constexpr (TOP)
+        top.sh = &top_shared, top.list = reinterpret_cast<uint64_t*>(sm + Stream::kBytes), top.k = a.k,
+        top.cap = top_list(a.k, lg);
     const RowList list(a.tok, a.z.T, a.N, blockIdx.x >> lg, gridDim.x >> lg);
     const RowStep step(a.z, gridDim.x >> lg);
     Stream stream(a.z, a.V, list, step, rank, lg, sm);
@@ -426,17 +385,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) score_row_kernel(Sc
         const Segment g = segment_of<DT>(zr, a.V, rank, lg);
         const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
         const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
-        int64_t t = 0;
         float z_t = 0.0f;
         if (tid == 0 && a.logprob) {
-            t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
+            const int64_t t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
             z_t = t >= 0 && t < a.V ? to_float(zr[t]) : NAN;
         }
-        if constexpr (TOP) {
-            top.begin();
-            __syncthreads();
-        }
+        int group_lg = 0;  // kTopGroups groups of 2^group_lg steps are enough
+        if constexpr (TOP)
+            while ((Stream::kStep * kTopGroups << group_lg) < g.v1 - g.v0) ++group_lg;
         Sums r = no_sums();
+        float most = -INFINITY;
+        int n = 0;
         for (int v = g.v0; v < g.v1; v += Stream::kStep) {
             uint4 raw[kU];
             stream.take(raw, v, g.v1);
@@ -447,23 +406,27 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) score_row_kernel(Sc
             stream.issue();
             add_values<kElems, true, false>(r, x, cm, a.c);
             if constexpr (TOP) {
-                uint32_t valid = 0;
-#pragma unroll
-                for (int u = 0; u < kU; ++u) valid |= (v + tid + u * kThreads < g.v1 ? 1u : 0u) << u;
-                top.add(raw, cm, r.m, valid, g.h0 + (v + tid) * kVec);
+                most = fmaxf(most, cm);
+                ++n;
+                if ((n & ((1 << group_lg) - 1)) == 0 || v + Stream::kStep >= g.v1) {
+                    top_shared.most[(n - 1) >> group_lg][tid] = upper16(most);
+                    most = -INFINITY;
+                }
             }
         }
+        if constexpr (TOP) top.offer(r.m, parity);
         if (tid < ends) {
             const float x[1] = {end};
             add_values<1, true, false>(r, x, end, a.c);
-            if constexpr (TOP) top.add_end(end, end_at, tid < g.head);
         }
         r = cta_join<kThreads, true, false>(r, part[parity], a.c);
+        float bound = 0.0f;
+        if constexpr (TOP) bound = top.bound(parity);
         if (ctas > 1) r = cluster_join<true, false>(r, &mine[parity], ctas, a.c);
         parity ^= 1;
         if (rank == 0 && tid == 0) score_write(a, row, z_t, r);
         if constexpr (TOP) {
-            top.finish();
+            top.find(zr, g, group_lg, end, end_at, ends, bound);
             uint64_t* best = top.list;
             if (ctas > 1) {
                 cluster_sync();
