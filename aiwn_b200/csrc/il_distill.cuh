@@ -399,13 +399,11 @@ __device__ __forceinline__ uint4 without(const uint4& r, uint32_t bits) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-constexpr int kDistillStages = 5;  // steps that are loaded ahead
-
 template <int DT, int kThreads, bool TAIL, bool S1, bool GRAD>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_row_kernel(DistillArgs a, uint32_t lg) {
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(DistillArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
-    using Stream = RowStream<DT, kThreads, GRAD ? 2 : 1, kDistillStages>;
-    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems, kWarps = kThreads / 32;
+    using Stream = RowStream<DT, kThreads, GRAD ? 2 : 1>;
+    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kWarps = kThreads / 32;
     if (a.skip_if_one && *a.g == 1.0f) return;
     extern __shared__ __align__(16) unsigned char sm[];  // the stream's places, the bitmap
     uint32_t* named = reinterpret_cast<uint32_t*>(sm + Stream::kBytes);
@@ -494,26 +492,34 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_row_kernel(
             });
             if ((tid & 31) == 0) slots[parity][tid >> 5] = x;
         }
-        Sums s = no_sums();
-        for (int v = g.v0; v < g.v1; v += Stream::kStep) {
-            uint4 raw[kU];
-            stream.take(raw, v, g.v1);
+        Running<false, S1> run;
+        run.begin();
+        auto use = [&](uint4 (&raw)[kU], int v) {  // v: of the first vector
             if constexpr (TAIL) {
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    const int w = v + tid + u * kThreads;
+                    const int w = v + u * kThreads;
                     const int b = w < g.v1 ? (w - g.v0) * kVec : 0;
                     const uint32_t bits = named[b >> 5] >> (b & 31) & ((1u << kVec) - 1u);
                     if (bits) raw[u] = without<DT>(raw[u], bits);
                 }
             }
-            float x[kElems];
-#pragma unroll
-            for (int u = 0; u < kU; ++u) unpack16<DT>(raw[u], x + u * kVec);
-            const float cm = max_of<DT>(raw);
+            run.template add<DT>(raw, max_of<DT>(raw), a.c);
+        };
+        int left = g.v1 - g.v0;
+        for (; left >= Stream::kStep; left -= Stream::kStep) {
+            uint4 raw[kU];
+            stream.template take<true>(raw, 0);
             stream.issue();
-            add_values<kElems, false, S1>(s, x, cm, a.c);
+            use(raw, g.v1 - left + tid);
         }
+        if (left > 0) {
+            uint4 raw[kU];
+            stream.template take<false>(raw, (left - tid + kThreads - 1) / kThreads);
+            stream.issue();
+            use(raw, g.v1 - left + tid);
+        }
+        Sums s = run.sums(a.c);
         if (tid < ends) {
             float x[1] = {end};
             if constexpr (TAIL) {
@@ -537,26 +543,35 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) distill_row_kernel(
         if constexpr (GRAD) {
             __syncthreads();
             const DistillRow r = shared_row[parity];
-            for (int v = g.v0; v < g.v1; v += Stream::kStep) {
-                uint4 raw[kU];
-                stream.take(raw, v, g.v1);
-                float x[kElems];
-#pragma unroll
-                for (int u = 0; u < kU; ++u) unpack16<DT>(raw[u], x + u * kVec);
-                stream.issue();
-                r.template at_all<S1, kElems>(x);
+            auto write = [&](const uint4 (&raw)[kU], int v, int mine) {
+                T* to = dr + g.h0 + (int64_t)v * kVec;
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    const int w = v + tid + u * kThreads;
-                    if (w >= g.v1) continue;
-                    T* to = dr + g.h0 + (int64_t)w * kVec;
+                    if (u >= mine) continue;
+                    float x[kVec];
+                    unpack16<DT>(raw[u], x);
+                    r.template at_all<S1, kVec>(x);
                     if (wide) {
-                        __stcs(reinterpret_cast<uint4*>(to), pack16<DT>(x + u * kVec));
+                        __stcs(reinterpret_cast<uint4*>(to) + u * kThreads, pack16<DT>(x));
                     } else {
 #pragma unroll
-                        for (int e = 0; e < kVec; ++e) to[e] = from_float<T>(x[u * kVec + e]);
+                        for (int e = 0; e < kVec; ++e) to[u * kThreads * kVec + e] = from_float<T>(x[e]);
                     }
                 }
+            };
+            left = g.v1 - g.v0;
+            for (; left >= Stream::kStep; left -= Stream::kStep) {
+                uint4 raw[kU];
+                stream.template take<true>(raw, 0);
+                stream.issue();
+                write(raw, g.v1 - left + tid, kU);
+            }
+            if (left > 0) {
+                uint4 raw[kU];
+                const int mine = (left - tid + kThreads - 1) / kThreads;
+                stream.template take<false>(raw, mine);
+                stream.issue();
+                write(raw, g.v1 - left + tid, mine);
             }
             if (tid < ends) dr[end_at] = from_float<T>(r.template at<S1>(end));
             __syncthreads();

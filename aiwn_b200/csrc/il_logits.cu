@@ -40,7 +40,7 @@ int check_rows(int dtype, int64_t B, int64_t T, int64_t V, double temperature) {
 // the row stride of the operands and their element size: natural alignment of the base is all that is asked
 int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_BF16 ? 1u : 3u)) ? IL_ERR_ALIGN : IL_OK; }
 
-// Rows of more than kWarpVocab logits.  1024 threads an SM, in CTAs of 512, 256 or 128: a
+// Rows of more than kWarpVocab logits.  512 threads an SM, in CTAs of 512, 256 or 128: a
 // warp's share of what a row costs beside its logits is the same whatever the row's length,
 // so that shorter rows get fewer warps.  Then the CTAs of a row: those that take the
 // shortest time by a simple count, in which a cluster of c CTAs has 1/c of a row to load
@@ -65,9 +65,9 @@ Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, bool twice) {
             if (V / c > (1 << 18) || (threads == t && c < ctas) || (threads && threads != t)) continue;
             if (threads && best != 0.0) break;
             if (best != 0.0 && bytes / c < 16 * t) break;  // less than half a step of the CTA's threads
-            const int64_t clusters = (int64_t)sms * (1024 / t) / c;
+            const int64_t clusters = (int64_t)sms * (512 / t) / c;
             const double rounds = (double)((N + clusters - 1) / clusters);
-            const double rate = 1.0 / (1024 / t);  // CTAs of an SM share it
+            const double rate = 1.0 / (512 / t);  // CTAs of an SM share it
             double time = rounds * (bytes / c / rate * 1.0 + (c > 1 ? 2.0 : 1.0) * kRowCost * 2);
             if (twice && (double)(N < clusters ? N : clusters) * bytes > kResident) time *= 1.3;
             if (best == 0.0 || time < best) {
@@ -167,7 +167,7 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
             });
         return with_bool(k > 0, [&](auto top) {
             return with_threads(p.threads, [&](auto th) {
-                const size_t smem = RowStream<dt.value, th.value, 1, kScoreStages>::kBytes +
+                const size_t smem = RowStream<dt.value, th.value, 1>::kBytes +
                                     (top.value ? 8 * (size_t)top_list(a.k, (int)p.lg) : 0);
                 return launch(score_row_kernel<dt.value, th.value, top.value>, p.grid, th.value, p.lg, smem, s, a, p.lg);
             });
@@ -269,7 +269,7 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
                     });
                 return with_bool(dlogits != nullptr, [&](auto gr) {
                     return with_threads(p.threads, [&](auto th) {
-                        const size_t smem = RowStream<dt.value, th.value, 1, kDistillStages>::kBytes +
+                        const size_t smem = RowStream<dt.value, th.value, 1>::kBytes +
                                             (tl.value ? 4 * (size_t)distill_words(a.V, 1 << p.lg) : 0);
                         return launch(distill_row_kernel<dt.value, th.value, tl.value, s1.value, gr.value>, p.grid,
                                       th.value, p.lg, smem, s, a, p.lg);

@@ -96,6 +96,31 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
 }
 
+// two floats in one 64-bit register pair: one instruction for both
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // 16 bytes to floats and back
 template <int DT>
 __device__ __forceinline__ void unpack16(const uint4& r, float* x) {
@@ -143,31 +168,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
-}
-
-// two floats in one 64-bit register pair: one instruction for both
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
 }
 
 constexpr float kLn2 = 0.693147180559945309f;
@@ -267,6 +267,112 @@ __device__ __forceinline__ float max_of(const uint4 (&r)[kU]) {
     }
 }
 
+// Values below -2^100 raised to it (NaN stays): their exponential is 0 next to any maximum
+// of ordinary size, and their exponent then is finite, so that 0 times it is 0.
+template <int DT>
+__device__ __forceinline__ uint4 floor16(const uint4& r) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == kF32) {
+            y[i] = __float_as_uint(max_nan(__uint_as_float(w[i]), -1.2676506e30f));
+        } else {
+            const uint32_t low = 0xf180f180u;  // -2^100, twice
+            const __nv_bfloat162 v = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w[i]),
+                                                 *reinterpret_cast<const __nv_bfloat162*>(&low));
+            y[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+    return make_uint4(y[0], y[1], y[2], y[3]);
+}
+
+// A thread's sums while a row goes by.  The exponent is taken to a whole number H next to
+// m log2(e) / tau: d = z c - H is one fused multiply-add, rounded once, and a new maximum
+// rescales by a power of two, without rounding.  Where |m| c is 2^22 or more (a row of nothing
+// but a mask's huge negative values) such an H has no meaning, and d = (z - m) c.
+template <bool U, bool S1>
+struct Running {
+    float m, s, u, s1, h, h1;  // h, h1: -H for c and for log2(e)
+    bool huge;
+
+    __device__ __forceinline__ void begin() {
+        m = -INFINITY;
+        s = u = s1 = h = h1 = 0.0f;
+        huge = false;
+    }
+    __device__ __forceinline__ static bool is_huge(float t) { return !(fabsf(t) < 4194304.0f); }
+
+    __device__ __forceinline__ void raise(float top, float c) {
+        const float t = top * c;
+        const bool now = is_huge(t) || (S1 && is_huge(top * kLog2e));
+        const float g = now ? -t : -rintf(t), g1 = now ? -top * kLog2e : -rintf(top * kLog2e);
+        if (m != -INFINITY) {
+            const float d = fmaxf(now && huge ? (m - top) * c : g - h, kMinExp), f = exp2_approx(d);
+            if constexpr (U) u = f * (u + s * d);
+            s *= f;
+            if constexpr (S1) s1 *= exp2_approx(fmaxf(now && huge ? (m - top) * kLog2e : g1 - h1, kMinExp));
+        }
+        m = top, h = g, h1 = g1, huge = now;
+    }
+
+    // kU 16-byte vectors whose maximum is cm; they are summed among themselves first: a long row's
+    // small terms would be lost one by one in a sum that already holds the row's largest
+    template <int DT, int kU>
+    __device__ __forceinline__ void add(const uint4 (&r)[kU], float cm, float c) {
+        constexpr int kVec = Elem<DT>::kVec;
+        if (cm > m) raise(cm, c);
+        if (huge) {
+#pragma unroll
+            for (int q = 0; q < kU; ++q) {
+                float x[kVec];
+                unpack16<DT>(r[q], x);
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) {
+                    const float d = exponent(x[i], m, c), e = exp2_approx(d);
+                    s += e;
+                    if constexpr (U) u = fmaf(e, d, u);
+                    if constexpr (S1) s1 += exp2_approx(exponent(x[i], m, kLog2e));
+                }
+            }
+        } else {
+            float e0 = 0.0f, e1 = 0.0f, u0 = 0.0f, u1 = 0.0f, f0 = 0.0f, f1 = 0.0f;  // of the even and the odd values
+#pragma unroll
+            for (int q = 0; q < kU; ++q) {
+                float x[kVec];
+                unpack16<DT>(U ? floor16<DT>(r[q]) : r[q], x);
+#pragma unroll
+                for (int i = 0; i < kVec; i += 2) {
+                    const float d0 = fmaf(x[i], c, h), d1 = fmaf(x[i + 1], c, h);
+                    const float a0 = exp2_approx(d0), a1 = exp2_approx(d1);
+                    e0 += a0;
+                    e1 += a1;
+                    if constexpr (U) u0 = fmaf(a0, d0, u0), u1 = fmaf(a1, d1, u1);
+                    if constexpr (S1) {
+                        f0 += exp2_approx(fmaf(x[i], kLog2e, h1));
+                        f1 += exp2_approx(fmaf(x[i + 1], kLog2e, h1));
+                    }
+                }
+            }
+            s += e0 + e1;
+            if constexpr (U) u += u0 + u1;
+            if constexpr (S1) s1 += f0 + f1;
+        }
+    }
+
+    // the same sums taken to the maximum itself
+    __device__ __forceinline__ Sums sums(float c) const {
+        Sums r{m, s, u, s1};
+        if (m != -INFINITY && !huge) {
+            const float d = fmaf(m, c, h), f = exp2_approx(-d);
+            if constexpr (U) r.u = f * (u - d * s);
+            r.s = f * s;
+            if constexpr (S1) r.s1 = exp2_approx(-fmaf(m, kLog2e, h1)) * s1;
+        }
+        return r;
+    }
+};
+
 // lanes of a warp, all lanes get the result; kLanes = 32 or 16 (lanes 0..15 hold values)
 template <int kLanes = 32>
 __device__ __forceinline__ float warp_sum(float v) {
@@ -279,11 +385,12 @@ __device__ __forceinline__ double warp_sum(double v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// NaN lanes are left out
+// the largest of the lanes' values, NaN lanes left out (NaN where there is nothing else)
 __device__ __forceinline__ float warp_max(float v) {
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
+    const uint32_t b = __float_as_uint(v);
+    const uint32_t key = v != v ? 0u : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, key);
+    return __uint_as_float(top ^ ((uint32_t)((int32_t)~top >> 31) | 0x80000000u));  // 0: all bits set, a NaN
 }
 
 // every lane's sums -> the warp's, in all lanes
@@ -387,17 +494,8 @@ struct RowList {
     }
 };
 
-__device__ __forceinline__ uint64_t policy_evict_first() {
-    uint64_t p;
-    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
-    return p;
-}
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, uint64_t policy) {
-    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
-                 : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int n>
@@ -409,12 +507,13 @@ __device__ __forceinline__ void copy_wait() {
 // ahead of their use and across the ends of rows, so that loads go on while a
 // row's sums are joined.  Each thread copies what it will read itself into
 // places of its own (cp.async), so that no barrier is involved.  Every row is
-// gone through kPasses times; the last time its lines may leave the L2 first.
-template <int DT, int kThreads, int kPasses, int kStages>
+// gone through kPasses times.
+template <int DT, int kThreads, int kPasses>
 struct RowStream {
-    static constexpr int kVec = Elem<DT>::kVec, kU = 2, kElems = kU * kVec;
+    static constexpr int kVec = Elem<DT>::kVec, kU = 4, kElems = kU * kVec, kStages = 4;
     static constexpr int kStep = kU * kThreads;  // vectors of a step
-    static constexpr int kBytes = kStages * kStep * 16;
+    static constexpr uint32_t kStepBytes = kStep * 16, kBytes = kStages * kStepBytes;
+    static_assert((kStages & (kStages - 1)) == 0, "the places are gone round by a mask");
     using T = typename Elem<DT>::type;
 
     const RowsIn& z;
@@ -423,83 +522,82 @@ struct RowStream {
     const RowList& list;
     const RowStep& step;
     RowAt at;
-    uint32_t slots;      // shared address of this thread's places
-    uint32_t i, live;    // row being loaded, its window
-    int v, v1;           // this thread's next vector, the end
-    int left;            // passes over the row after this one
-    uint32_t put, get;   // bytes
-    const uint4* body;
-    uint64_t policy;
+    uint32_t slots;     // shared address of this thread's places
+    uint32_t i, live;   // row being loaded, its window
+    uint32_t put, get;  // bytes
+    const uint4* src;   // this thread's next vector
+    int mine, steps;    // vectors and steps left of this pass
+    int passes;         // left after this one
 
     __device__ __forceinline__ RowStream(const RowsIn& z_, int V_, const RowList& list_, const RowStep& step_,
                                          uint32_t rank_, uint32_t lg_, void* shared)
-        : z(z_), V(V_), rank(rank_), lg(lg_), list(list_), step(step_), at(z_, list_.first), i(0), v(0), v1(0),
-          left(0), put(0), get(0) {
+        : z(z_), V(V_), rank(rank_), lg(lg_), list(list_), step(step_), at(z_, list_.first), i(0), put(0), get(0),
+          mine(0), steps(0), passes(0), src(nullptr) {
         slots = smem_addr(shared) + threadIdx.x * 16;
-        policy = policy_evict_first();
         live = list.window(0);
-        begin_row();
+        next_row();
 #pragma unroll 1
         for (int n = 0; n < kStages; ++n) issue();
     }
 
-    __device__ __forceinline__ void next_row() {
-        step.move(at, z.T);
-        if ((++i & 31) == 0 && i < list.count) live = list.window(i);
+    __device__ __forceinline__ void begin_pass(const Segment& g, const T* zr) {
+        src = reinterpret_cast<const uint4*>(zr + g.h0) + g.v0 + threadIdx.x;
+        mine = (g.v1 - g.v0 - (int)threadIdx.x + kThreads - 1) / kThreads;
+        steps = (g.v1 - g.v0 + kStep - 1) / kStep;
     }
 
-    // to the first row from i on that has vectors to load
-    __device__ __forceinline__ void begin_row() {
-        for (; i < list.count; next_row()) {
+    // to the first row from i on that has vectors to load; steps is 0 if there is none
+    __device__ __forceinline__ void next_row() {
+        for (; i < list.count; step.move(at, z.T), ++i) {
+            if ((i & 31) == 0 && i) live = list.window(i);
             if (!(live >> (i & 31) & 1u)) continue;
             const T* zr = reinterpret_cast<const T*>(z.p) + at.off;
             const Segment g = segment_of<DT>(zr, V, rank, lg);
             if (g.v0 >= g.v1) continue;
-            body = reinterpret_cast<const uint4*>(zr + g.h0);
-            v = g.v0 + threadIdx.x, v1 = g.v1;
-            left = kPasses - 1;
+            begin_pass(g, zr);
+            passes = kPasses - 1;
             return;
         }
     }
 
     __device__ __forceinline__ void issue() {
-        if (i < list.count) {
+        if (steps) {
 #pragma unroll
             for (int u = 0; u < kU; ++u)
-                if (v + u * kThreads < v1) {
-                    const uint32_t to = slots + put + u * (kThreads * 16);
-                    if (kPasses == 1 || left == 0) copy_async16(to, body + v + u * kThreads, policy);
-                    else copy_async16(to, body + v + u * kThreads);
-                }
-            v += kStep;
-            if (v - (int)threadIdx.x >= v1) {
-                if (kPasses > 1 && left > 0) {
-                    --left;
+                if (u < mine) copy_async16(slots + put + u * (kThreads * 16), src + u * kThreads);
+            src += kStep;
+            mine -= kU;
+            if (--steps == 0) {
+                if (kPasses > 1 && passes > 0) {
+                    --passes;
                     const T* zr = reinterpret_cast<const T*>(z.p) + at.off;
-                    v = segment_of<DT>(zr, V, rank, lg).v0 + threadIdx.x;
+                    begin_pass(segment_of<DT>(zr, V, rank, lg), zr);
                 } else {
+                    step.move(at, z.T);
+                    ++i;
                     next_row();
-                    begin_row();
                 }
             }
         }
         copy_commit();
-        put = put + kStep * 16 == kBytes ? 0 : put + kStep * 16;
+        put = (put + kStepBytes) & (kBytes - 1);
     }
 
-    // this thread's next kU vectors, -inf from `end` on; first: the step's first vector
-    __device__ __forceinline__ void take(uint4 (&r)[kU], int first, int end) {
+    // this thread's next kU vectors, of which the row has `mine`; the others are -inf
+    template <bool FULL>
+    __device__ __forceinline__ void take(uint4 (&r)[kU], int mine) {
         copy_wait<kStages - 1>();
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            r[u] = neg_inf16<DT>();
-            if (first + (int)threadIdx.x + u * kThreads < end)
+            const uint32_t from = slots + get + u * (kThreads * 16);
+            if (!FULL) r[u] = neg_inf16<DT>();
+            if (FULL || u < mine)
                 asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(r[u].x), "=r"(r[u].y), "=r"(r[u].z), "=r"(r[u].w)
-                             : "r"(slots + get + u * (kThreads * 16))
+                             : "r"(from)
                              : "memory");
         }
-        get = get + kStep * 16 == kBytes ? 0 : get + kStep * 16;
+        get = (get + kStepBytes) & (kBytes - 1);
     }
 };
 

@@ -8,11 +8,11 @@
 // backward reads it once more and writes its gradient.
 //
 // The k largest.  While a row goes by, each thread keeps the maximum of every
-// eighth of what it reads (rounded up to 16 bits, in shared memory), and
+// sixteenth of what it reads (rounded up to 16 bits, in shared memory), and
 // nothing else is done for them.  Then, with W warps and j = k / W rounded up,
 // the least of the warps' j-th largest thread maxima is a bound that at least k
 // logits reach, and of a row in no particular order not many more; the few
-// eighths that reach it are read again, and their logits that reach it are
+// sixteenths that reach it are read again, and their logits that reach it are
 // sorted.  Entries are (order-preserving bits of z) << 32 | ~index, so that all
 // are distinct and equal logits go by their index.  Where more logits reach the
 // bound than the list holds, the k-th largest of those listed is a higher bound
@@ -211,7 +211,7 @@ __device__ __forceinline__ uint16_t upper16(float v) {
     return (uint16_t)((v == INFINITY ? b : up) >> 16);
 }
 
-constexpr int kTopGroups = 8;
+constexpr int kTopGroups = 16;
 
 template <int DT, int kThreads, int kU>
 struct Top {
@@ -351,13 +351,11 @@ struct Top {
     }
 };
 
-constexpr int kScoreStages = 5;  // steps that are loaded ahead
-
 template <int DT, int kThreads, bool TOP>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) score_row_kernel(ScoreArgs a, uint32_t lg) {
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) score_row_kernel(ScoreArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
-    using Stream = RowStream<DT, kThreads, 1, kScoreStages>;
-    constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kElems = Stream::kElems, kWarps = kThreads / 32;
+    using Stream = RowStream<DT, kThreads, 1>;
+    constexpr int kU = Stream::kU, kWarps = kThreads / 32;
     using TopOf = Top<DT, kThreads, kU>;
     extern __shared__ __align__(16) unsigned char sm[];  // the stream's places, the list
     __shared__ float4 part[2][kWarps], mine[2];
@@ -393,27 +391,36 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) score_row_kernel(Sc
         int group_lg = 0;  // kTopGroups groups of 2^group_lg steps are enough
         if constexpr (TOP)
             while ((Stream::kStep * kTopGroups << group_lg) < g.v1 - g.v0) ++group_lg;
-        Sums r = no_sums();
+        Running<true, false> run;
+        run.begin();
         float most = -INFINITY;
         int n = 0;
-        for (int v = g.v0; v < g.v1; v += Stream::kStep) {
-            uint4 raw[kU];
-            stream.take(raw, v, g.v1);
-            float x[kElems];
-#pragma unroll
-            for (int u = 0; u < kU; ++u) unpack16<DT>(raw[u], x + u * kVec);
+        auto use = [&](const uint4 (&raw)[kU], bool last) {
             const float cm = max_of<DT>(raw);
-            stream.issue();
-            add_values<kElems, true, false>(r, x, cm, a.c);
+            run.template add<DT>(raw, cm, a.c);
             if constexpr (TOP) {
                 most = fmaxf(most, cm);
                 ++n;
-                if ((n & ((1 << group_lg) - 1)) == 0 || v + Stream::kStep >= g.v1) {
+                if ((n & ((1 << group_lg) - 1)) == 0 || last) {
                     top_shared.most[(n - 1) >> group_lg][tid] = upper16(most);
                     most = -INFINITY;
                 }
             }
+        };
+        int left = g.v1 - g.v0;
+        for (; left >= Stream::kStep; left -= Stream::kStep) {
+            uint4 raw[kU];
+            stream.template take<true>(raw, 0);
+            stream.issue();
+            use(raw, left == Stream::kStep);
         }
+        if (left > 0) {
+            uint4 raw[kU];
+            stream.template take<false>(raw, (left - tid + kThreads - 1) / kThreads);
+            stream.issue();
+            use(raw, true);
+        }
+        Sums r = run.sums(a.c);
         if constexpr (TOP) top.offer(r.m, parity);
         if (tid < ends) {
             const float x[1] = {end};
