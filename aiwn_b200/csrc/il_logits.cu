@@ -82,7 +82,7 @@ Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, bool twice) {
 
 template <class... P, class... A>
 int launch(void (*kern)(P...), unsigned grid, int threads, uint32_t lg, size_t smem, cudaStream_t s, A... args) {
-    if (smem > 40 * 1024 &&  // beyond 48 KB with the static arrays
+    if (smem > 16 * 1024 &&  // beyond 48 KB with the static arrays
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
         cudaGetLastError();
         return IL_ERR_LAUNCH;
@@ -168,7 +168,7 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
         return with_bool(k > 0, [&](auto top) {
             return with_threads(p.threads, [&](auto th) {
                 const size_t smem = RowStream<dt.value, th.value, 1>::kBytes +
-                                    (top.value ? 8 * (size_t)top_list(a.k, (int)p.lg) : 0);
+                                    (top.value ? 8 * (size_t)(top_list(a.k, (int)p.lg) + (p.lg ? a.k : 0)) : 0);
                 return launch(score_row_kernel<dt.value, th.value, top.value>, p.grid, th.value, p.lg, smem, s, a, p.lg);
             });
         });

@@ -8,12 +8,12 @@
 // backward reads it once more and writes its gradient.
 //
 // The k largest.  While a row goes by, each thread keeps the maximum of every
-// sixteenth of what it reads (rounded up to 16 bits, in shared memory), and
+// sixteenth (or eighth, or thirty-second) of what it reads, rounded up to 16 bits, and
 // nothing else is done for them.  Then, with W warps and j = k / W rounded up,
 // the least of the warps' j-th largest thread maxima is a bound that at least k
 // logits reach, and of a row in no particular order not many more; the few
-// sixteenths that reach it are read again, and their logits that reach it are
-// sorted.  Entries are (order-preserving bits of z) << 32 | ~index, so that all
+// of these that reach it are read again, and their logits that reach it are
+// ranked.  Entries are (order-preserving bits of z) << 32 | ~index, so that all
 // are distinct and equal logits go by their index.  Where more logits reach the
 // bound than the list holds, the k-th largest of those listed is a higher bound
 // for another round; where that is no higher, the list is of the logits above
@@ -145,11 +145,10 @@ __global__ void __launch_bounds__(256) score_warp_kernel(ScoreArgs a) {
 
 // ---- longer rows: a CTA, or a cluster of CTAs, a row --------------------------------
 
-// entries of the list of candidates: some times k; in a cluster k and those of 2^lg CTAs, to be sorted
+// entries of the list of candidates: some times k; in a cluster also the k of each of 2^lg CTAs
 __host__ __device__ constexpr int top_list(int k, int lg) {
-    int merge = 1, n = 512;
-    while (merge < k << lg) merge <<= 1;
-    while (lg && n < k + merge) n <<= 1;
+    int n = 512;
+    while (lg && n < k << lg) n <<= 1;
     return n;
 }
 
@@ -211,31 +210,51 @@ __device__ __forceinline__ uint16_t upper16(float v) {
     return (uint16_t)((v == INFINITY ? b : up) >> 16);
 }
 
-constexpr int kTopGroups = 16;
+// Sends every entry of list[0 .. n - 1] (all distinct) whose rank is below k to out(rank, entry): each is compared
+// with all, which for a few hundred entries takes no barrier and less time than sorting them.
+template <int kThreads, class Out>
+__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int k, Out out) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t x = list[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int m = 0; m < n; ++m) rank += list[m] > x;
+        if (rank < k) out(rank, x);
+    }
+}
+
+// the j-th largest of the lanes' values (j: 1 .. 32)
+__device__ __forceinline__ float warp_largest(float v, int j) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int d = size >> 1; d > 0; d >>= 1) {
+            const float y = __shfl_xor_sync(0xffffffffu, v, d);
+            v = ((lane & size) == 0) == ((lane & d) == 0) ? fmaxf(v, y) : fminf(v, y);
+        }
+    return __shfl_sync(0xffffffffu, v, j - 1);
+}
 
 template <int DT, int kThreads, int kU>
 struct Top {
     static constexpr int kVec = Elem<DT>::kVec, kWarps = kThreads / 32, kStep = kU * kThreads;
+    static constexpr int kGroups = 4096 / kThreads;  // of steps, that a row's steps are put into
     struct Shared {
-        uint16_t most[kTopGroups][kThreads];  // maxima of the groups of steps
-        uint16_t hits[kTopGroups * kThreads];
+        uint16_t most[kGroups][kThreads];       // maxima of the groups
+        uint16_t hits[kWarps][kGroups * 32];
         float deposit[2][kWarps];
         int scan[kWarps];
-        int count, hit_count;
+        int count;
     };
     using T = typename Elem<DT>::type;
     Shared* sh;
-    uint64_t* list;  // shared, room for cap entries
+    uint64_t* list;  // shared, room for cap entries and for k
     int k, cap;
 
     // the least of the warps' j-th largest of their lanes' values is left by two calls with a barrier between
     __device__ __forceinline__ void offer(float all, int parity) const {
-        float v = all, t = -INFINITY;
-        for (int j = 0; j < (k + kWarps - 1) / kWarps; ++j) {
-            t = warp_max(v);
-            const unsigned who = __ballot_sync(0xffffffffu, v == t);
-            if ((threadIdx.x & 31) == __ffs(who) - 1) v = NAN;  // no maximum takes it again
-        }
+        const float t = warp_largest(all, (k + kWarps - 1) / kWarps);
         if ((threadIdx.x & 31) == 0) sh->deposit[parity][threadIdx.x >> 5] = t;
     }
     __device__ __forceinline__ float bound(int parity) const {
@@ -250,30 +269,52 @@ struct Top {
         return above ? z > bound : z >= bound;  // not NaN
     }
 
-    // Lists the part's logits that reach the bound (above: that are above it); false: more than the list holds.
-    // lg: log2 of the steps of a group; end, end_at, ends: this thread's logit of the row's ends.
+    // Lists the part's logits that reach the bound (above: that are above it), sh->count of them; false: more than
+    // the list holds.  sh->count is 0.  lg: log2 of the steps of a group; end, end_at, ends: this thread's logit of
+    // the row's ends.
     __device__ __forceinline__ bool collect(const T* zr, const Segment& g, int lg, float end, int end_at, int ends,
                                             float bound, bool above) const {
-        const int tid = threadIdx.x;
+        const int tid = threadIdx.x, lane = tid & 31;
         const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
-        if (tid == 0) sh->count = 0, sh->hit_count = 0;
-        __syncthreads();
         const int groups = (g.v1 - g.v0 + (kStep << lg) - 1) / (kStep << lg);
-        for (int n = 0; n < groups; ++n)
-            if (reaches(__uint_as_float((uint32_t)sh->most[n][tid] << 16), bound, above))
-                sh->hits[atomicAdd(&sh->hit_count, 1)] = (uint16_t)(n * kThreads + tid);
+        uint16_t* hits = sh->hits[tid >> 5];  // of this warp
+        int n = 0;
+        for (int i = 0; i < groups; ++i) {
+            const bool hit = reaches(__uint_as_float((uint32_t)sh->most[i][tid] << 16), bound, above);
+            const unsigned who = __ballot_sync(0xffffffffu, hit);
+            if (hit) hits[n + __popc(who & ((1u << lane) - 1u))] = (uint16_t)(i * kThreads + tid);
+            n += __popc(who);
+        }
+        __syncwarp();
         if (tid < ends && reaches(end, bound, above)) put(end, end_at);
-        __syncthreads();
-        const int hits = sh->hit_count, per = kU << lg;
-        for (int n = tid; n < hits * per; n += kThreads) {
-            const int h = sh->hits[n / per], q = n % per;
-            const int v = g.v0 + ((h / kThreads << lg) + q / kU) * kStep + q % kU * kThreads + h % kThreads;
-            if (v >= g.v1) continue;
-            float x[kVec];
-            unpack16<DT>(__ldg(body + v), x);
+        // vector q of hit h is item (h << per) + q; four items of a lane are loaded at a time
+        const int per = 2 + lg, items = n << per;
+        static_assert(kU == 4, "a step of a group is 4 vectors");
+        for (int i = lane; i < items; i += 4 * 32) {
+            uint4 r[4];
+            int v[4];
 #pragma unroll
-            for (int e = 0; e < kVec; ++e)
-                if (reaches(x[e], bound, above)) put(x[e], g.h0 + v * kVec + e);
+            for (int w = 0; w < 4; ++w) {
+                const int item = i + w * 32;
+                v[w] = -1;
+                if (item < items) {
+                    const int h = hits[item >> per], q = item & ((1 << per) - 1);
+                    const int at = g.v0 + ((h / kThreads << lg) + q / kU) * kStep + q % kU * kThreads + h % kThreads;
+                    if (at < g.v1) {
+                        v[w] = at;
+                        r[w] = __ldg(body + at);
+                    }
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                if (v[w] < 0) continue;
+                float x[kVec];
+                unpack16<DT>(r[w], x);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e)
+                    if (reaches(x[e], bound, above)) put(x[e], g.h0 + v[w] * kVec + e);
+            }
         }
         __syncthreads();
         return sh->count <= cap;
@@ -324,9 +365,9 @@ struct Top {
         __syncthreads();
     }
 
-    // list[0 .. k - 1]: the largest of the part, sorted; 0 where it has fewer
-    __device__ __forceinline__ void find(const T* zr, const Segment& g, int lg, float end, int end_at, int ends,
-                                         float bound) const {
+    // list[0 .. result - 1] has the k largest of the part among few others; all of the part where it has fewer than k
+    __device__ __forceinline__ int find(const T* zr, const Segment& g, int lg, float end, int end_at, int ends,
+                                        float bound) const {
         bool above = bound == -INFINITY;
         while (!collect(zr, g, lg, end, end_at, ends, bound, above)) {
             sort_list<kThreads>(list, cap);
@@ -334,20 +375,15 @@ struct Top {
             above = !(b > bound);
             bound = b;
             __syncthreads();
+            if (threadIdx.x == 0) sh->count = 0;
+            __syncthreads();
         }
         if (above && sh->count < k) {
             const int need = k - sh->count;
             __syncthreads();
             fill(zr, g, bound, need);
         }
-        const int c = sh->count;
-        sort_list<kThreads>(list, c);
-        if (c < k) {
-            int p = 2;
-            while (p < c) p <<= 1;
-            for (int i = p + threadIdx.x; i < k; i += kThreads) list[i] = 0;
-            __syncthreads();
-        }
+        return sh->count;
     }
 };
 
@@ -370,6 +406,9 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) score_row_kernel(Sco
     const RowStep step(a.z, gridDim.x >> lg);
     Stream stream(a.z, a.V, list, step, rank, lg, sm);
     RowAt at(a.z, list.first);
+    if constexpr (TOP) {
+        if (tid == 0) top_shared.count = 0;
+    }
     uint32_t live = 0;
     int parity = 0;
     for (uint32_t i = 0; i < list.count; ++i, step.move(at, a.z.T)) {
@@ -384,13 +423,13 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) score_row_kernel(Sco
         const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
         const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
         float z_t = 0.0f;
-        if (tid == 0 && a.logprob) {
+        if (tid == kThreads - 1 && a.logprob) {
             const int64_t t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
             z_t = t >= 0 && t < a.V ? to_float(zr[t]) : NAN;
         }
-        int group_lg = 0;  // kTopGroups groups of 2^group_lg steps are enough
+        int group_lg = 0;  // kGroups groups of 2^group_lg steps are enough
         if constexpr (TOP)
-            while ((Stream::kStep * kTopGroups << group_lg) < g.v1 - g.v0) ++group_lg;
+            while ((Stream::kStep * TopOf::kGroups << group_lg) < g.v1 - g.v0) ++group_lg;
         Running<true, false> run;
         run.begin();
         float most = -INFINITY;
@@ -431,27 +470,51 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) score_row_kernel(Sco
         if constexpr (TOP) bound = top.bound(parity);
         if (ctas > 1) r = cluster_join<true, false>(r, &mine[parity], ctas, a.c);
         parity ^= 1;
-        if (rank == 0 && tid == 0) score_write(a, row, z_t, r);
         if constexpr (TOP) {
-            top.find(zr, g, group_lg, end, end_at, ends, bound);
-            uint64_t* best = top.list;
-            if (ctas > 1) {
+            const int c = top.find(zr, g, group_lg, end, end_at, ends, bound);
+            const float log_s = logf(r.s);
+            auto write = [&](int n, uint64_t x) {
+                a.top_index[(int64_t)row * a.k + n] = (uint32_t)~x;
+                a.top_logprob[(int64_t)row * a.k + n] = log_prob(key_value((uint32_t)(x >> 32)), r.m, r.s, log_s, a.tau);
+            };
+            if (ctas == 1) {
+                rank_list<kThreads>(top.list, c, a.k, write);
+            } else {
+                uint64_t* best = top.list + top.cap;  // of this CTA, sorted
+                for (int n = tid; n < a.k; n += kThreads)
+                    if (n >= c) best[n] = 0;
+                rank_list<kThreads>(top.list, c, a.k, [&](int n, uint64_t x) { best[n] = x; });
+                cluster_sync();
+                if (rank == 0)
+                    for (int n = tid; n < (int)ctas * a.k; n += kThreads)
+                        top.list[n] = ld_dsmem_u64(map_to_rank(smem_addr(best + n % a.k), n / a.k));
                 cluster_sync();
                 if (rank == 0) {
-                    best = top.list + a.k;
-                    for (int n = tid; n < (int)ctas * a.k; n += kThreads)
-                        best[n] = ld_dsmem_u64(map_to_rank(smem_addr(top.list + n % a.k), n / a.k));
+                    // an entry's rank is its place in its own list and, by halving, those in the others
+                    for (int n = tid; n < (int)ctas * a.k; n += kThreads) {
+                        const uint64_t x = top.list[n];
+                        if (x == 0) continue;
+                        int place = n % a.k;
+                        for (int q = 0; q < (int)ctas && place < a.k; ++q) {
+                            if (q == n / a.k) continue;
+                            const uint64_t* other = top.list + q * a.k;
+                            int lo = 0, hi = a.k;
+                            while (lo < hi) {
+                                const int mid = (lo + hi) >> 1;
+                                if (other[mid] > x) lo = mid + 1;
+                                else hi = mid;
+                            }
+                            place += lo;
+                        }
+                        if (place < a.k) write(place, x);
+                    }
                 }
-                cluster_sync();
-                if (rank == 0) sort_list<kThreads>(best, (int)ctas * a.k);
             }
-            if (rank == 0 && tid < a.k) {
-                const float log_s = logf(r.s);
-                a.top_index[(int64_t)row * a.k + tid] = (uint32_t)~best[tid];
-                a.top_logprob[(int64_t)row * a.k + tid] =
-                    log_prob(key_value((uint32_t)(best[tid] >> 32)), r.m, r.s, log_s, a.tau);
-            }
+            if (rank == 0 && tid == kThreads - 1) score_write(a, row, z_t, r);
             __syncthreads();
+            if (tid == 0) top_shared.count = 0;
+        } else {
+            if (rank == 0 && tid == kThreads - 1) score_write(a, row, z_t, r);
         }
     }
     if (ctas > 1) cluster_sync();  // no CTA ends while another may still read its shared memory
@@ -569,13 +632,12 @@ __global__ void __launch_bounds__(kGradThreads, 2) score_grad_row_kernel(ScoreGr
     ScoreGrad r;
     if (live) r = score_grad_row(a, row, t);
     const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
-    for (int v = g.v0 + tid; v < g.v1; v += kGradThreads) {
+    auto write = [&](int v, const uint4& raw) {
         float y[kVec];
         if (live) {
-            float x[kVec];
-            unpack16<DT>(__ldcs(body + v), x);
+            unpack16<DT>(raw, y);
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) y[e] = r.at(x[e]) * r.inv_tau;
+            for (int e = 0; e < kVec; ++e) y[e] = r.at(y[e]) * r.inv_tau;
         } else {
 #pragma unroll
             for (int e = 0; e < kVec; ++e) y[e] = 0.0f;
@@ -587,6 +649,16 @@ __global__ void __launch_bounds__(kGradThreads, 2) score_grad_row_kernel(ScoreGr
 #pragma unroll
             for (int e = 0; e < kVec; ++e) to[e] = from_float<T>(y[e]);
         }
+    };
+    constexpr int kAhead = 4;  // vectors of a thread that are loaded at a time
+    for (int v = g.v0 + tid; v < g.v1; v += kAhead * kGradThreads) {
+        uint4 raw[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (live && v + u * kGradThreads < g.v1) raw[u] = __ldcs(body + v + u * kGradThreads);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (v + u * kGradThreads < g.v1) write(v + u * kGradThreads, raw[u]);
     }
     if (tid < g.head) dr[tid] = from_float<T>(live ? r.at(to_float(zr[tid])) * r.inv_tau : 0.0f);
     if (tid < g.tail) dr[g.t0 + tid] = from_float<T>(live ? r.at(to_float(zr[g.t0 + tid])) * r.inv_tau : 0.0f);
