@@ -119,11 +119,17 @@ def _check(rc: int, what: str):
 
 
 def _p(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
+
+
+# the current stream's handle of a device index, without a Stream object where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _stream(dev: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    if _raw_stream is not None and dev.index is not None:
+        return _raw_stream(dev.index)
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
 def _need_cuda(*ts):
@@ -414,11 +420,11 @@ def token_logprobs(logits, tokens, ignore_index: int, temperature: float, logpro
     """logprob, entropy [B, T] and top_index, top_logprob [B, T, k] <- logits [B, T, V] (rows with any strides) and
     tokens [B, T] (or None, with logprob None); stats [B, T, 2] for the backward, or None."""
     _same_device(logits, tokens, logprob, entropy, stats, top_index, top_logprob)
-    B, T, V, sb, st = _logit_rows("logits", logits)
+    B, T, V, _, _ = _logit_rows("logits", logits)
     k = top_index.shape[-1]
     if k > min(V, MAX_TOP):
         raise ILError(f"top_k {k}: at most {MAX_TOP}, and no more than the {V} logits of a row")
-    tb, tt = _token_strides("tokens", tokens, B, T)
+    _token_strides("tokens", tokens, B, T)
     _expect("logprob", logprob, (B, T))
     if tokens is not None and logprob is None:
         raise ILError("tokens without an output for their log probabilities")
@@ -428,11 +434,22 @@ def token_logprobs(logits, tokens, ignore_index: int, temperature: float, logpro
     _expect("top_logprob", top_logprob, (B, T, k))
     _on_cuda(logits, tokens)
     _need_cuda(logprob, entropy, stats, top_index, top_logprob)
-    lib = load()
-    with _on_device(logits.device):
-        _check(lib.il_token_logprobs(_p(logits), x_dtype_code(logits), B, T, V, sb, st, _p(tokens), tb, tt,
-                                     int(ignore_index), k, float(temperature), _p(logprob), _p(entropy), _p(stats),
-                                     _p(top_index), _p(top_logprob), _stream(logits.device)), "il_token_logprobs")
+    run_token_logprobs(logits, tokens, ignore_index, temperature, k, logprob, entropy, stats, top_index, top_logprob)
+
+
+def run_token_logprobs(logits, tokens, ignore_index, temperature, k, logprob, entropy, stats, top_index, top_logprob):
+    """token_logprobs of operands that have been checked."""
+    B, T, V = logits.shape
+    sb, st, _ = logits.stride()
+    tb, tt = tokens.stride() if tokens is not None else (0, 0)
+    dev = logits.device
+    lib = _lib or load()
+    with _on_device(dev):
+        rc = lib.il_token_logprobs(_p(logits), _DTYPES[logits.dtype], B, T, V, sb, st, _p(tokens), tb, tt,
+                                   ignore_index, k, temperature, _p(logprob), _p(entropy), _p(stats), _p(top_index),
+                                   _p(top_logprob), _stream(dev))
+    if rc:
+        _check(rc, "il_token_logprobs")
 
 
 def token_logprobs_backward(logits, tokens, ignore_index: int, temperature: float, entropy, stats, top_index,
@@ -440,13 +457,13 @@ def token_logprobs_backward(logits, tokens, ignore_index: int, temperature: floa
     """dlogits [B, T, V] <- gradient of token_logprobs from g_logprob, g_entropy [B, T] and g_top [B, T, k] (each may
     be None)."""
     _same_device(logits, tokens, entropy, stats, top_index, g_logprob, g_entropy, g_top, dlogits)
-    B, T, V, sb, st = _logit_rows("logits", logits)
+    B, T, V, _, _ = _logit_rows("logits", logits)
     k = top_index.shape[-1]
     if k > min(V, MAX_TOP):
         raise ILError(f"top_k {k}: at most {MAX_TOP}, and no more than the {V} logits of a row")
-    tb, tt = _token_strides("tokens", tokens, B, T)
+    _token_strides("tokens", tokens, B, T)
     _expect("dlogits", dlogits, (B, T, V), logits.dtype)
-    *_, db, dt = _logit_rows("dlogits", dlogits)
+    _logit_rows("dlogits", dlogits)
     for name, t in (("entropy", entropy), ("g_logprob", g_logprob), ("g_entropy", g_entropy)):
         _expect(name, t, (B, T))
     if g_logprob is not None and tokens is None:
@@ -456,12 +473,26 @@ def token_logprobs_backward(logits, tokens, ignore_index: int, temperature: floa
     _expect("g_top", g_top, (B, T, k))
     _on_cuda(logits, tokens, dlogits)
     _need_cuda(entropy, stats, top_index, g_logprob, g_entropy, g_top)
-    lib = load()
-    with _on_device(logits.device):
-        _check(lib.il_token_logprobs_backward(
-            _p(logits), x_dtype_code(logits), B, T, V, sb, st, _p(tokens), tb, tt, int(ignore_index), k,
-            float(temperature), _p(entropy), _p(stats), _p(top_index), _p(g_logprob), _p(g_entropy), _p(g_top),
-            _p(dlogits), db, dt, _stream(logits.device)), "il_token_logprobs_backward")
+    run_token_logprobs_backward(logits, tokens, ignore_index, temperature, k, entropy, stats, top_index, g_logprob,
+                                g_entropy, g_top, dlogits)
+
+
+def run_token_logprobs_backward(logits, tokens, ignore_index, temperature, k, entropy, stats, top_index, g_logprob,
+                                g_entropy, g_top, dlogits):
+    """token_logprobs_backward of operands that have been checked."""
+    B, T, V = logits.shape
+    sb, st, _ = logits.stride()
+    db, dt, _ = dlogits.stride()
+    tb, tt = tokens.stride() if tokens is not None else (0, 0)
+    dev = logits.device
+    lib = _lib or load()
+    with _on_device(dev):
+        rc = lib.il_token_logprobs_backward(
+            _p(logits), _DTYPES[logits.dtype], B, T, V, sb, st, _p(tokens), tb, tt, ignore_index, k, temperature,
+            _p(entropy), _p(stats), _p(top_index), _p(g_logprob), _p(g_entropy), _p(g_top), _p(dlogits), db, dt,
+            _stream(dev))
+    if rc:
+        _check(rc, "il_token_logprobs_backward")
 
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -477,7 +508,7 @@ def distill(logits, top_index, top_logprob, targets, ignore_index: int, alpha: f
     logits [B, T, V] from the teacher's top_index (int64) and top_logprob [B, T, k]; the gradient is multiplied by g
     (like loss, on the device; None: 1), and nothing is written where only_if_not_one is set and g is 1."""
     _same_device(logits, top_index, top_logprob, targets, loss, dlogits, workspace, g)
-    B, T, V, sb, st = _logit_rows("logits", logits)
+    B, T, V, _, _ = _logit_rows("logits", logits)
     if reduction not in REDUCTIONS:
         raise ILError(f"reduction {reduction!r}: one of {sorted(REDUCTIONS)}")
     if top_index.dim() != 3 or top_index.shape[2] > MAX_TOP:
@@ -485,27 +516,39 @@ def distill(logits, top_index, top_logprob, targets, ignore_index: int, alpha: f
     k = top_index.shape[2]
     _expect("top_index", top_index, (B, T, k), torch.int64)
     _expect("top_logprob", top_logprob, (B, T, k))
-    tb, tt = _token_strides("targets", targets, B, T)
+    _token_strides("targets", targets, B, T)
     if alpha < 1.0 and targets is None:
         raise ILError(f"alpha {alpha} < 1 needs targets")
     shape = (B, T) if reduction == "none" else ()
     _expect("loss", loss, shape)
     _expect("g", g, shape)
-    db = dt = 0
     if dlogits is not None:
         _expect("dlogits", dlogits, (B, T, V), logits.dtype)
-        *_, db, dt = _logit_rows("dlogits", dlogits)
+        _logit_rows("dlogits", dlogits)
     if workspace is not None and workspace.dtype != torch.uint8:
         raise ILError("workspace must be a uint8 tensor")
     _on_cuda(logits, targets, dlogits)
     _need_cuda(top_index, top_logprob, loss, workspace, g)
-    lib = load()
-    with _on_device(logits.device):
-        _check(lib.il_distill(
-            _p(logits), x_dtype_code(logits), B, T, V, sb, st, _p(top_index), _p(top_logprob), k, _p(targets), tb, tt,
-            int(ignore_index), float(alpha), float(temperature), int(bool(tail)), REDUCTIONS[reduction], _p(g),
-            int(bool(only_if_not_one)), _p(loss), _p(dlogits), db, dt, _p(workspace),
-            0 if workspace is None else workspace.numel(), _stream(logits.device)), "il_distill")
+    run_distill(logits, top_index, top_logprob, targets, ignore_index, alpha, temperature, int(bool(tail)),
+                REDUCTIONS[reduction], loss, dlogits, workspace, g, int(bool(only_if_not_one)))
+
+
+def run_distill(logits, top_index, top_logprob, targets, ignore_index, alpha, temperature, tail, reduction, loss,
+                dlogits, workspace, g=None, only_if_not_one=0):
+    """distill of operands that have been checked; reduction by its number."""
+    B, T, V = logits.shape
+    sb, st, _ = logits.stride()
+    tb, tt = targets.stride() if targets is not None else (0, 0)
+    db, dt, _ = dlogits.stride() if dlogits is not None else (0, 0, 0)
+    dev = logits.device
+    lib = _lib or load()
+    with _on_device(dev):
+        rc = lib.il_distill(_p(logits), _DTYPES[logits.dtype], B, T, V, sb, st, _p(top_index), _p(top_logprob),
+                            top_index.shape[2], _p(targets), tb, tt, ignore_index, alpha, temperature, tail, reduction,
+                            _p(g), only_if_not_one, _p(loss), _p(dlogits), db, dt, _p(workspace),
+                            0 if workspace is None else workspace.numel(), _stream(dev))
+    if rc:
+        _check(rc, "il_distill")
 
 
 def bin_counts(x, K: int, bw: float, counts):

@@ -255,7 +255,7 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
             if (targets) a.scale_p = ws;
             else a.scale = 1.0f / (float)(N > 1 ? N : 1);
         }
-        if (loss || a.scale_p)
+        if (loss)
             if ((st = launch(distill_begin_kernel, 1, 1024, 0, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
     }
     const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits != nullptr) : Plan{1, 256, 0, 1};

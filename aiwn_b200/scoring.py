@@ -37,30 +37,39 @@ class TokenScores(NamedTuple):
 
 def _rows(logits):
     """logits as [B, T, V] rows that the kernels can read, without a copy where the strides allow it."""
-    if logits.dim() < 1:
-        raise ILError("logits must be [..., V]")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ILError(f"logits must be [..., V] with V >= 1, got shape {tuple(logits.shape)}")
+    _lib.x_dtype_code(logits)
     V = logits.shape[-1]
+    if V > _lib.MAX_VOCAB:
+        raise ILError(f"logits: {V} logits a row, at most {_lib.MAX_VOCAB}")
     if V > 1 and logits.stride(-1) != 1:
         logits = logits.contiguous()
-    if logits.dim() == 1:
-        return logits[None, None]
-    if logits.dim() == 2:
-        return logits[None]
-    return logits if logits.dim() == 3 else logits.reshape(1, -1, V)
+    d = logits.dim()
+    return logits if d == 3 else logits[None] if d == 2 else logits[None, None] if d == 1 else logits.reshape(1, -1, V)
 
 
 def _per_row(name, t, lead, rows, dtype):
     """t [*lead, ...] as [B, T, ...] like the rows."""
     if t.dtype != dtype:
         raise ILError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if tuple(t.shape[:len(lead)]) != tuple(lead):
+    if t.shape[:len(lead)] != lead:
         raise ILError(f"{name}: shape {tuple(t.shape)} for logits over {tuple(lead)}")
-    return t.reshape(*rows.shape[:2], *t.shape[len(lead):])
+    if t.device != rows.device:
+        raise ILError(f"tensors on different devices: {name} on {t.device}, the logits on {rows.device}")
+    return t if len(lead) == 2 else t.reshape(*rows.shape[:2], *t.shape[len(lead):])
+
+
+def _need_cuda(rows):
+    if not rows.is_cuda:
+        raise ILError("aiwn_b200 kernels need CUDA tensors; there is no CPU path")
 
 
 def _gradient_like(rows):
     """Room for the gradient of rows, its rows aligned to 16 bytes as those of the logits are where it can be had by
     padding rows to less than 16 bytes (then the kernels load and store the same 16-byte vectors)."""
+    if rows.is_contiguous() and rows.data_ptr() % 16 == 0:
+        return torch.empty_like(rows)
     B, T, V = rows.shape
     n = 16 // rows.element_size()
     start = rows.data_ptr() // rows.element_size() % n
@@ -77,41 +86,46 @@ def _temperature(t):
     return t
 
 
-def _score(rows, tokens, k, temperature, ignore_index, with_stats):
-    B, T, V = rows.shape
-    if not 0 <= k <= min(V, _lib.MAX_TOP):
-        raise ILError(f"top_k {k}: at most {_lib.MAX_TOP}, and no more than the {V} logits of a row")
-    new = dict(dtype=torch.float32, device=rows.device)
-    logprob = torch.empty(B, T, **new) if tokens is not None else None
-    entropy = torch.empty(B, T, **new)
-    stats = torch.empty(B, T, 2, **new) if with_stats else None
-    index = torch.empty(B, T, k, dtype=torch.int64, device=rows.device)
-    top = torch.empty(B, T, k, **new)
-    _lib.token_logprobs(rows, tokens, ignore_index, temperature, logprob, entropy, stats, index, top)
-    return logprob, entropy, stats, index, top
+def _score(rows, tokens, k, temperature, ignore_index, lead, with_stats):
+    """(logprob, entropy, top_index, top_logprob) over the leading dimensions `lead`, and stats or None."""
+    dev = rows.device
+    logprob = torch.empty(lead, dtype=torch.float32, device=dev) if tokens is not None else None
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    index = torch.empty((*lead, k), dtype=torch.int64, device=dev)
+    top = torch.empty((*lead, k), dtype=torch.float32, device=dev)
+    stats = torch.empty((*lead, 2), dtype=torch.float32, device=dev) if with_stats else None
+    _lib.run_token_logprobs(rows, tokens, ignore_index, temperature, k, logprob, entropy, stats, index, top)
+    return logprob, entropy, index, top, stats
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, tokens, k, temperature, ignore_index):
-        logprob, entropy, stats, index, top = _score(rows, tokens, k, temperature, ignore_index, True)
+    def forward(ctx, rows, tokens, k, temperature, ignore_index, lead):
+        logprob, entropy, index, top, stats = _score(rows, tokens, k, temperature, ignore_index, lead, True)
         ctx.save_for_backward(rows, tokens, entropy, stats, index)
-        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        ctx.opts = k, temperature, ignore_index
         ctx.mark_non_differentiable(index)
         ctx.set_materialize_grads(False)
         return logprob, entropy, index, top
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprob, g_entropy, _, g_top):
+    def _grad(ctx, g_logprob, g_entropy, _, g_top):
         rows, tokens, entropy, stats, index = ctx.saved_tensors
         if g_logprob is None and g_entropy is None and g_top is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         g_logprob, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logprob, g_entropy, g_top))
+        k, temperature, ignore_index = ctx.opts
         d = _gradient_like(rows)
-        _lib.token_logprobs_backward(rows, tokens, ctx.ignore_index, ctx.temperature, entropy, stats, index,
-                                     g_logprob, g_entropy, g_top, d)
-        return d, None, None, None, None
+        _lib.run_token_logprobs_backward(rows, tokens, ignore_index, temperature, k, entropy, stats, index, g_logprob,
+                                         g_entropy, g_top, d)
+        return d, None, None, None, None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_grad.__func__))
+
+    @staticmethod
+    def backward(ctx, *g):
+        # once_differentiable only matters, and is only paid for, under create_graph=True
+        return _TokenLogprobs._once(ctx, *g) if torch.is_grad_enabled() else _TokenLogprobs._grad(ctx, *g)
 
 
 def token_logprobs(logits, tokens=None, top_k: int = 0, *, temperature: float = 1.0,
@@ -120,19 +134,19 @@ def token_logprobs(logits, tokens=None, top_k: int = 0, *, temperature: float = 
     entropy of each row and its ``top_k`` (at most 128) largest alternatives.
 
     ``tokens=None`` leaves the log probabilities out.  Rows whose token is ``ignore_index`` are padding: log
-    probability 0, entropy 0, alternatives -1 at -inf, no gradient; their logits are not read.  A row whose logits are
-    all -inf gives log probability -inf and entropy 0; a token outside [0, V), a NaN or a +inf logit gives NaN.
+    probability 0, entropy 0, alternatives -1 at -inf, no gradient.  A row whose logits are all -inf gives log
+    probability -inf and entropy 0; a token outside [0, V), a NaN or a +inf logit gives NaN.
     The gradient of the logits is that of all three floating results (not twice differentiable)."""
     rows = _rows(logits)
     lead = logits.shape[:-1]
-    temperature = _temperature(temperature)
+    temperature, k, ignore_index = _temperature(temperature), int(top_k), int(ignore_index)
+    if not 0 <= k <= min(rows.shape[2], _lib.MAX_TOP):
+        raise ILError(f"top_k {k}: at most {_lib.MAX_TOP}, and no more than the {rows.shape[2]} logits of a row")
     tok = None if tokens is None else _per_row("tokens", tokens, lead, rows, torch.int64)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        logprob, entropy, index, top = _TokenLogprobs.apply(rows, tok, int(top_k), temperature, int(ignore_index))
-    else:
-        logprob, entropy, _, index, top = _score(rows, tok, int(top_k), temperature, int(ignore_index), False)
-    return TokenScores(None if logprob is None else logprob.reshape(lead), entropy.reshape(lead),
-                       index.reshape(*lead, index.shape[-1]), top.reshape(*lead, top.shape[-1]))
+    _need_cuda(rows)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenScores(*_TokenLogprobs.apply(rows, tok, k, temperature, ignore_index, lead))
+    return TokenScores(*_score(rows, tok, k, temperature, ignore_index, lead, False)[:4])
 
 
 class _Distill(torch.autograd.Function):
@@ -141,32 +155,38 @@ class _Distill(torch.autograd.Function):
     of the same graph gets a tensor of its own.  "none" writes the gradient in the backward."""
 
     @staticmethod
-    def forward(ctx, rows, index, logprob, targets, opts):
-        loss, d, ws = _distill(rows, index, logprob, targets, opts, opts["reduction"] != "none")
+    def forward(ctx, rows, index, logprob, targets, opts, lead):
+        loss, d, ws = _distill(rows, index, logprob, targets, opts, lead, opts[4] != 0)
         ctx.save_for_backward(rows, index, logprob, targets)
         ctx.opts, ctx.d, ctx.ws = opts, d, ws
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
+    def _grad(ctx, g):
         rows, index, logprob, targets = ctx.saved_tensors
         d, ctx.d = ctx.d, None
         ready = d is not None
         if not ready:
             d = _gradient_like(rows)
-        _lib.distill(rows, index, logprob, targets, loss=None, dlogits=d, workspace=ctx.ws, g=g.contiguous(),
-                     only_if_not_one=ready, **ctx.opts)
-        return d, None, None, None, None
+        _lib.run_distill(rows, index, logprob, targets, *ctx.opts, None, d, ctx.ws, g.contiguous(), int(ready))
+        return d, None, None, None, None, None
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_grad.__func__))
+
+    @staticmethod
+    def backward(ctx, g):
+        # once_differentiable only matters, and is only paid for, under create_graph=True
+        return _Distill._once(ctx, g) if torch.is_grad_enabled() else _Distill._grad(ctx, g)
 
 
-def _distill(rows, index, logprob, targets, opts, gradient):
-    B, T, _ = rows.shape
-    each = opts["reduction"] == "none"
-    loss = torch.empty((B, T) if each else (), dtype=torch.float32, device=rows.device)
-    ws = None if each else torch.empty(_lib.distill_workspace_bytes(B * T), dtype=torch.uint8, device=rows.device)
+def _distill(rows, index, logprob, targets, opts, lead, gradient):
+    whole = opts[4] != 0
+    loss = torch.empty(() if whole else lead, dtype=torch.float32, device=rows.device)
+    ws = None
+    if whole:
+        ws = torch.empty(_lib.distill_workspace_bytes(loss.numel()), dtype=torch.uint8, device=rows.device)
     d = _gradient_like(rows) if gradient else None
-    _lib.distill(rows, index, logprob, targets, loss=loss, dlogits=d, workspace=ws, **opts)
+    _lib.run_distill(rows, index, logprob, targets, *opts, loss, d, ws)
     return loss, d, ws
 
 
@@ -192,13 +212,17 @@ def distill_loss(logits, top_index, top_logprob, targets=None, *, alpha: float =
         raise ILError(f"alpha {alpha}: between 0 and 1")
     if reduction not in _lib.REDUCTIONS:
         raise ILError(f"reduction {reduction!r}: one of {sorted(_lib.REDUCTIONS)}")
+    if alpha < 1.0 and targets is None:
+        raise ILError(f"alpha {alpha} < 1 needs targets")
+    if top_index.dim() != len(lead) + 1 or top_index.shape[-1] > _lib.MAX_TOP:
+        raise ILError(f"top_index must be [..., k] with k <= {_lib.MAX_TOP}, got shape {tuple(top_index.shape)}")
+    if top_logprob.shape != top_index.shape:
+        raise ILError(f"top_logprob: shape {tuple(top_logprob.shape)}, expected {tuple(top_index.shape)}")
     index = _per_row("top_index", top_index, lead, rows, torch.int64).contiguous()
-    logprob = _per_row("top_logprob", top_logprob.detach(), lead, rows, torch.float32).contiguous()
+    logprob = _per_row("top_logprob", top_logprob, lead, rows, torch.float32).detach().contiguous()
     tgt = None if targets is None else _per_row("targets", targets, lead, rows, torch.int64)
-    opts = dict(ignore_index=int(ignore_index), alpha=alpha, temperature=_temperature(temperature), tail=bool(tail),
-                reduction=reduction)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        loss = _Distill.apply(rows, index, logprob, tgt, opts)
-    else:
-        loss, _, _ = _distill(rows, index, logprob, tgt, opts, False)
-    return loss.reshape(lead) if reduction == "none" else loss
+    opts = (int(ignore_index), alpha, _temperature(temperature), int(bool(tail)), _lib.REDUCTIONS[reduction])
+    _need_cuda(rows)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Distill.apply(rows, index, logprob, tgt, opts, lead)
+    return _distill(rows, index, logprob, tgt, opts, lead, False)[0]

@@ -259,7 +259,9 @@ IL_API int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, 
  * reduction 0; NULL: 1).  With only_if_not_one, nothing is written to loss or
  * dlogits when *g == 1.  A slot index >= V or, with alpha < 1, a target
  * outside [0, V) makes the row NaN.  workspace: il_distill_workspace_bytes(N)
- * (reduction 1 and 2), 16-byte aligned, used until the call's kernels end.
+ * (reduction 1 and 2), 16-byte aligned, used until the call's kernels end; a
+ * call without loss reads the number of rows from it, so that it takes the
+ * workspace of a call with loss on the same targets.
  */
 IL_API int64_t il_distill_workspace_bytes(int64_t N);
 IL_API int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, int64_t stride_b,
