@@ -64,6 +64,11 @@ struct SlotSums {
     int bad, pad;
 };
 
+// a barrier of the warps that keep the slots
+__device__ __forceinline__ void slot_barrier(int threads) {
+    asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+}
+
 template <bool TAIL>
 __device__ __forceinline__ float slot_weight(float l, float top) {
     return TAIL ? expf(l) : expf(l - top);
@@ -111,30 +116,12 @@ __device__ __forceinline__ SlotSums slot_sums(const DistillArgs& a, const Slot (
 // at one that slots name: 2^((z - h1) c) inside + 2^((z - h1) log2 e) coef1 - soft sum of the slots' weights;
 // less `hard` at the target.
 struct DistillRow {
-    float loss, h, coef, h1, coef1, inside, soft, hard, top, c;
+    float h, coef, h1, coef1, inside, soft, hard, top, c;
     template <bool S1>
     __device__ __forceinline__ float at(float z) const {
         float y = exp2_approx((z - h) * c) * coef;
         if constexpr (S1) y = fmaf(exp2_approx((z - h1) * kLog2e), coef1, y);
         return y;
-    }
-    // at() of n values, in place
-    template <bool S1, int n>
-    __device__ __forceinline__ void at_all(float (&x)[n]) const {
-        const uint64_t hh = pack2(-h, -h), cc = pack2(c, c), co = pack2(coef, coef);
-        const uint64_t hh1 = pack2(-h1, -h1), cc1 = pack2(kLog2e, kLog2e), co1 = pack2(coef1, coef1);
-#pragma unroll
-        for (int i = 0; i < n; i += 2) {
-            const uint64_t z = pack2(x[i], x[i + 1]);
-            float d, f;
-            unpack2(mul2(add2(z, hh), cc), d, f);
-            uint64_t y = mul2(pack2(exp2_approx(d), exp2_approx(f)), co);
-            if constexpr (S1) {
-                unpack2(mul2(add2(z, hh1), cc1), d, f);
-                y = fma2(pack2(exp2_approx(d), exp2_approx(f)), co1, y);
-            }
-            unpack2(y, x[i], x[i + 1]);
-        }
     }
     template <bool S1>
     __device__ __forceinline__ float at_slot(float z, float weight) const {
@@ -144,84 +131,116 @@ struct DistillRow {
     }
 };
 
-// s: the sums of the row, or of what no slot names (tail); part: the slots' of `parts` warps;
-// z_t: the target's logit, NaN for one outside the vocabulary
-template <bool TAIL, bool S1>
-__device__ __forceinline__ DistillRow distill_row(const DistillArgs& a, uint32_t row, Sums s, const SlotSums* part,
-                                                  int parts, float z_t, bool gradient) {
-    DistillRow r;
-    float top = 0.0f, mass = 0.0f;
-    bool bad = false;
-    if constexpr (!TAIL) {
-        top = -INFINITY;
-        for (int n = 0; n < parts; ++n)
-            if (part[n].mass != 0.0f) top = fmaxf(top, part[n].top);
-        top = shift_of(top);
+// at() of many values, (z - h) c as one fused multiply-add: with b = -h c rounded and r = h c + b exactly, the
+// exponential of z c + b is 2^r too large, which the factor takes back.  Not where |h| c is 2^22 or more.
+template <bool S1>
+struct DistillMany {
+    float c, b, f, b1, f1;
+    bool huge;
+    __device__ __forceinline__ explicit DistillMany(const DistillRow& r) : c(r.c) {
+        b = -(r.h * c);
+        f = r.coef * fmaf(fmaf(r.h, c, b), -kLn2, 1.0f);
+        b1 = -(r.h1 * kLog2e);
+        f1 = r.coef1 * fmaf(fmaf(r.h1, kLog2e, b1), -kLn2, 1.0f);
+        huge = !(fabsf(b) < 4194304.0f) || (S1 && !(fabsf(b1) < 4194304.0f));
     }
-    const Sums rest = s;
-    double left = 0.0;
-    for (int n = 0; n < parts; ++n) {
-        bad |= part[n].bad != 0;
-        const float f = TAIL ? 1.0f : part[n].mass != 0.0f ? expf(part[n].top - top) : 0.0f;
-        mass = fmaf(part[n].mass, f, mass);
-        if constexpr (TAIL) {
-            s = join<false, S1>(s, part[n].s, a.c);
-            left += part[n].left;
+    template <int n>
+    __device__ __forceinline__ void operator()(const DistillRow& r, float (&x)[n]) const {
+        if (huge) {
+#pragma unroll
+            for (int i = 0; i < n; ++i) x[i] = r.template at<S1>(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const float z = x[i];
+                x[i] = exp2_approx(fmaf(z, c, b)) * f;
+                if constexpr (S1) x[i] = fmaf(exp2_approx(fmaf(z, kLog2e, b1)), f1, x[i]);
+            }
         }
     }
-    const float h = shift_of(s.m);
-    const float inv_mass = TAIL ? 1.0f : mass != 0.0f ? 1.0f / mass : 0.0f;  // NaN stays
-    left = 1.0 - left;
-    const float q_rest = !TAIL || left < 0.0 ? 0.0f : (float)left;  // NaN stays
-    const float Q = TAIL ? (left < 0.0 ? mass : 1.0f + 0.0f * q_rest) : mass != 0.0f ? 1.0f + 0.0f * mass : 0.0f;
-    r.c = a.c;
-    r.h1 = h;
-    r.top = top;
-    const float s1 = S1 ? s.s1 : s.s;
-    {
-        const float log_s = logf(s.s);
+};
+
+// What a row's sums and its slots' come to.  s: the sums of the row, or of what no slot names (tail); part: the
+// slots' of `parts` warps; z_t: the target's logit, NaN for one outside the vocabulary
+template <bool TAIL, bool S1>
+struct DistillSums {
+    Sums s, rest;
+    float top, mass, inv_mass, q_rest, Q;
+    bool bad;
+
+    __device__ __forceinline__ DistillSums(const DistillArgs& a, Sums sums, const SlotSums* part, int parts, float z_t)
+        : s(sums), rest(sums) {
+        top = 0.0f, mass = 0.0f;
+        bad = a.hard && z_t != z_t;
+        if constexpr (!TAIL) {
+            top = -INFINITY;
+            for (int n = 0; n < parts; ++n)
+                if (part[n].mass != 0.0f) top = fmaxf(top, part[n].top);
+            top = shift_of(top);
+        }
+        double left = 1.0;
+        for (int n = 0; n < parts; ++n) {
+            bad |= part[n].bad != 0;
+            mass = fmaf(part[n].mass, weight_of(part[n]), mass);
+            if constexpr (TAIL) {
+                s = join<false, S1>(s, part[n].s, a.c);
+                left -= part[n].left;
+            }
+        }
+        inv_mass = TAIL ? 1.0f : mass != 0.0f ? 1.0f / mass : 0.0f;  // NaN stays
+        q_rest = !TAIL || left < 0.0 ? 0.0f : (float)left;           // NaN stays
+        Q = TAIL ? (left < 0.0 ? mass : 1.0f + 0.0f * q_rest) : mass != 0.0f ? 1.0f + 0.0f * mass : 0.0f;
+    }
+    // of a warp's slots next to the others'
+    __device__ __forceinline__ float weight_of(const SlotSums& p) const {
+        return TAIL ? 1.0f : p.mass != 0.0f ? expf(p.top - top) : 0.0f;
+    }
+
+    __device__ __forceinline__ DistillRow gradient(const DistillArgs& a, uint32_t row) const {
+        DistillRow r;
+        float w = a.scale * (a.scale_p ? *a.scale_p : 1.0f) * (a.g ? a.g[a.g_rows ? row : 0] : 1.0f);
+        if (bad) w = NAN;
+        const float s1 = S1 ? s.s1 : s.s;
+        const float soft = w * a.alpha * a.tau, hard = a.hard ? w * (1.0f - a.alpha) : 0.0f;
+        const float inv = s.s == 0.0f ? 0.0f : 1.0f / s.s;
+        r.c = a.c;
+        r.h1 = shift_of(s.m);
+        r.top = top;
+        r.soft = soft * inv_mass;
+        r.hard = hard;
+        r.coef1 = S1 ? hard * (s1 == 0.0f ? 0.0f : 1.0f / s1) : 0.0f;
+        r.inside = soft * Q * inv + (S1 ? 0.0f : hard * inv);
+        if constexpr (TAIL) {
+            const float f = exp2_approx(exponent(rest.m, r.h1, a.c));
+            r.h = shift_of(rest.m);
+            r.coef = rest.s == 0.0f ? 0.0f * w : f * r.inside - soft * q_rest / rest.s;
+        } else {
+            r.h = r.h1;
+            r.coef = r.inside;
+        }
+        return r;
+    }
+
+    __device__ __forceinline__ float loss(const DistillArgs& a, const SlotSums* part, int parts, float z_t) const {
+        const float h = shift_of(s.m), s1 = S1 ? s.s1 : s.s, log_s = logf(s.s);
         // sum q (ln q - (z - h) / tau), then + sum q (ln s)
         float kl = 0.0f, used = 0.0f;
         for (int n = 0; n < parts; ++n) {
-            if (part[n].mass == 0.0f) continue;
-            const float f = TAIL ? 1.0f : expf(part[n].top - top);
-            if (f == 0.0f) continue;
+            const float f = weight_of(part[n]);
+            if (part[n].mass == 0.0f || f == 0.0f) continue;
             const float q = part[n].mass * f * inv_mass;
             kl += part[n].cross * f * inv_mass + q * ((TAIL ? 0.0f : part[n].top - top) - (part[n].base - h) / a.tau);
             used += q;
         }
         if (used != 0.0f) kl += used * (s.s == 0.0f ? INFINITY : log_s - (TAIL ? 0.0f : logf(mass)));
-        const float hr = shift_of(rest.m);
         if (TAIL && q_rest != 0.0f)
             kl += rest.s == 0.0f ? (q_rest != q_rest ? NAN : INFINITY)
-                                 : q_rest * (logf(q_rest) - ((hr - h) / a.tau + logf(rest.s) - log_s));
-        r.loss = a.alpha == 0.0f ? 0.0f : a.alpha * a.tau * a.tau * kl;
-        if (a.hard) {
-            r.loss -= (1.0f - a.alpha) * (s1 == 0.0f ? -INFINITY : z_t - h - logf(s1));
-            bad |= z_t != z_t;
-        }
-        if (bad) r.loss = NAN;
+                                 : q_rest * (logf(q_rest) - ((shift_of(rest.m) - h) / a.tau + logf(rest.s) - log_s));
+        float loss = a.alpha == 0.0f ? 0.0f : a.alpha * a.tau * a.tau * kl;
+        if (a.hard) loss -= (1.0f - a.alpha) * (s1 == 0.0f ? -INFINITY : z_t - h - logf(s1));
+        return bad ? NAN : loss;
     }
-    if (gradient) {
-        float w = a.scale * (a.scale_p ? *a.scale_p : 1.0f) * (a.g ? a.g[a.g_rows ? row : 0] : 1.0f);
-        if (bad) w = NAN;
-        const float soft = w * a.alpha * a.tau, hard = a.hard ? w * (1.0f - a.alpha) : 0.0f;
-        const float inv = s.s == 0.0f ? 0.0f : 1.0f / s.s, inv1 = s1 == 0.0f ? 0.0f : 1.0f / s1;
-        r.soft = soft * inv_mass;
-        r.hard = hard;
-        r.coef1 = S1 ? hard * inv1 : 0.0f;
-        r.inside = soft * Q * inv + (S1 ? 0.0f : hard * inv);
-        if constexpr (TAIL) {
-            const float f = exp2_approx(exponent(rest.m, h, a.c));
-            r.h = shift_of(rest.m);
-            r.coef = rest.s == 0.0f ? 0.0f * w : f * r.inside - soft * q_rest / rest.s;
-        } else {
-            r.h = h;
-            r.coef = r.inside;
-        }
-    }
-    return r;
-}
+};
 
 // The gradient at slot q's token (q == k: at the target) of logit z, written by the first slot
 // that names it.  index, logprob: the row's k slots, index[k] the target or -1.
@@ -326,7 +345,7 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
         if (lane == 0) idx[a.k] = in ? (int)t : -1;
         if constexpr (TAIL) named[warp][lane] = 0;
         __syncwarp();
-        bool firsts[kPer];
+        bool firsts[kPer] = {};
         if constexpr (TAIL) {
 #pragma unroll
             for (int q = 0; q < kPer; ++q) {
@@ -352,10 +371,14 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
             s.s = warp_sum(s.s);
             if constexpr (S1) s.s1 = warp_sum(s.s1);
         }
-        const DistillRow r = distill_row<TAIL, S1>(a, row, s, &slots, 1, z_t, dr != nullptr);
-        sum += r.loss;
-        if (a.loss && a.each && lane == 0) a.loss[row] = r.loss;
+        const DistillSums<TAIL, S1> all(a, s, &slots, 1, z_t);
+        if (a.loss) {
+            const float loss = all.loss(a, &slots, 1, z_t);
+            sum += loss;
+            if (a.each && lane == 0) a.loss[row] = loss;
+        }
         if (dr) {
+            const DistillRow r = all.gradient(a, row);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int j = lane + 32 * e;
@@ -399,6 +422,9 @@ __device__ __forceinline__ uint4 without(const uint4& r, uint32_t bits) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Of a CTA's warps the last ones keep the slots, one a lane, and are a row ahead: the slots' indices and values are
+// read a row before their logits, and those (and what they come to) right after the sums of the row before.  The
+// first warp brings a row's sums and its slots' together.
 template <int DT, int kThreads, bool TAIL, bool S1, bool GRAD>
 __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(DistillArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
@@ -414,83 +440,95 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
     __shared__ DistillRow shared_row[2];
     const int tid = threadIdx.x;
     const uint32_t ctas = 1u << lg, rank = blockIdx.x & (ctas - 1);
-    const int slot_warps = (a.k + 31) / 32;
+    const int slot_warps = (a.k + 31) / 32, own = tid - (kThreads - 32 * slot_warps);  // slot of this thread
+    const T* z0 = reinterpret_cast<const T*>(a.z.p);
     if constexpr (TAIL) {
         for (int i = tid; i < distill_words(a.V, ctas); i += kThreads) named[i] = 0;
-        __syncthreads();
     }
     const RowList list(a.tok, a.z.T, a.N, blockIdx.x >> lg, gridDim.x >> lg);
     const RowStep step(a.z, gridDim.x >> lg);
     Stream stream(a.z, a.V, list, step, rank, lg, sm);
-    RowAt at(a.z, list.first);
-    uint32_t window = 0;
-    int parity = 0;
-    float sum = 0.0f;
-    // a slot of the next row, read while this one's logits go by
-    Slot next{-1, -INFINITY, -INFINITY};
-    bool next_ok = true;
-    auto read_ahead = [&](uint32_t i) {
-        if (tid < a.k && i < list.count) next_ok = read_slot(a, (int64_t)list.row(i) * a.k + tid, next.j, next.l);
-    };
-    read_ahead(0);
-    for (uint32_t i = 0; i < list.count; ++i, step.move(at, a.z.T)) {
-        if ((i & 31) == 0) window = list.window(i);
-        const uint32_t row = list.row(i);
-        const bool live = window >> (i & 31) & 1u;
-        const T* zr = reinterpret_cast<const T*>(a.z.p) + at.off;
-        T* dr = GRAD ? reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row) : nullptr;
-        const Segment g = segment_of<DT>(zr, a.V, rank, lg);
-        const bool wide = (((uintptr_t)zr ^ (uintptr_t)dr) & 15u) == 0;  // 16-byte stores
-        const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
-        Slot slot[1] = {next};
-        const bool ok = next_ok;
-        read_ahead(i + 1);
-        if (!live) {
+    // rows of padding
+    if (a.tok.p && (GRAD || (a.loss && a.each))) {
+        for (uint32_t i = 0; i < list.count; ++i) {
+            const uint32_t live = list.window(i & ~31u), row = list.row(i);
+            if (live >> (i & 31) & 1u) continue;
             if (a.loss && a.each && rank == 0 && tid == 0) a.loss[row] = 0.0f;
             if constexpr (GRAD) {
-                if (wide) {
-                    uint4* to = reinterpret_cast<uint4*>(dr + g.h0);
-                    for (int v = g.v0 + tid; v < g.v1; v += kThreads) __stcs(to + v, make_uint4(0, 0, 0, 0));
-                    if (tid < ends) dr[end_at] = from_float<T>(0.0f);
-                } else {
-                    for (int j = g.j0 + tid; j < g.j1; j += kThreads) dr[j] = from_float<T>(0.0f);
+                T* dr = reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row);
+                const Segment g = segment_of<DT>(dr, a.V, rank, lg);
+                uint4* to = reinterpret_cast<uint4*>(dr + g.h0);
+                for (int v = g.v0 + tid; v < g.v1; v += kThreads) __stcs(to + v, make_uint4(0, 0, 0, 0));
+                if (tid < g.head + g.tail) dr[tid < g.head ? tid : g.t0 + tid - g.head] = from_float<T>(0.0f);
+            }
+        }
+    }
+    int parity = 0;
+    float sum = 0.0f;
+    LiveRows at(a.z, list, step);
+    LiveRows ahead = at;  // the row after the one that the slots' logits are read of
+    Slot slot[1] = {{-1, -INFINITY, -INFINITY}}, next{-1, -INFINITY, -INFINITY};
+    bool ok = true, next_ok = true;
+    auto read_ahead = [&] {  // this thread's slot of row `ahead`
+        next = Slot{-1, -INFINITY, -INFINITY};
+        next_ok = true;
+        if (own >= 0 && own < a.k && ahead.valid())
+            next_ok = read_slot(a, (int64_t)ahead.row() * a.k + own, next.j, next.l);
+    };
+    auto bit_of = [&](const Segment& g, int j) {  // of a logit of this part: vectors first, then head and tail
+        const int body = (g.v1 - g.v0) * kVec;
+        return j < g.h0 ? body + j : j >= g.t0 ? body + 8 + (j - g.t0) : j - g.h0 - g.v0 * kVec;
+    };
+    // the slots' indices of row `ahead` into buffer p, and their bits
+    auto name = [&](int p) {
+        slot[0] = next;
+        ok = next_ok;
+        if (own >= 0 && own < a.k) {
+            index[p][own] = slot[0].j;
+            logprob[p][own] = slot[0].l;
+            if constexpr (TAIL) {
+                const Segment g = segment_of<DT>(z0 + ahead.at.off, a.V, rank, lg);
+                if (slot[0].j >= g.j0 && slot[0].j < g.j1) {
+                    const int b = bit_of(g, slot[0].j);
+                    atomicOr(&named[b >> 5], 1u << (b & 31));
                 }
             }
-            continue;
         }
-        int64_t t = -1;
-        float z_t = 0.0f;
-        if (a.hard) {
-            t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
-            z_t = t >= 0 && t < a.V ? to_float(zr[t]) : NAN;
-        }
-        const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
-        int* idx = index[parity];
-        if (tid < a.k) {
-            if (slot[0].j >= 0) slot[0].z = to_float(zr[slot[0].j]);
-            idx[tid] = slot[0].j;
-            logprob[parity][tid] = slot[0].l;
-        }
-        if (tid == 0) idx[a.k] = z_t == z_t && a.hard ? (int)t : -1;
-        // bit of a logit of this part: vectors first, then head and tail
-        auto bit_of = [&](int j) {
-            const int body = (g.v1 - g.v0) * kVec;
-            return j < g.h0 ? body + j : j >= g.t0 ? body + 8 + (j - g.t0) : j - g.h0 - g.v0 * kVec;
-        };
-        if constexpr (TAIL) {
-            if (tid < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) {
-                const int b = bit_of(slot[0].j);
-                atomicOr(&named[b >> 5], 1u << (b & 31));
-            }
-            __syncthreads();
-        }
-        if (tid < 32 * slot_warps) {
-            const SlotSums x = slot_sums<TAIL, S1, 1>(a, slot, 1, tid < a.k && !ok, [&](int) {
+    };
+    // what those slots come to; `ahead` moves on.  After a barrier of the CTA behind name()
+    auto weigh = [&](int p) {
+        if (own >= 0 && ahead.valid()) {
+            if (slot[0].j >= 0) slot[0].z = to_float(z0[ahead.at.off + slot[0].j]);
+            const SlotSums x = slot_sums<TAIL, S1, 1>(a, slot, 1, own < a.k && !ok, [&](int) {
                 bool first = true;
-                for (int n = 0; n < tid; ++n) first &= idx[n] != slot[0].j;
+                for (int n = 0; n < own; ++n) first &= index[p][n] != slot[0].j;
                 return first;
             });
-            if ((tid & 31) == 0) slots[parity][tid >> 5] = x;
+            if ((tid & 31) == 0) slots[p][own >> 5] = x;
+        }
+        ahead.next();
+        read_ahead();
+    };
+    read_ahead();
+    __syncthreads();  // the bitmap is zero
+    name(0);
+    __syncthreads();
+    weigh(0);
+    for (; at.valid(); at.next()) {
+        const uint32_t row = at.row();
+        const T* zr = z0 + at.at.off;
+        T* dr = GRAD ? reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row) : nullptr;
+        const Segment g = segment_of<DT>(zr, a.V, rank, lg);
+        const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
+        const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
+        float z_t = 0.0f;
+        if (tid < 32) {
+            int64_t t = -1;
+            if (a.hard) {
+                t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
+                z_t = t >= 0 && t < a.V ? to_float(zr[t]) : NAN;
+            }
+            if (tid == 0) index[parity][a.k] = t >= 0 && t < a.V ? (int)t : -1;
         }
         Running<false, S1> run;
         run.begin();
@@ -523,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
         if (tid < ends) {
             float x[1] = {end};
             if constexpr (TAIL) {
-                const int b = bit_of(end_at);
+                const int b = bit_of(g, end_at);
                 if (named[b >> 5] >> (b & 31) & 1u) x[0] = -INFINITY;
             }
             add_values<1, false, S1>(s, x, x[0], a.c);
@@ -531,18 +569,31 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
         s = cta_join<kThreads, false, S1>(s, part[parity], a.c);
         if constexpr (TAIL) {
             // all of the CTA have read the bitmap
-            if (tid < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) named[bit_of(slot[0].j) >> 5] = 0;
+            if (own >= 0 && own < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) named[bit_of(g, slot[0].j) >> 5] = 0;
+            if (own >= 0) slot_barrier(32 * slot_warps);
         }
         if (ctas > 1) s = cluster_join<false, S1>(s, &mine[parity], ctas, a.c);
-        if (tid < 32) {
-            const DistillRow r = distill_row<TAIL, S1>(a, row, s, slots[parity], slot_warps, z_t, GRAD);
-            if (rank == 0) sum += r.loss;
-            if (a.loss && a.each && rank == 0 && tid == 0) a.loss[row] = r.loss;
-            if (GRAD && tid == 0) shared_row[parity] = r;
-        }
+        name(parity ^ 1);
         if constexpr (GRAD) {
-            __syncthreads();
+            if (tid < 32) {
+                const DistillSums<TAIL, S1> all(a, s, slots[parity], slot_warps, z_t);
+                const DistillRow r = all.gradient(a, row);
+                if (tid == 0) shared_row[parity] = r;
+            }
+        }
+        if constexpr (GRAD || TAIL) __syncthreads();
+        else if (slot_warps > 1 && own >= 0) slot_barrier(32 * slot_warps);
+        if (tid < 32 && a.loss) {
+            const DistillSums<TAIL, S1> all(a, s, slots[parity], slot_warps, z_t);
+            const float loss = all.loss(a, slots[parity], slot_warps, z_t);
+            if (rank == 0) sum += loss;
+            if (a.each && rank == 0 && tid == 0) a.loss[row] = loss;
+        }
+        weigh(parity ^ 1);
+        if constexpr (GRAD) {
             const DistillRow r = shared_row[parity];
+            const DistillMany<S1> many(r);
+            const bool wide = (((uintptr_t)zr ^ (uintptr_t)dr) & 15u) == 0;  // 16-byte stores
             auto write = [&](const uint4 (&raw)[kU], int v, int mine) {
                 T* to = dr + g.h0 + (int64_t)v * kVec;
 #pragma unroll
@@ -550,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
                     if (u >= mine) continue;
                     float x[kVec];
                     unpack16<DT>(raw[u], x);
-                    r.template at_all<S1, kVec>(x);
+                    many(r, x);
                     if (wide) {
                         __stcs(reinterpret_cast<uint4*>(to) + u * kThreads, pack16<DT>(x));
                     } else {
@@ -576,10 +627,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
             if (tid < ends) dr[end_at] = from_float<T>(r.template at<S1>(end));
             __syncthreads();
             for (int q = tid; q <= a.k; q += kThreads)
-                if (idx[q] >= g.j0 && idx[q] < g.j1)
-                    distill_grad_slot<T, TAIL, S1>(r, idx, logprob[parity], a.k, q, zr, dr);
-        } else if constexpr (TAIL) {
-            __syncthreads();  // the bitmap is clear
+                if (index[parity][q] >= g.j0 && index[parity][q] < g.j1)
+                    distill_grad_slot<T, TAIL, S1>(r, index[parity], logprob[parity], a.k, q, zr, dr);
         }
         parity ^= 1;
     }

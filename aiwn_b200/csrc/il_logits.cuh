@@ -494,6 +494,36 @@ struct RowList {
     }
 };
 
+// goes through the rows of a list that are not padding
+struct LiveRows {
+    const RowList& list;
+    const RowStep& step;
+    uint32_t i, window;
+    RowAt at;
+
+    // whole warps
+    __device__ __forceinline__ LiveRows(const RowsIn& z, const RowList& list_, const RowStep& step_)
+        : list(list_), step(step_), i(0), at(z, list_.first) {
+        window = list.window(0);
+        seek();
+    }
+    __device__ __forceinline__ bool valid() const { return i < list.count; }
+    __device__ __forceinline__ uint32_t row() const { return list.row(i); }
+    __device__ __forceinline__ void next() {
+        step_on();
+        seek();
+    }
+
+private:
+    __device__ __forceinline__ void step_on() {
+        step.move(at, list.T);
+        if ((++i & 31) == 0 && i < list.count) window = list.window(i);
+    }
+    __device__ __forceinline__ void seek() {
+        while (i < list.count && !(window >> (i & 31) & 1u)) step_on();
+    }
+};
+
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -519,11 +549,8 @@ struct RowStream {
     const RowsIn& z;
     const int V;
     const uint32_t rank, lg;
-    const RowList& list;
-    const RowStep& step;
-    RowAt at;
+    LiveRows rows;      // at the row being loaded
     uint32_t slots;     // shared address of this thread's places
-    uint32_t i, live;   // row being loaded, its window
     uint32_t put, get;  // bytes
     const uint4* src;   // this thread's next vector
     int mine, steps;    // vectors and steps left of this pass
@@ -531,11 +558,10 @@ struct RowStream {
 
     __device__ __forceinline__ RowStream(const RowsIn& z_, int V_, const RowList& list_, const RowStep& step_,
                                          uint32_t rank_, uint32_t lg_, void* shared)
-        : z(z_), V(V_), rank(rank_), lg(lg_), list(list_), step(step_), at(z_, list_.first), i(0), put(0), get(0),
-          mine(0), steps(0), passes(0), src(nullptr) {
+        : z(z_), V(V_), rank(rank_), lg(lg_), rows(z_, list_, step_), put(0), get(0), src(nullptr), mine(0), steps(0),
+          passes(0) {
         slots = smem_addr(shared) + threadIdx.x * 16;
-        live = list.window(0);
-        next_row();
+        begin_row();
 #pragma unroll 1
         for (int n = 0; n < kStages; ++n) issue();
     }
@@ -546,15 +572,14 @@ struct RowStream {
         steps = (g.v1 - g.v0 + kStep - 1) / kStep;
     }
 
-    // to the first row from i on that has vectors to load; steps is 0 if there is none
-    __device__ __forceinline__ void next_row() {
-        for (; i < list.count; step.move(at, z.T), ++i) {
-            if ((i & 31) == 0 && i) live = list.window(i);
-            if (!(live >> (i & 31) & 1u)) continue;
-            const T* zr = reinterpret_cast<const T*>(z.p) + at.off;
-            const Segment g = segment_of<DT>(zr, V, rank, lg);
+    __device__ __forceinline__ const T* row_at() const { return reinterpret_cast<const T*>(z.p) + rows.at.off; }
+
+    // the first row from here on that has vectors to load; steps stays 0 if there is none
+    __device__ __forceinline__ void begin_row() {
+        for (; rows.valid(); rows.next()) {
+            const Segment g = segment_of<DT>(row_at(), V, rank, lg);
             if (g.v0 >= g.v1) continue;
-            begin_pass(g, zr);
+            begin_pass(g, row_at());
             passes = kPasses - 1;
             return;
         }
@@ -570,12 +595,10 @@ struct RowStream {
             if (--steps == 0) {
                 if (kPasses > 1 && passes > 0) {
                     --passes;
-                    const T* zr = reinterpret_cast<const T*>(z.p) + at.off;
-                    begin_pass(segment_of<DT>(zr, V, rank, lg), zr);
+                    begin_pass(segment_of<DT>(row_at(), V, rank, lg), row_at());
                 } else {
-                    step.move(at, z.T);
-                    ++i;
-                    next_row();
+                    rows.next();
+                    begin_row();
                 }
             }
         }

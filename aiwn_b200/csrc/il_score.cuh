@@ -405,20 +405,18 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) score_row_kernel(Sco
     const RowList list(a.tok, a.z.T, a.N, blockIdx.x >> lg, gridDim.x >> lg);
     const RowStep step(a.z, gridDim.x >> lg);
     Stream stream(a.z, a.V, list, step, rank, lg, sm);
-    RowAt at(a.z, list.first);
     if constexpr (TOP) {
         if (tid == 0) top_shared.count = 0;
     }
-    uint32_t live = 0;
     int parity = 0;
-    for (uint32_t i = 0; i < list.count; ++i, step.move(at, a.z.T)) {
-        if ((i & 31) == 0) live = list.window(i);
-        const uint32_t row = list.row(i);
-        if (!(live >> (i & 31) & 1u)) {
-            if (rank == 0) score_padding(a, row, tid, kThreads);
-            continue;
+    if (rank == 0 && a.tok.p)
+        for (uint32_t i = 0; i < list.count; ++i) {
+            const uint32_t live = list.window(i & ~31u);
+            if (!(live >> (i & 31) & 1u)) score_padding(a, list.row(i), tid, kThreads);
         }
-        const T* zr = reinterpret_cast<const T*>(a.z.p) + at.off;
+    for (LiveRows at(a.z, list, step); at.valid(); at.next()) {
+        const uint32_t row = at.row();
+        const T* zr = reinterpret_cast<const T*>(a.z.p) + at.at.off;
         const Segment g = segment_of<DT>(zr, a.V, rank, lg);
         const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
         const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
