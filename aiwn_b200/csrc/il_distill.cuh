@@ -145,20 +145,25 @@ struct DistillMany {
         huge = !(fabsf(b) < 4194304.0f) || (S1 && !(fabsf(b1) < 4194304.0f));
     }
     template <int n>
-    __device__ __forceinline__ void operator()(const DistillRow& r, float (&x)[n]) const {
-        if (huge) {
+    __device__ __forceinline__ void operator()(float (&x)[n]) const {
 #pragma unroll
-            for (int i = 0; i < n; ++i) x[i] = r.template at<S1>(x[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < n; ++i) {
-                const float z = x[i];
-                x[i] = exp2_approx(fmaf(z, c, b)) * f;
-                if constexpr (S1) x[i] = fmaf(exp2_approx(fmaf(z, kLog2e, b1)), f1, x[i]);
-            }
+        for (int i = 0; i < n; ++i) {
+            const float z = x[i];
+            x[i] = exp2_approx(fmaf(z, c, b)) * f;
+            if constexpr (S1) x[i] = fmaf(exp2_approx(fmaf(z, kLog2e, b1)), f1, x[i]);
         }
     }
 };
+
+// a vector's gradient, of any size and to any address
+template <int DT, bool S1>
+__device__ __noinline__ void write_slowly(const DistillRow* r, uint4 z, typename Elem<DT>::type* to) {
+    constexpr int kVec = Elem<DT>::kVec;
+    float x[kVec];
+    unpack16<DT>(z, x);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) to[e] = from_float<typename Elem<DT>::type>(r->template at<S1>(x[e]));
+}
 
 // What a row's sums and its slots' come to.  s: the sums of the row, or of what no slot names (tail); part: the
 // slots' of `parts` warps; z_t: the target's logit, NaN for one outside the vocabulary
@@ -403,8 +408,10 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
 
 // ---- longer rows: a CTA, or a cluster of CTAs, a row --------------------------------
 
-// words of the bitmap of a part of a row: its vectors' logits, 8 of the head, 8 of the tail
-__host__ __device__ constexpr int distill_words(int V, int ctas) { return (V / ctas + 8 + 31) / 32 + 2; }
+// bytes of the bitmap of a part of a row: one a vector, to the end of a step, and 16 for the row's ends
+__host__ __device__ constexpr int distill_bitmap(int V, int ctas, int vec, int step) {
+    return (V / vec / ctas + 1 + step - 1) / step * step + 16;
+}
 
 // a vector with -inf in place of the logits whose bits are set
 template <int DT>
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
     constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kWarps = kThreads / 32;
     if (a.skip_if_one && *a.g == 1.0f) return;
     extern __shared__ __align__(16) unsigned char sm[];  // the stream's places, the bitmap
-    uint32_t* named = reinterpret_cast<uint32_t*>(sm + Stream::kBytes);
+    uint8_t* named = sm + Stream::kBytes;
     __shared__ float4 part[2][kWarps], mine[2];
     __shared__ SlotSums slots[2][kMaxTop / 32];
     __shared__ int index[2][kMaxTop + 1];
@@ -443,7 +450,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
     const int slot_warps = (a.k + 31) / 32, own = tid - (kThreads - 32 * slot_warps);  // slot of this thread
     const T* z0 = reinterpret_cast<const T*>(a.z.p);
     if constexpr (TAIL) {
-        for (int i = tid; i < distill_words(a.V, ctas); i += kThreads) named[i] = 0;
+        for (int i = tid; i < distill_bitmap(a.V, ctas, kVec, Stream::kStep) / 4; i += kThreads)
+            reinterpret_cast<uint32_t*>(named)[i] = 0;
     }
     const RowList list(a.tok, a.z.T, a.N, blockIdx.x >> lg, gridDim.x >> lg);
     const RowStep step(a.z, gridDim.x >> lg);
@@ -475,10 +483,14 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
         if (own >= 0 && own < a.k && ahead.valid())
             next_ok = read_slot(a, (int64_t)ahead.row() * a.k + own, next.j, next.l);
     };
-    auto bit_of = [&](const Segment& g, int j) {  // of a logit of this part: vectors first, then head and tail
-        const int body = (g.v1 - g.v0) * kVec;
-        return j < g.h0 ? body + j : j >= g.t0 ? body + 8 + (j - g.t0) : j - g.h0 - g.v0 * kVec;
+    // byte and bit of a logit of this part: those of its vector; in the last 16 bytes, of the head and the tail
+    const int ends_byte = TAIL ? distill_bitmap(a.V, ctas, kVec, Stream::kStep) - 16 : 0;
+    auto bit_of = [&](const Segment& g, int j) {
+        const int i = j - g.h0;
+        return j < g.h0 ? ends_byte * 8 + j : j >= g.t0 ? ends_byte * 8 + 8 + (j - g.t0)
+                                                        : (i / kVec - g.v0) * 8 + i % kVec;
     };
+    uint32_t* named_words = reinterpret_cast<uint32_t*>(named);
     // the slots' indices of row `ahead` into buffer p, and their bits
     auto name = [&](int p) {
         slot[0] = next;
@@ -490,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
                 const Segment g = segment_of<DT>(z0 + ahead.at.off, a.V, rank, lg);
                 if (slot[0].j >= g.j0 && slot[0].j < g.j1) {
                     const int b = bit_of(g, slot[0].j);
-                    atomicOr(&named[b >> 5], 1u << (b & 31));
+                    atomicOr(&named_words[b >> 5], 1u << (b & 31));
                 }
             }
         }
@@ -534,12 +546,13 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
         run.begin();
         auto use = [&](uint4 (&raw)[kU], int v) {  // v: of the first vector
             if constexpr (TAIL) {
+                const uint8_t* byte = named + (v - g.v0);
+                uint32_t bits[kU], any = 0;
 #pragma unroll
-                for (int u = 0; u < kU; ++u) {
-                    const int w = v + u * kThreads;
-                    const int b = w < g.v1 ? (w - g.v0) * kVec : 0;
-                    const uint32_t bits = named[b >> 5] >> (b & 31) & ((1u << kVec) - 1u);
-                    if (bits) raw[u] = without<DT>(raw[u], bits);
+                for (int u = 0; u < kU; ++u) any |= bits[u] = byte[u * kThreads];
+                if (any) {
+#pragma unroll
+                    for (int u = 0; u < kU; ++u) raw[u] = without<DT>(raw[u], bits[u]);
                 }
             }
             run.template add<DT>(raw, max_of<DT>(raw), a.c);
@@ -562,14 +575,14 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
             float x[1] = {end};
             if constexpr (TAIL) {
                 const int b = bit_of(g, end_at);
-                if (named[b >> 5] >> (b & 31) & 1u) x[0] = -INFINITY;
+                if (named_words[b >> 5] >> (b & 31) & 1u) x[0] = -INFINITY;
             }
             add_values<1, false, S1>(s, x, x[0], a.c);
         }
         s = cta_join<kThreads, false, S1>(s, part[parity], a.c);
         if constexpr (TAIL) {
             // all of the CTA have read the bitmap
-            if (own >= 0 && own < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) named[bit_of(g, slot[0].j) >> 5] = 0;
+            if (own >= 0 && own < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) named_words[bit_of(g, slot[0].j) >> 5] = 0;
             if (own >= 0) slot_barrier(32 * slot_warps);
         }
         if (ctas > 1) s = cluster_join<false, S1>(s, &mine[parity], ctas, a.c);
@@ -594,20 +607,22 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
             const DistillRow r = shared_row[parity];
             const DistillMany<S1> many(r);
             const bool wide = (((uintptr_t)zr ^ (uintptr_t)dr) & 15u) == 0;  // 16-byte stores
+            const bool plain = wide && !many.huge;
             auto write = [&](const uint4 (&raw)[kU], int v, int mine) {
                 T* to = dr + g.h0 + (int64_t)v * kVec;
+                if (plain) {
 #pragma unroll
-                for (int u = 0; u < kU; ++u) {
-                    if (u >= mine) continue;
-                    float x[kVec];
-                    unpack16<DT>(raw[u], x);
-                    many(r, x);
-                    if (wide) {
+                    for (int u = 0; u < kU; ++u) {
+                        if (u >= mine) continue;
+                        float x[kVec];
+                        unpack16<DT>(raw[u], x);
+                        many(x);
                         __stcs(reinterpret_cast<uint4*>(to) + u * kThreads, pack16<DT>(x));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < kVec; ++e) to[u * kThreads * kVec + e] = from_float<T>(x[e]);
                     }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kU; ++u)
+                        if (u < mine) write_slowly<DT, S1>(&shared_row[parity], raw[u], to + u * kThreads * kVec);
                 }
             };
             left = g.v1 - g.v0;

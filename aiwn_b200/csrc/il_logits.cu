@@ -270,7 +270,9 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
                 return with_bool(dlogits != nullptr, [&](auto gr) {
                     return with_threads(p.threads, [&](auto th) {
                         const size_t smem = RowStream<dt.value, th.value, 1>::kBytes +
-                                            (tl.value ? 4 * (size_t)distill_words(a.V, 1 << p.lg) : 0);
+                                            (tl.value ? distill_bitmap(a.V, 1 << p.lg, Elem<dt.value>::kVec,
+                                                                       RowStream<dt.value, th.value, 1>::kStep)
+                                                      : 0);
                         return launch(distill_row_kernel<dt.value, th.value, tl.value, s1.value, gr.value>, p.grid,
                                       th.value, p.lg, smem, s, a, p.lg);
                     });

@@ -170,6 +170,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return y;
 }
 
+__device__ __forceinline__ float sum2(uint64_t v) {
+    float a, b;
+    unpack2(v, a, b);
+    return a + b;
+}
+
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kMinExp = -150.0f;
 
@@ -287,6 +293,23 @@ __device__ __forceinline__ uint4 floor16(const uint4& r) {
     return make_uint4(y[0], y[1], y[2], y[3]);
 }
 
+// the sums of a vector to the maximum m, whatever its size
+template <int DT, bool U, bool S1>
+__device__ __noinline__ Sums huge_vector(uint4 r, float m, float c) {
+    constexpr int kVec = Elem<DT>::kVec;
+    float x[kVec];
+    unpack16<DT>(r, x);
+    Sums a{m, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+        const float d = exponent(x[i], m, c), e = exp2_approx(d);
+        a.s += e;
+        if constexpr (U) a.u = fmaf(e, d, a.u);
+        if constexpr (S1) a.s1 += exp2_approx(exponent(x[i], m, kLog2e));
+    }
+    return a;
+}
+
 // A thread's sums while a row goes by.  The exponent is taken to a whole number H next to
 // m log2(e) / tau: d = z c - H is one fused multiply-add, rounded once, and a new maximum
 // rescales by a power of two, without rounding.  Where |m| c is 2^22 or more (a row of nothing
@@ -325,18 +348,11 @@ struct Running {
         if (huge) {
 #pragma unroll
             for (int q = 0; q < kU; ++q) {
-                float x[kVec];
-                unpack16<DT>(r[q], x);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    const float d = exponent(x[i], m, c), e = exp2_approx(d);
-                    s += e;
-                    if constexpr (U) u = fmaf(e, d, u);
-                    if constexpr (S1) s1 += exp2_approx(exponent(x[i], m, kLog2e));
-                }
+                const Sums x = huge_vector<DT, U, S1>(r[q], m, c);
+                s += x.s, u += x.u, s1 += x.s1;
             }
         } else {
-            float e0 = 0.0f, e1 = 0.0f, u0 = 0.0f, u1 = 0.0f, f0 = 0.0f, f1 = 0.0f;  // of the even and the odd values
+            uint64_t e = 0, f = 0, v = 0;  // of the even and the odd values
 #pragma unroll
             for (int q = 0; q < kU; ++q) {
                 float x[kVec];
@@ -344,19 +360,19 @@ struct Running {
 #pragma unroll
                 for (int i = 0; i < kVec; i += 2) {
                     const float d0 = fmaf(x[i], c, h), d1 = fmaf(x[i + 1], c, h);
-                    const float a0 = exp2_approx(d0), a1 = exp2_approx(d1);
-                    e0 += a0;
-                    e1 += a1;
-                    if constexpr (U) u0 = fmaf(a0, d0, u0), u1 = fmaf(a1, d1, u1);
+                    const uint64_t a = pack2(exp2_approx(d0), exp2_approx(d1));
+                    const bool first = q == 0 && i == 0;
+                    e = first ? a : add2(e, a);
+                    if constexpr (U) v = first ? mul2(a, pack2(d0, d1)) : fma2(a, pack2(d0, d1), v);
                     if constexpr (S1) {
-                        f0 += exp2_approx(fmaf(x[i], kLog2e, h1));
-                        f1 += exp2_approx(fmaf(x[i + 1], kLog2e, h1));
+                        const uint64_t b = pack2(exp2_approx(fmaf(x[i], kLog2e, h1)), exp2_approx(fmaf(x[i + 1], kLog2e, h1)));
+                        f = first ? b : add2(f, b);
                     }
                 }
             }
-            s += e0 + e1;
-            if constexpr (U) u += u0 + u1;
-            if constexpr (S1) s1 += f0 + f1;
+            s += sum2(e);
+            if constexpr (U) u += sum2(v);
+            if constexpr (S1) s1 += sum2(f);
         }
     }
 
@@ -587,9 +603,14 @@ struct RowStream {
 
     __device__ __forceinline__ void issue() {
         if (steps) {
+            if (steps > 1) {  // a whole one
 #pragma unroll
-            for (int u = 0; u < kU; ++u)
-                if (u < mine) copy_async16(slots + put + u * (kThreads * 16), src + u * kThreads);
+                for (int u = 0; u < kU; ++u) copy_async16(slots + put + u * (kThreads * 16), src + u * kThreads);
+            } else {
+#pragma unroll
+                for (int u = 0; u < kU; ++u)
+                    if (u < mine) copy_async16(slots + put + u * (kThreads * 16), src + u * kThreads);
+            }
             src += kStep;
             mine -= kU;
             if (--steps == 0) {
