@@ -61,7 +61,7 @@ struct SlotSums {
     float top, mass, cross, base;
     double left;  // sum of exp(l_i) in 64 bits (tail)
     Sums s;       // of the slots' logits, each token once (tail)
-    int bad, pad;
+    int bad, again;  // a slot beyond the vocabulary; a token that an earlier slot names too
 };
 
 // a barrier of the warps that keep the slots
@@ -74,9 +74,25 @@ __device__ __forceinline__ float slot_weight(float l, float top) {
     return TAIL ? expf(l) : expf(l - top);
 }
 
-// n: slots of this lane; first: whether slot q is the first to name its token (tail)
-template <bool TAIL, bool S1, int n, class First>
-__device__ __forceinline__ SlotSums slot_sums(const DistillArgs& a, const Slot (&x)[n], int used, bool bad, First first) {
+// Whether the slots of this lane, lane + 32 q of those from index[base] on, are the first of index[0 ..] to name their
+// tokens.  After a barrier of those who wrote `index`.
+template <int n>
+__device__ __forceinline__ void slot_firsts(const Slot (&x)[n], int used, const int* index, int base, bool (&first)[n]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int q = 0; q < n; ++q) {
+        first[q] = true;
+        if (q >= used) continue;
+        const unsigned peers = __match_any_sync(0xffffffffu, x[q].j);
+        first[q] = lane == __ffs(peers) - 1;
+        for (int i = 0; i < base + 32 * q; ++i) first[q] &= index[i] != x[q].j;
+    }
+}
+
+// n: slots of this lane; first: whether slot q is the first to name its token
+template <bool TAIL, bool S1, int n>
+__device__ __forceinline__ SlotSums slot_sums(const DistillArgs& a, const Slot (&x)[n], int used, bool bad,
+                                              const bool (&first)[n]) {
     SlotSums r;
     float top = -INFINITY, base = -INFINITY;
 #pragma unroll
@@ -96,7 +112,7 @@ __device__ __forceinline__ SlotSums slot_sums(const DistillArgs& a, const Slot (
         if (w != 0.0f) cross += w * ((x[q].l - r.top) - (x[q].z - r.base) / a.tau);
         if constexpr (TAIL) {
             if (is) left += exp((double)x[q].l);
-            if (is && first(q)) {
+            if (is && first[q]) {
                 const float y[1] = {x[q].z};
                 add_values<1, false, S1>(r.s, y, x[q].z, a.c);
             }
@@ -108,7 +124,11 @@ __device__ __forceinline__ SlotSums slot_sums(const DistillArgs& a, const Slot (
         r.left = warp_sum(left);
         r.s = warp_join<false, S1>(r.s, a.c);
     }
+    bool again = false;
+#pragma unroll
+    for (int q = 0; q < n; ++q) again |= x[q].j >= 0 && !first[q];
     r.bad = __any_sync(0xffffffffu, bad);
+    r.again = __any_sync(0xffffffffu, again);
     return r;
 }
 
@@ -247,27 +267,31 @@ struct DistillSums {
     }
 };
 
-// The gradient at slot q's token (q == k: at the target) of logit z, written by the first slot
-// that names it.  index, logprob: the row's k slots, index[k] the target or -1.
+// The gradient at the token of logit z of a slot of weight w (exp(l), up to the row's common factor).
+// again: other slots may name it too; then the first of them writes for all.  index, logprob: the row's k slots,
+// index[k] the target or -1.
 template <class T, bool TAIL, bool S1>
 __device__ __forceinline__ void distill_grad_slot(const DistillRow& r, const int* index, const float* logprob, int k,
-                                                  int q, const T* zr, T* dr) {
+                                                  int q, bool again, float z, T* dr) {
     const int j = index[q];
-    bool first = true;
-    for (int n = 0; n < q; ++n) first &= index[n] != j;
-    if (!first) return;
-    const float z = to_float(zr[j]);
-    float y;
-    if (q < k) {
-        float weight = 0.0f;
-        for (int n = q; n < k; ++n)
+    float weight = slot_weight<TAIL>(logprob[q], r.top);
+    if (again) {
+        for (int n = 0; n < q; ++n)
+            if (index[n] == j) return;
+        for (int n = q + 1; n < k; ++n)
             if (index[n] == j) weight += slot_weight<TAIL>(logprob[n], r.top);
-        y = r.template at_slot<S1>(z, weight);
-    } else {
-        y = r.template at<S1>(z);
     }
-    if (index[k] == j) y -= r.hard;
-    dr[j] = from_float<T>(y);
+    const float y = r.template at_slot<S1>(z, weight);
+    dr[j] = from_float<T>(index[k] == j ? y - r.hard : y);
+}
+
+// One warp: the gradient at the target of logit z, where no slot names it
+template <class T, bool S1>
+__device__ __forceinline__ void distill_grad_target(const DistillRow& r, const int* index, int k, float z, T* dr) {
+    const int j = index[k], lane = threadIdx.x & 31;
+    bool named = false;
+    for (int n = lane; n < k; n += 32) named |= index[n] == j;
+    if (!__any_sync(0xffffffffu, named) && lane == 0) dr[j] = from_float<T>(r.template at<S1>(z) - r.hard);
 }
 
 // A slot as it stands in memory; false: its index is beyond the vocabulary
@@ -278,11 +302,11 @@ __device__ __forceinline__ bool read_slot(const DistillArgs& a, int64_t at, int&
     return x < a.V;
 }
 
-// The rows' losses of a CTA are added up; the last CTA adds up the CTAs', in their order.
-__device__ __forceinline__ void distill_total(const DistillArgs& a, float sum, float* shared, int threads) {
+// The rows' losses of a CTA have been added up by thread `owner`; the last CTA adds up the CTAs', in their order.
+__device__ __forceinline__ void distill_total(const DistillArgs& a, float sum, int owner, float* shared, int threads) {
     if (!a.loss || a.each) return;
     __shared__ bool last;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == owner) {
         a.partial[blockIdx.x] = sum;
         __threadfence();
         last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
@@ -350,17 +374,15 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
         if (lane == 0) idx[a.k] = in ? (int)t : -1;
         if constexpr (TAIL) named[warp][lane] = 0;
         __syncwarp();
-        bool firsts[kPer] = {};
+        bool first[kPer];
+        slot_firsts<kPer>(slot, used, idx, 0, first);
         if constexpr (TAIL) {
 #pragma unroll
-            for (int q = 0; q < kPer; ++q) {
-                const uint32_t bit = 1u << (slot[q].j & 31);
-                firsts[q] = slot[q].j >= 0 && !(atomicOr(&named[warp][slot[q].j >> 5], bit) & bit);
-            }
+            for (int q = 0; q < kPer; ++q)
+                if (first[q] && slot[q].j >= 0) atomicOr(&named[warp][slot[q].j >> 5], 1u << (slot[q].j & 31));
             __syncwarp();
         }
-        const SlotSums slots =
-            slot_sums<TAIL, S1, kPer>(a, slot, used, bad, [&](int q) { return TAIL ? firsts[q] : true; });
+        const SlotSums slots = slot_sums<TAIL, S1, kPer>(a, slot, used, bad, first);
         Sums s = no_sums();
         {
             float y[E], cm = -INFINITY;
@@ -390,8 +412,11 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
                 if (j < a.V) dr[j] = from_float<T>(r.template at<S1>(x[e]));
             }
             __syncwarp();
-            for (int q = lane; q <= a.k; q += 32)
-                if (idx[q] >= 0) distill_grad_slot<T, TAIL, S1>(r, idx, logprob[warp], a.k, q, zr, dr);
+#pragma unroll
+            for (int q = 0; q < kPer; ++q)
+                if (slot[q].j >= 0)
+                    distill_grad_slot<T, TAIL, S1>(r, idx, logprob[warp], a.k, lane + 32 * q, slots.again, slot[q].z, dr);
+            if (in) distill_grad_target<T, S1>(r, idx, a.k, z_t, dr);
         }
         __syncwarp();
     }
@@ -402,7 +427,7 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
         float v = 0.0f;
         for (int w = 0; w < 8; ++w) v += total[w];
         __syncthreads();
-        distill_total(a, v, total, 256);
+        distill_total(a, v, 0, total, 256);
     }
 }
 
@@ -431,9 +456,9 @@ __device__ __forceinline__ uint4 without(const uint4& r, uint32_t bits) {
 
 // Of a CTA's warps the last ones keep the slots, one a lane, and are a row ahead: the slots' indices and values are
 // read a row before their logits, and those (and what they come to) right after the sums of the row before.  The
-// first warp brings a row's sums and its slots' together.
+// first two warps bring a row's sums and its slots' together.
 template <int DT, int kThreads, bool TAIL, bool S1, bool GRAD>
-__global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(DistillArgs a, uint32_t lg) {
+__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads) distill_row_kernel(DistillArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
     using Stream = RowStream<DT, kThreads, GRAD ? 2 : 1>;
     constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kWarps = kThreads / 32;
@@ -475,6 +500,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
     float sum = 0.0f;
     LiveRows at(a.z, list, step);
     LiveRows ahead = at;  // the row after the one that the slots' logits are read of
+    // slot[0]: of the row that `at` will be at; now_*: the same of the row that it is at
     Slot slot[1] = {{-1, -INFINITY, -INFINITY}}, next{-1, -INFINITY, -INFINITY};
     bool ok = true, next_ok = true;
     auto read_ahead = [&] {  // this thread's slot of row `ahead`
@@ -511,11 +537,9 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
     auto weigh = [&](int p) {
         if (own >= 0 && ahead.valid()) {
             if (slot[0].j >= 0) slot[0].z = to_float(z0[ahead.at.off + slot[0].j]);
-            const SlotSums x = slot_sums<TAIL, S1, 1>(a, slot, 1, own < a.k && !ok, [&](int) {
-                bool first = true;
-                for (int n = 0; n < own; ++n) first &= index[p][n] != slot[0].j;
-                return first;
-            });
+            bool first[1];
+            slot_firsts<1>(slot, 1, index[p], own & ~31, first);
+            const SlotSums x = slot_sums<TAIL, S1, 1>(a, slot, 1, own < a.k && !ok, first);
             if ((tid & 31) == 0) slots[p][own >> 5] = x;
         }
         ahead.next();
@@ -534,7 +558,9 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
         const int ends = g.head + g.tail, end_at = tid < g.head ? tid : g.t0 + tid - g.head;
         const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
         float z_t = 0.0f;
-        if (tid < 32) {
+        const int now_j = slot[0].j;
+        const float now_z = slot[0].z;
+        if (tid < 64) {
             int64_t t = -1;
             if (a.hard) {
                 t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
@@ -552,7 +578,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
                 for (int u = 0; u < kU; ++u) any |= bits[u] = byte[u * kThreads];
                 if (any) {
 #pragma unroll
-                    for (int u = 0; u < kU; ++u) raw[u] = without<DT>(raw[u], bits[u]);
+                    for (int u = 0; u < kU; ++u)
+                        if (bits[u]) raw[u] = without<DT>(raw[u], bits[u]);
                 }
             }
             run.template add<DT>(raw, max_of<DT>(raw), a.c);
@@ -582,26 +609,24 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
         s = cta_join<kThreads, false, S1>(s, part[parity], a.c);
         if constexpr (TAIL) {
             // all of the CTA have read the bitmap
-            if (own >= 0 && own < a.k && slot[0].j >= g.j0 && slot[0].j < g.j1) named_words[bit_of(g, slot[0].j) >> 5] = 0;
+            if (own >= 0 && own < a.k && now_j >= g.j0 && now_j < g.j1) named_words[bit_of(g, now_j) >> 5] = 0;
             if (own >= 0) slot_barrier(32 * slot_warps);
         }
         if (ctas > 1) s = cluster_join<false, S1>(s, &mine[parity], ctas, a.c);
         name(parity ^ 1);
-        if constexpr (GRAD) {
-            if (tid < 32) {
-                const DistillSums<TAIL, S1> all(a, s, slots[parity], slot_warps, z_t);
+        if (tid < 64 && (a.loss || GRAD)) {  // the first warp: the gradient, the second: the loss
+            const DistillSums<TAIL, S1> all(a, s, slots[parity], slot_warps, z_t);
+            if (tid >= 32) {
+                const float loss = all.loss(a, slots[parity], slot_warps, z_t);
+                if (rank == 0) sum += loss;
+                if (a.loss && a.each && rank == 0 && tid == 32) a.loss[row] = loss;
+            } else if constexpr (GRAD) {
                 const DistillRow r = all.gradient(a, row);
                 if (tid == 0) shared_row[parity] = r;
             }
         }
         if constexpr (GRAD || TAIL) __syncthreads();
         else if (slot_warps > 1 && own >= 0) slot_barrier(32 * slot_warps);
-        if (tid < 32 && a.loss) {
-            const DistillSums<TAIL, S1> all(a, s, slots[parity], slot_warps, z_t);
-            const float loss = all.loss(a, slots[parity], slot_warps, z_t);
-            if (rank == 0) sum += loss;
-            if (a.each && rank == 0 && tid == 0) a.loss[row] = loss;
-        }
         weigh(parity ^ 1);
         if constexpr (GRAD) {
             const DistillRow r = shared_row[parity];
@@ -641,15 +666,19 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) distill_row_kernel(D
             }
             if (tid < ends) dr[end_at] = from_float<T>(r.template at<S1>(end));
             __syncthreads();
-            for (int q = tid; q <= a.k; q += kThreads)
-                if (index[parity][q] >= g.j0 && index[parity][q] < g.j1)
-                    distill_grad_slot<T, TAIL, S1>(r, index[parity], logprob[parity], a.k, q, zr, dr);
+            if (own >= 0 && own < a.k && now_j >= g.j0 && now_j < g.j1) {
+                bool again = false;
+                for (int n = 0; n < slot_warps; ++n) again |= slots[parity][n].again != 0;
+                distill_grad_slot<T, TAIL, S1>(r, index[parity], logprob[parity], a.k, own, again, now_z, dr);
+            }
+            if (tid < 32 && index[parity][a.k] >= g.j0 && index[parity][a.k] < g.j1)
+                distill_grad_target<T, S1>(r, index[parity], a.k, z_t, dr);
         }
         parity ^= 1;
     }
     if (ctas > 1) cluster_sync();  // no CTA ends while another may still read its shared memory
     __syncthreads();
-    distill_total(a, sum, total, kThreads);
+    distill_total(a, sum, 32, total, kThreads);
 }
 
 // ws[0] = 1 / (rows that are not padding, at least 1), ws[1]: the ticket, 0; one CTA of 1024 threads

@@ -16,8 +16,8 @@ namespace {
 using namespace il;
 
 constexpr double kLog2e64 = 1.4426950408889634074;
-constexpr double kRowCost = 16384;
-constexpr double kResident = 48e6;  // bytes of rows that the L2 keeps from one pass over them to the next
+constexpr double kRowCost = 32768;
+constexpr double kResident = 62e6;  // bytes of rows that the L2 keeps from one pass over them to the next
 constexpr int64_t kMaxGrid = 8192;  // CTAs of a kernel that adds up a whole loss
 
 // how a [B, T, V] operand is cut up
@@ -40,13 +40,14 @@ int check_rows(int dtype, int64_t B, int64_t T, int64_t V, double temperature) {
 // the row stride of the operands and their element size: natural alignment of the base is all that is asked
 int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_BF16 ? 1u : 3u)) ? IL_ERR_ALIGN : IL_OK; }
 
-// Rows of more than kWarpVocab logits.  512 threads an SM, in CTAs of 512, 256 or 128: a
-// warp's share of what a row costs beside its logits is the same whatever the row's length,
-// so that shorter rows get fewer warps.  Then the CTAs of a row: those that take the
-// shortest time by a simple count, in which a cluster of c CTAs has 1/c of a row to load
-// and the rest costs as much as kRowCost bytes, twice as much in a cluster.
+// Rows of more than kWarpVocab logits.  An SM holds kSmThreads threads, in CTAs of 128, 256 or 512: a warp's share
+// of what a row costs beside its logits is the same whatever the row's length, so that shorter rows get fewer warps.
+// Then the CTAs of a row: those that take the shortest time by a simple count, in which a cluster of c CTAs has 1/c
+// of a row to load and the rest costs as much as kRowCost bytes, twice as much in a cluster.  shared(t, lg): bytes of
+// shared memory of a CTA beside its stream.
 // AIWN_IL_LOGITS=threads,ctas pins both where they can serve the row (for the tests).
-Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, bool twice) {
+template <class Shared>
+Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, bool twice, Shared shared) {
     Plan p{0, 256, 0, 0};
     if (V <= kWarpVocab) {
         p.regs = (int)((V + 31) / 32);
@@ -64,12 +65,17 @@ Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, bool twice) {
             const int c = 1 << lg;
             if (V / c > (1 << 18) || (threads == t && c < ctas) || (threads && threads != t)) continue;
             if (threads && best != 0.0) break;
-            if (best != 0.0 && bytes / c < 16 * t) break;  // less than half a step of the CTA's threads
-            const int64_t clusters = (int64_t)sms * (512 / t) / c;
+            if (best != 0.0 && bytes / c < 16 * t) break;  // less than a quarter of a step of the CTA's threads
+            const int64_t by_smem = 227 * 1024 / (RowStream<kF32, 1, 1>::kBytes * t + shared(t, lg) + 3 * 1024);
+            int64_t held = by_smem < kSmThreads / t ? by_smem : kSmThreads / t;
+            if (held < 1) continue;
+            if (twice)  // no more rows at a time than the L2 keeps from one pass over them to the next
+                while (held > 1 && (double)sms * held / c * bytes > kResident) --held;
+            const int64_t clusters = (int64_t)sms * held / c;
             const double rounds = (double)((N + clusters - 1) / clusters);
-            const double rate = 1.0 / (512 / t);  // CTAs of an SM share it
-            double time = rounds * (bytes / c / rate * 1.0 + (c > 1 ? 2.0 : 1.0) * kRowCost * 2);
-            if (twice && (double)(N < clusters ? N : clusters) * bytes > kResident) time *= 1.3;
+            // CTAs of an SM share its rate, which few threads do not reach
+            const double rate = held * t < 640 ? held * t / 640.0 : 1.0;
+            const double time = rounds * (bytes / c * held / rate + (c > 1 ? 2.0 : 1.0) * kRowCost);
             if (best == 0.0 || time < best) {
                 best = time;
                 p.threads = t;
@@ -158,7 +164,9 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.logprob = tokens ? logprob : nullptr, a.entropy = entropy, a.stats = reinterpret_cast<float2*>(stats);
     a.top_index = top_index, a.top_logprob = top_logprob;
-    const Plan p = plan_rows(a.N, V, dtype, sms, false);
+    const Plan p = plan_rows(a.N, V, dtype, sms, false, [&](int, int lg) {
+        return k > 0 ? 9 * 1024 + 8 * (top_list(a.k, lg) + (lg ? a.k : 0)) : 0;
+    });
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
@@ -199,7 +207,7 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.stats = reinterpret_cast<const float2*>(stats), a.entropy = entropy, a.top_index = top_index;
     a.g_logprob = g_logprob, a.g_entropy = g_entropy, a.g_top = k > 0 ? g_top : nullptr;
-    const Plan p = plan_rows(a.N, V, dtype, sms, false);
+    const Plan p = plan_rows(a.N, V, dtype, sms, false, [](int, int) { return 0; });
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
@@ -258,7 +266,9 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
         if (loss)
             if ((st = launch(distill_begin_kernel, 1, 1024, 0, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
     }
-    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits != nullptr) : Plan{1, 256, 0, 1};
+    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits != nullptr, [&](int t, int lg) {
+        return tail ? distill_bitmap(a.V, 1 << lg, dtype == IL_BF16 ? 8 : 4, 4 * t) : 0;
+    }) : Plan{1, 256, 0, 1};
     const bool two = a.hard && a.tau != 1.0f;
     return with_dtype(dtype, [&](auto dt) {
         return with_bool(tail != 0, [&](auto tl) {

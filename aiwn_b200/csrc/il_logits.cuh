@@ -28,6 +28,7 @@ constexpr int kMaxTop = 128;         // alternatives, or the teacher's slots, of
 constexpr int kMaxVocab = 1 << 21;   // a row split over 16 CTAs keeps its bitmap in shared memory
 constexpr int kWarpVocab = 1024;     // rows up to this long are held in one warp's registers
 constexpr int kMaxCluster = 16;
+constexpr int kSmThreads = 768;      // of the CTAs that an SM holds of the kernels of longer rows
 constexpr float kLog2e = 1.44269504088896341f;
 
 // rows r = b*T + t of a [B, T, V] tensor whose last dimension is contiguous
@@ -556,10 +557,9 @@ __device__ __forceinline__ void copy_wait() {
 // gone through kPasses times.
 template <int DT, int kThreads, int kPasses>
 struct RowStream {
-    static constexpr int kVec = Elem<DT>::kVec, kU = 4, kElems = kU * kVec, kStages = 4;
+    static constexpr int kVec = Elem<DT>::kVec, kU = 4, kElems = kU * kVec, kStages = 3;
     static constexpr int kStep = kU * kThreads;  // vectors of a step
     static constexpr uint32_t kStepBytes = kStep * 16, kBytes = kStages * kStepBytes;
-    static_assert((kStages & (kStages - 1)) == 0, "the places are gone round by a mask");
     using T = typename Elem<DT>::type;
 
     const RowsIn& z;
@@ -624,7 +624,7 @@ struct RowStream {
             }
         }
         copy_commit();
-        put = (put + kStepBytes) & (kBytes - 1);
+        put = put + kStepBytes == kBytes ? 0 : put + kStepBytes;
     }
 
     // this thread's next kU vectors, of which the row has `mine`; the others are -inf
@@ -641,7 +641,7 @@ struct RowStream {
                              : "r"(from)
                              : "memory");
         }
-        get = (get + kStepBytes) & (kBytes - 1);
+        get = get + kStepBytes == kBytes ? 0 : get + kStepBytes;
     }
 };
 

@@ -239,7 +239,7 @@ __device__ __forceinline__ float warp_largest(float v, int j) {
 template <int DT, int kThreads, int kU>
 struct Top {
     static constexpr int kVec = Elem<DT>::kVec, kWarps = kThreads / 32, kStep = kU * kThreads;
-    static constexpr int kGroups = 4096 / kThreads;  // of steps, that a row's steps are put into
+    static constexpr int kGroups = 2048 / kThreads;  // of steps, that a row's steps are put into
     struct Shared {
         uint16_t most[kGroups][kThreads];       // maxima of the groups
         uint16_t hits[kWarps][kGroups * 32];
@@ -388,7 +388,7 @@ struct Top {
 };
 
 template <int DT, int kThreads, bool TOP>
-__global__ void __launch_bounds__(kThreads, 512 / kThreads) score_row_kernel(ScoreArgs a, uint32_t lg) {
+__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads) score_row_kernel(ScoreArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
     using Stream = RowStream<DT, kThreads, 1>;
     constexpr int kU = Stream::kU, kWarps = kThreads / 32;
