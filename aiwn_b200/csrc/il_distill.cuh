@@ -458,7 +458,7 @@ __device__ __forceinline__ uint4 without(const uint4& r, uint32_t bits) {
 // read a row before their logits, and those (and what they come to) right after the sums of the row before.  The
 // first two warps bring a row's sums and its slots' together.
 template <int DT, int kThreads, bool TAIL, bool S1, bool GRAD>
-__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads) distill_row_kernel(DistillArgs a, uint32_t lg) {
+__global__ void __launch_bounds__(kThreads, sm_threads(GRAD ? 2 : 1) / kThreads) distill_row_kernel(DistillArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
     using Stream = RowStream<DT, kThreads, GRAD ? 2 : 1>;
     constexpr int kVec = Elem<DT>::kVec, kU = Stream::kU, kWarps = kThreads / 32;

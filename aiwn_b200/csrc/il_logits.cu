@@ -40,14 +40,16 @@ int check_rows(int dtype, int64_t B, int64_t T, int64_t V, double temperature) {
 // the row stride of the operands and their element size: natural alignment of the base is all that is asked
 int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_BF16 ? 1u : 3u)) ? IL_ERR_ALIGN : IL_OK; }
 
-// Rows of more than kWarpVocab logits.  An SM holds kSmThreads threads, in CTAs of 128, 256 or 512: a warp's share
+// Rows of more than kWarpVocab logits.  An SM holds 512 or 768 threads, in CTAs of 128, 256 or 512: a warp's share
 // of what a row costs beside its logits is the same whatever the row's length, so that shorter rows get fewer warps.
-// Then the CTAs of a row: those that take the shortest time by a simple count, in which a cluster of c CTAs has 1/c
-// of a row to load and the rest costs as much as kRowCost bytes, twice as much in a cluster.  shared(t, lg): bytes of
-// shared memory of a CTA beside its stream.
+// Where all rows are at work at once and leave SMs idle, a cluster of c CTAs takes a row.  Of these the one that takes
+// the shortest time by a simple count: a CTA has 1/c of a row to load at its share of the SM's rate, and the rest costs
+// as much as kRowCost bytes, more for each doubling of a cluster.  A row that is gone through twice finds itself in the
+// L2 the second time as long as the rows at work are not more than kResident bytes.
+// shared(t, lg): bytes of shared memory of a CTA beside its stream.
 // AIWN_IL_LOGITS=threads,ctas pins both where they can serve the row (for the tests).
 template <class Shared>
-Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, bool twice, Shared shared) {
+Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, int passes, Shared shared) {
     Plan p{0, 256, 0, 0};
     if (V <= kWarpVocab) {
         p.regs = (int)((V + 31) / 32);
@@ -56,33 +58,36 @@ Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, bool twice, Shared shar
         return p;
     }
     const double bytes = (double)V * (dtype == IL_BF16 ? 2 : 4);
+    const int stream = passes > 1 ? RowStream<kF32, 1, 2>::kBytes : RowStream<kF32, 1, 1>::kBytes;  // a thread
     double best = 0.0;
     int threads = 0, ctas = 0;
     const char* pin = getenv("AIWN_IL_LOGITS");
     if (pin && sscanf(pin, "%d,%d", &threads, &ctas) != 2) threads = ctas = 0;
-    for (int t = 128; t <= 512; t *= 2)
+    for (int t = 128; t <= 512; t *= 2) {
+        if (threads && threads != t) continue;
         for (int lg = 0; (1 << lg) <= kMaxCluster; ++lg) {
             const int c = 1 << lg;
-            if (V / c > (1 << 18) || (threads == t && c < ctas) || (threads && threads != t)) continue;
-            if (threads && best != 0.0) break;
-            if (best != 0.0 && bytes / c < 16 * t) break;  // less than a quarter of a step of the CTA's threads
-            const int64_t by_smem = 227 * 1024 / (RowStream<kF32, 1, 1>::kBytes * t + shared(t, lg) + 3 * 1024);
-            int64_t held = by_smem < kSmThreads / t ? by_smem : kSmThreads / t;
+            if (V / c > (1 << 18) || (threads && c < ctas)) continue;
+            if (threads && p.grid) break;
+            const int64_t by_smem = 227 * 1024 / (stream * t + shared(t, lg) + 3 * 1024);
+            int64_t held = by_smem < sm_threads(passes) / t ? by_smem : sm_threads(passes) / t;
             if (held < 1) continue;
-            if (twice)  // no more rows at a time than the L2 keeps from one pass over them to the next
+            if (p.grid && lg > 0 && !threads && (N * c > sms * held || bytes / c < 16 * t)) break;
+            if (passes > 1)
                 while (held > 1 && (double)sms * held / c * bytes > kResident) --held;
-            const int64_t clusters = (int64_t)sms * held / c;
+            const int64_t clusters = (int64_t)sms * held / c, used = N < clusters ? N : clusters;
             const double rounds = (double)((N + clusters - 1) / clusters);
-            // CTAs of an SM share its rate, which few threads do not reach
-            const double rate = held * t < 640 ? held * t / 640.0 : 1.0;
-            const double time = rounds * (bytes / c * held / rate + (c > 1 ? 2.0 : 1.0) * kRowCost);
-            if (best == 0.0 || time < best) {
+            const double on_sm = (double)((used * c + sms - 1) / sms);  // CTAs that share an SM
+            const double rate = on_sm * t < 640 ? on_sm * t / 640.0 : 1.0;
+            const double time = rounds * (bytes / c * on_sm / rate + (1 + lg) * kRowCost);
+            if (p.grid == 0 || time < best) {
                 best = time;
                 p.threads = t;
                 p.lg = lg;
-                p.grid = (unsigned)((N < clusters ? N : clusters) * c);
+                p.grid = (unsigned)(used * c);
             }
         }
+    }
     return p;
 }
 
@@ -164,7 +169,7 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.logprob = tokens ? logprob : nullptr, a.entropy = entropy, a.stats = reinterpret_cast<float2*>(stats);
     a.top_index = top_index, a.top_logprob = top_logprob;
-    const Plan p = plan_rows(a.N, V, dtype, sms, false, [&](int, int lg) {
+    const Plan p = plan_rows(a.N, V, dtype, sms, 1, [&](int, int lg) {
         return k > 0 ? 9 * 1024 + 8 * (top_list(a.k, lg) + (lg ? a.k : 0)) : 0;
     });
     cudaStream_t s = (cudaStream_t)stream;
@@ -207,7 +212,7 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.stats = reinterpret_cast<const float2*>(stats), a.entropy = entropy, a.top_index = top_index;
     a.g_logprob = g_logprob, a.g_entropy = g_entropy, a.g_top = k > 0 ? g_top : nullptr;
-    const Plan p = plan_rows(a.N, V, dtype, sms, false, [](int, int) { return 0; });
+    const Plan p = plan_rows(a.N, V, dtype, sms, 1, [](int, int) { return 0; });
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
@@ -266,7 +271,7 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
         if (loss)
             if ((st = launch(distill_begin_kernel, 1, 1024, 0, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
     }
-    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits != nullptr, [&](int t, int lg) {
+    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits ? 2 : 1, [&](int t, int lg) {
         return tail ? distill_bitmap(a.V, 1 << lg, dtype == IL_BF16 ? 8 : 4, 4 * t) : 0;
     }) : Plan{1, 256, 0, 1};
     const bool two = a.hard && a.tau != 1.0f;
@@ -279,7 +284,7 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
                     });
                 return with_bool(dlogits != nullptr, [&](auto gr) {
                     return with_threads(p.threads, [&](auto th) {
-                        const size_t smem = RowStream<dt.value, th.value, 1>::kBytes +
+                        const size_t smem = RowStream<dt.value, th.value, gr.value ? 2 : 1>::kBytes +
                                             (tl.value ? distill_bitmap(a.V, 1 << p.lg, Elem<dt.value>::kVec,
                                                                        RowStream<dt.value, th.value, 1>::kStep)
                                                       : 0);

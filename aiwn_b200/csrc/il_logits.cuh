@@ -28,7 +28,8 @@ constexpr int kMaxTop = 128;         // alternatives, or the teacher's slots, of
 constexpr int kMaxVocab = 1 << 21;   // a row split over 16 CTAs keeps its bitmap in shared memory
 constexpr int kWarpVocab = 1024;     // rows up to this long are held in one warp's registers
 constexpr int kMaxCluster = 16;
-constexpr int kSmThreads = 768;      // of the CTAs that an SM holds of the kernels of longer rows
+// threads of the CTAs that an SM holds of the kernels of longer rows, which go through a row once or twice
+constexpr int sm_threads(int passes) { return passes > 1 ? 512 : 768; }
 constexpr float kLog2e = 1.44269504088896341f;
 
 // rows r = b*T + t of a [B, T, V] tensor whose last dimension is contiguous
@@ -557,7 +558,7 @@ __device__ __forceinline__ void copy_wait() {
 // gone through kPasses times.
 template <int DT, int kThreads, int kPasses>
 struct RowStream {
-    static constexpr int kVec = Elem<DT>::kVec, kU = 4, kElems = kU * kVec, kStages = 3;
+    static constexpr int kVec = Elem<DT>::kVec, kU = 4, kElems = kU * kVec, kStages = kPasses > 1 ? 4 : 3;
     static constexpr int kStep = kU * kThreads;  // vectors of a step
     static constexpr uint32_t kStepBytes = kStep * 16, kBytes = kStages * kStepBytes;
     using T = typename Elem<DT>::type;

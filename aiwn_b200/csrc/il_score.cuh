@@ -388,7 +388,7 @@ struct Top {
 };
 
 template <int DT, int kThreads, bool TOP>
-__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads) score_row_kernel(ScoreArgs a, uint32_t lg) {
+__global__ void __launch_bounds__(kThreads, sm_threads(1) / kThreads) score_row_kernel(ScoreArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
     using Stream = RowStream<DT, kThreads, 1>;
     constexpr int kU = Stream::kU, kWarps = kThreads / 32;
