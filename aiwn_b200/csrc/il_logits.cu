@@ -46,10 +46,10 @@ int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_
 // the shortest time by a simple count: a CTA has 1/c of a row to load at its share of the SM's rate, and the rest costs
 // as much as kRowCost bytes, more for each doubling of a cluster.  A row that is gone through twice finds itself in the
 // L2 the second time as long as the rows at work are not more than kResident bytes.
-// shared(t, lg): bytes of shared memory of a CTA beside its stream.
+// shared(t, lg): bytes of shared memory of a CTA beside its stream; least: threads that it has at least.
 // AIWN_IL_LOGITS=threads,ctas pins both where they can serve the row (for the tests).
 template <class Shared>
-Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, int passes, Shared shared) {
+Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, int passes, int least, Shared shared) {
     Plan p{0, 256, 0, 0};
     if (V <= kWarpVocab) {
         p.regs = (int)((V + 31) / 32);
@@ -64,7 +64,7 @@ Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, int passes, Shared shar
     const char* pin = getenv("AIWN_IL_LOGITS");
     if (pin && sscanf(pin, "%d,%d", &threads, &ctas) != 2) threads = ctas = 0;
     for (int t = 128; t <= 512; t *= 2) {
-        if (threads && threads != t) continue;
+        if (threads ? threads != t : t < least) continue;
         for (int lg = 0; (1 << lg) <= kMaxCluster; ++lg) {
             const int c = 1 << lg;
             if (V / c > (1 << 18) || (threads && c < ctas)) continue;
@@ -169,7 +169,9 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.logprob = tokens ? logprob : nullptr, a.entropy = entropy, a.stats = reinterpret_cast<float2*>(stats);
     a.top_index = top_index, a.top_logprob = top_logprob;
-    const Plan p = plan_rows(a.N, V, dtype, sms, 1, [&](int, int lg) {
+    // more alternatives than a quarter of the lanes make the bound of their maxima a weak one (4096 x 131072 bf16, 128
+    // alternatives: 627 us with 128 threads, 393 us with 256)
+    const Plan p = plan_rows(a.N, V, dtype, sms, 1, a.k > 64 ? 256 : 128, [&](int, int lg) {
         return k > 0 ? 9 * 1024 + 8 * (top_list(a.k, lg) + (lg ? a.k : 0)) : 0;
     });
     cudaStream_t s = (cudaStream_t)stream;
@@ -212,7 +214,7 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.stats = reinterpret_cast<const float2*>(stats), a.entropy = entropy, a.top_index = top_index;
     a.g_logprob = g_logprob, a.g_entropy = g_entropy, a.g_top = k > 0 ? g_top : nullptr;
-    const Plan p = plan_rows(a.N, V, dtype, sms, 1, [](int, int) { return 0; });
+    const Plan p = plan_rows(a.N, V, dtype, sms, 1, 128, [](int, int) { return 0; });
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
@@ -271,7 +273,7 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
         if (loss)
             if ((st = launch(distill_begin_kernel, 1, 1024, 0, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
     }
-    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits ? 2 : 1, [&](int t, int lg) {
+    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits ? 2 : 1, 128, [&](int t, int lg) {
         return tail ? distill_bitmap(a.V, 1 << lg, dtype == IL_BF16 ? 8 : 4, 4 * t) : 0;
     }) : Plan{1, 256, 0, 1};
     const bool two = a.hard && a.tau != 1.0f;

@@ -239,10 +239,11 @@ __device__ __forceinline__ float warp_largest(float v, int j) {
 template <int DT, int kThreads, int kU>
 struct Top {
     static constexpr int kVec = Elem<DT>::kVec, kWarps = kThreads / 32, kStep = kU * kThreads;
-    static constexpr int kGroups = 2048 / kThreads;  // of steps, that a row's steps are put into
+    static constexpr int kGroups = 4096 / kThreads;  // of steps, that a row's steps are put into
+    static constexpr int kHits = 128;                // that a warp reads again at a time
     struct Shared {
         uint16_t most[kGroups][kThreads];       // maxima of the groups
-        uint16_t hits[kWarps][kGroups * 32];
+        uint16_t hits[kWarps][kHits];
         float deposit[2][kWarps];
         int scan[kWarps];
         int count;
@@ -262,35 +263,20 @@ struct Top {
     }
 
     __device__ __forceinline__ void put(float z, int index) const {
-        const int at = atomicAdd(&sh->count, 1);
+        const int at = (int)atom_add_shared_u32(smem_addr(&sh->count), 1u);
         if (at < cap) list[at] = ((uint64_t)order_key(z) << 32) | (uint32_t)~index;
     }
     __device__ __forceinline__ static bool reaches(float z, float bound, bool above) {
         return above ? z > bound : z >= bound;  // not NaN
     }
 
-    // Lists the part's logits that reach the bound (above: that are above it), sh->count of them; false: more than
-    // the list holds.  sh->count is 0.  lg: log2 of the steps of a group; end, end_at, ends: this thread's logit of
-    // the row's ends.
-    __device__ __forceinline__ bool collect(const T* zr, const Segment& g, int lg, float end, int end_at, int ends,
-                                            float bound, bool above) const {
-        const int tid = threadIdx.x, lane = tid & 31;
-        const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
-        const int groups = (g.v1 - g.v0 + (kStep << lg) - 1) / (kStep << lg);
-        uint16_t* hits = sh->hits[tid >> 5];  // of this warp
-        int n = 0;
-        for (int i = 0; i < groups; ++i) {
-            const bool hit = reaches(__uint_as_float((uint32_t)sh->most[i][tid] << 16), bound, above);
-            const unsigned who = __ballot_sync(0xffffffffu, hit);
-            if (hit) hits[n + __popc(who & ((1u << lane) - 1u))] = (uint16_t)(i * kThreads + tid);
-            n += __popc(who);
-        }
-        __syncwarp();
-        if (tid < ends && reaches(end, bound, above)) put(end, end_at);
+    // lists what reaches the bound in n groups of this warp
+    __device__ __forceinline__ void reread(const uint4* body, const Segment& g, const uint16_t* hits, int n, int lg,
+                                           float bound, bool above) const {
         // vector q of hit h is item (h << per) + q; four items of a lane are loaded at a time
-        const int per = 2 + lg, items = n << per;
         static_assert(kU == 4, "a step of a group is 4 vectors");
-        for (int i = lane; i < items; i += 4 * 32) {
+        const int per = 2 + lg, items = n << per;
+        for (int i = threadIdx.x & 31; i < items; i += 4 * 32) {
             uint4 r[4];
             int v[4];
 #pragma unroll
@@ -309,11 +295,38 @@ struct Top {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 if (v[w] < 0) continue;
+                const uint4 one[1] = {r[w]};
+                if (!reaches(max_of<DT>(one), bound, above)) continue;
                 float x[kVec];
                 unpack16<DT>(r[w], x);
 #pragma unroll
                 for (int e = 0; e < kVec; ++e)
                     if (reaches(x[e], bound, above)) put(x[e], g.h0 + v[w] * kVec + e);
+            }
+        }
+    }
+
+    // Lists the part's logits that reach the bound (above: that are above it), sh->count of them; false: more than
+    // the list holds.  sh->count is 0.  lg: log2 of the steps of a group; end, end_at, ends: this thread's logit of
+    // the row's ends.
+    __device__ __forceinline__ bool collect(const T* zr, const Segment& g, int lg, float end, int end_at, int ends,
+                                            float bound, bool above) const {
+        const int tid = threadIdx.x, lane = tid & 31;
+        const uint4* body = reinterpret_cast<const uint4*>(zr + g.h0);
+        const int groups = (g.v1 - g.v0 + (kStep << lg) - 1) / (kStep << lg);
+        uint16_t* hits = sh->hits[tid >> 5];  // of this warp
+        if (tid < ends && reaches(end, bound, above)) put(end, end_at);
+        int n = 0;
+        for (int i = 0; i < groups; ++i) {
+            const bool hit = reaches(__uint_as_float((uint32_t)sh->most[i][tid] << 16), bound, above);
+            const unsigned who = __ballot_sync(0xffffffffu, hit);
+            if (hit) hits[n + __popc(who & ((1u << lane) - 1u))] = (uint16_t)(i * kThreads + tid);
+            n += __popc(who);
+            if (n > kHits - 32 || i == groups - 1) {
+                __syncwarp();
+                reread(body, g, hits, n, lg, bound, above);
+                __syncwarp();
+                n = 0;
             }
         }
         __syncthreads();
