@@ -29,6 +29,7 @@ from . import _lib
 from .layers import GaussianCDFNorm, IndexedLinear
 from .layers.indexed_linear import TRITON_OK, _Fn, grad_pair
 from .layers.indexed_linear_v2 import _FnV2
+from .scoring import TokenScores, distill_loss, token_logprobs
 
 
 class _LayerNormFn(torch.autograd.Function):
@@ -286,6 +287,19 @@ class IndexedGPT(nn.Module):
             loss = F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1))
         return logits, loss
 
+    def score(self, idx, targets=None, top_k: int = 0, *, temperature: float = 1.0,
+              ignore_index: int = -100) -> TokenScores:
+        """The log probabilities of ``targets`` [B, T] (the next tokens; None: left out), the entropy of each position
+        and its ``top_k`` alternatives under the model, as ``token_logprobs`` gives them.  Under ``torch.no_grad()``
+        its ``top_index`` and ``top_logprob`` are what another model's ``distill`` takes."""
+        return token_logprobs(self(idx)[0], targets, top_k, temperature=temperature, ignore_index=ignore_index)
+
+    def distill(self, idx, top_index, top_logprob, targets=None, **options):
+        """(logits, loss) like ``forward``, with ``distill_loss`` of a teacher's ``top_index`` and ``top_logprob``
+        [B, T, k] (and, for ``alpha < 1`` or padding, of ``targets``) as the loss; ``options`` are distill_loss's."""
+        logits, _ = self(idx)
+        return logits, distill_loss(logits, top_index, top_logprob, targets, **options)
+
     def get_indexed_layers(self):
         layers = []
         for blk in self.transformer["h"]:
@@ -303,6 +317,12 @@ class GraphedTrainStep:
         step = GraphedTrainStep(model, opt, batch, ctx)
         loss = step(x, y)          # device int64 [batch, ctx]; returns the loss tensor
 
+    With ``teacher_k`` > 0 the loss is ``model.distill``'s, on a teacher's ``teacher_k`` alternatives a position and
+    with the options ``distill`` (a dict of distill_loss's keywords):
+
+        step = GraphedTrainStep(model, opt, batch, ctx, teacher_k=8, distill=dict(alpha=0.5, temperature=2.0))
+        loss = step(x, y, top_index, top_logprob)   # [batch, ctx, 8], teacher.score(x, None, 8, temperature=2.0)'s
+
     The optimizer must be capturable.  Gradients live in the graph's memory
     pool and are overwritten (not accumulated) every step.  Construction runs
     ``warmup`` eager steps (on all-zero tokens) so that the optimizer state and
@@ -310,9 +330,17 @@ class GraphedTrainStep:
     zeroes the optimizer state: the model is unchanged until the first call.
     """
 
-    def __init__(self, model, optimizer, batch_size, block_size, clip: float = 1.0, warmup: int = 3):
+    def __init__(self, model, optimizer, batch_size, block_size, clip: float = 1.0, warmup: int = 3, *,
+                 teacher_k: int = 0, distill=None):
         dev = next(model.parameters()).device
         self.model, self.opt, self.clip = model, optimizer, clip
+        if distill and not teacher_k:
+            raise ValueError("distill options without teacher_k")
+        self.top_index = self.top_logprob = None
+        self.distill = dict(distill or {})
+        if teacher_k:  # no alternatives until the first call brings some
+            self.top_index = torch.full((batch_size, block_size, teacher_k), -1, dtype=torch.long, device=dev)
+            self.top_logprob = torch.zeros(batch_size, block_size, teacher_k, device=dev)
         self.x = torch.zeros(batch_size, block_size, dtype=torch.long, device=dev)
         self.y = torch.zeros(batch_size, block_size, dtype=torch.long, device=dev)
         saved = [p.detach().clone() for p in model.parameters()]
@@ -321,7 +349,7 @@ class GraphedTrainStep:
         with torch.cuda.stream(side):  # warm-up: optimizer state, autograd, kernel set-up
             for _ in range(warmup):
                 self.opt.zero_grad(set_to_none=True)
-                _, loss = self.model(self.x, self.y)
+                loss = self._loss()
                 loss.backward()
                 torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.clip)
                 self.opt.step()
@@ -336,13 +364,23 @@ class GraphedTrainStep:
         self.graph = torch.cuda.CUDAGraph()
         self.opt.zero_grad(set_to_none=True)
         with torch.cuda.graph(self.graph, capture_error_mode="relaxed"):
-            _, self.loss = self.model(self.x, self.y)
+            self.loss = self._loss()
             self.loss.backward()
             torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.clip)
             self.opt.step()
 
-    def __call__(self, x, y):
+    def _loss(self):
+        if self.top_index is None:
+            return self.model(self.x, self.y)[1]
+        return self.model.distill(self.x, self.top_index, self.top_logprob, self.y, **self.distill)[1]
+
+    def __call__(self, x, y, top_index=None, top_logprob=None):
+        if (top_index is None or top_logprob is None) != (self.top_index is None):
+            raise ValueError("a step with teacher_k takes top_index and top_logprob, one without takes neither")
         self.x.copy_(x, non_blocking=True)
         self.y.copy_(y, non_blocking=True)
+        if self.top_index is not None:
+            self.top_index.copy_(top_index, non_blocking=True)
+            self.top_logprob.copy_(top_logprob, non_blocking=True)
         self.graph.replay()
         return self.loss
