@@ -483,9 +483,11 @@ __global__ void __launch_bounds__(kThreads, sm_threads(GRAD ? 2 : 1) / kThreads)
     Stream stream(a.z, a.V, list, step, rank, lg, sm);
     // rows of padding
     if (a.tok.p && (GRAD || (a.loss && a.each))) {
+        uint32_t live = 0;
         for (uint32_t i = 0; i < list.count; ++i) {
-            const uint32_t live = list.window(i & ~31u), row = list.row(i);
+            if ((i & 31) == 0) live = list.window(i);
             if (live >> (i & 31) & 1u) continue;
+            const uint32_t row = list.row(i);
             if (a.loss && a.each && rank == 0 && tid == 0) a.loss[row] = 0.0f;
             if constexpr (GRAD) {
                 T* dr = reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row);

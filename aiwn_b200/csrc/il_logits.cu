@@ -63,16 +63,18 @@ Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, int passes, int least, 
     int threads = 0, ctas = 0;
     const char* pin = getenv("AIWN_IL_LOGITS");
     if (pin && sscanf(pin, "%d,%d", &threads, &ctas) != 2) threads = ctas = 0;
+    int lg0 = 0;  // the least that a CTA's part of a row allows
+    while ((V >> lg0) > (1 << 18)) ++lg0;
     for (int t = 128; t <= 512; t *= 2) {
         if (threads ? threads != t : t < least) continue;
-        for (int lg = 0; (1 << lg) <= kMaxCluster; ++lg) {
+        for (int lg = lg0; (1 << lg) <= kMaxCluster; ++lg) {
             const int c = 1 << lg;
-            if (V / c > (1 << 18) || (threads && c < ctas)) continue;
+            if (threads && c < ctas && 2 * c <= kMaxCluster) continue;
             if (threads && p.grid) break;
             const int64_t by_smem = 227 * 1024 / (stream * t + shared(t, lg) + 3 * 1024);
             int64_t held = by_smem < sm_threads(passes) / t ? by_smem : sm_threads(passes) / t;
             if (held < 1) continue;
-            if (p.grid && lg > 0 && !threads && (N * c > sms * held || bytes / c < 16 * t)) break;
+            if (lg > lg0 && !threads && (N * c > sms * held || bytes / c < 16 * t)) break;
             if (passes > 1)
                 while (held > 1 && (double)sms * held / c * bytes > kResident) --held;
             const int64_t clusters = (int64_t)sms * held / c, used = N < clusters ? N : clusters;

@@ -422,11 +422,13 @@ __global__ void __launch_bounds__(kThreads, sm_threads(1) / kThreads) score_row_
         if (tid == 0) top_shared.count = 0;
     }
     int parity = 0;
-    if (rank == 0 && a.tok.p)
+    if (rank == 0 && a.tok.p) {
+        uint32_t live = 0;
         for (uint32_t i = 0; i < list.count; ++i) {
-            const uint32_t live = list.window(i & ~31u);
+            if ((i & 31) == 0) live = list.window(i);
             if (!(live >> (i & 31) & 1u)) score_padding(a, list.row(i), tid, kThreads);
         }
+    }
     for (LiveRows at(a.z, list, step); at.valid(); at.next()) {
         const uint32_t row = at.row();
         const T* zr = reinterpret_cast<const T*>(a.z.p) + at.at.off;
@@ -607,19 +609,24 @@ __global__ void __launch_bounds__(256) score_grad_warp_kernel(ScoreGradArgs a) {
     const int lane = threadIdx.x & 31;
     const uint32_t warps = gridDim.x * 8;
     for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < a.N; row += warps) {
+        // everything is asked for before the first use of any of it
         const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : -1;
         T* dr = reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row);
-        if (a.tok.p && t == a.tok.ignore) {
-            for (int j = lane; j < a.V; j += 32) dr[j] = from_float<T>(0.0f);
-            continue;
-        }
         const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
-        const ScoreGrad r = score_grad_row(a, row, t);
+        float x[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int j = lane + 32 * e;
-            if (j < a.V) dr[j] = from_float<T>(r.at(to_float(zr[j])) * r.inv_tau);
+            x[e] = j < a.V ? to_float(zr[j]) : 0.0f;
         }
+        const ScoreGrad r = score_grad_row(a, row, t);
+        const bool live = !(a.tok.p && t == a.tok.ignore);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int j = lane + 32 * e;
+            if (j < a.V) dr[j] = from_float<T>(live ? r.at(x[e]) * r.inv_tau : 0.0f);
+        }
+        if (!live) continue;
         __syncwarp();
         score_grad_slots<T>(a, r, row, t, zr, dr, 0, a.V, lane, 32);
     }

@@ -88,12 +88,11 @@ def _temperature(t):
 
 def _score(rows, tokens, k, temperature, ignore_index, lead, with_stats):
     """(logprob, entropy, top_index, top_logprob) over the leading dimensions `lead`, and stats or None."""
-    dev = rows.device
-    logprob = torch.empty(lead, dtype=torch.float32, device=dev) if tokens is not None else None
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    index = torch.empty((*lead, k), dtype=torch.int64, device=dev)
-    top = torch.empty((*lead, k), dtype=torch.float32, device=dev)
-    stats = torch.empty((*lead, 2), dtype=torch.float32, device=dev) if with_stats else None
+    entropy = torch.empty(lead, dtype=torch.float32, device=rows.device)
+    logprob = torch.empty_like(entropy) if tokens is not None else None
+    index = torch.empty((*lead, k), dtype=torch.int64, device=rows.device)
+    top = entropy.new_empty((*lead, k))
+    stats = entropy.new_empty((*lead, 2)) if with_stats else None
     _lib.run_token_logprobs(rows, tokens, ignore_index, temperature, k, logprob, entropy, stats, index, top)
     return logprob, entropy, index, top, stats
 
