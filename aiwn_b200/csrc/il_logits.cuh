@@ -315,7 +315,10 @@ __device__ __noinline__ Sums huge_vector(uint4 r, float m, float c) {
 // A thread's sums while a row goes by.  The exponent is taken to a whole number H next to
 // m log2(e) / tau: d = z c - H is one fused multiply-add, rounded once, and a new maximum
 // rescales by a power of two, without rounding.  Where |m| c is 2^22 or more (a row of nothing
-// but a mask's huge negative values) such an H has no meaning, and d = (z - m) c.
+// but a mask's huge negative values) such an H has no meaning, and d = (z - m) c; so it is where
+// c is so small (a temperature above 10^20) that floor16's -2^100 would count for something.
+constexpr float kLeastFactor = 1e-20f;
+
 template <bool U, bool S1>
 struct Running {
     float m, s, u, s1, h, h1;  // h, h1: -H for c and for log2(e)
@@ -330,7 +333,7 @@ struct Running {
 
     __device__ __forceinline__ void raise(float top, float c) {
         const float t = top * c;
-        const bool now = is_huge(t) || (S1 && is_huge(top * kLog2e));
+        const bool now = is_huge(t) || (S1 && is_huge(top * kLog2e)) || (U && c < kLeastFactor);
         const float g = now ? -t : -rintf(t), g1 = now ? -top * kLog2e : -rintf(top * kLog2e);
         if (m != -INFINITY) {
             const float d = fmaxf(now && huge ? (m - top) * c : g - h, kMinExp), f = exp2_approx(d);

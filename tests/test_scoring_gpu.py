@@ -47,6 +47,9 @@ def mask_(z, kind, seed=1):
         z[..., torch.arange(V, device=DEV) != V // 2] = float("-inf")
     elif kind == "empty_row":
         z[0, 0] = float("-inf")
+    elif kind == "all_masked":  # by finite values: what is left is an even distribution
+        z[0, 0] = LOWEST
+        z[-1, -1] = -1e9
     elif kind == "equal":
         z.fill_(1.5)
     elif kind == "two_values":
@@ -91,7 +94,7 @@ def test_scores(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
-@pytest.mark.parametrize("kind", ["neg_inf", "lowest", "one_left", "empty_row", "equal", "two_values", "rising",
+@pytest.mark.parametrize("kind", ["neg_inf", "lowest", "one_left", "empty_row", "all_masked", "equal", "two_values", "rising",
                                   "falling", "signed_zeros"])
 def test_scores_of_masked_and_tied_rows(kind, dtype):
     for B, T, V, k in [(2, 2, 65, 30), (2, 3, 1024, 128), (2, 2, 1025, 128), (3, 2, 40007, 128), (1, 1, 131072, 64),
@@ -458,3 +461,127 @@ def test_long_rows_beyond_32_bit_offsets():
     check_scores(every, tokens, 20, 1.0, r)
     index, logprob = teacher(1, 2, V, 20)
     check_distill(every, index, logprob, tokens, alpha=0.5, tail=True)
+
+
+PINS = ["128,1", "256,1", "512,1", "128,4", "256,2", "512,16"]
+
+
+@pytest.mark.parametrize("pin", PINS)
+def test_every_plan(pin, monkeypatch):
+    """CTAs of every size and clusters of several, whatever the plan would take: rows whose part for a CTA is less than
+    a step and more than several, many rows a cluster, ties that run over a list, padding between the rows."""
+    monkeypatch.setenv("AIWN_IL_LOGITS", pin)
+    few = [(2, 3, 1025), (3, 2, 5003), (1, 3, 40007)]
+    many = [(300, 3, 1500), (700, 2, 4099)]
+    for dtype in (torch.float32, torch.bfloat16):
+        for n, (B, T, V) in enumerate(few + many):
+            for layout, k in (("behind", 0), ("offset", 7), ("shifted", 100)):
+                z = make_logits(B, T, V, dtype, layout, seed=n)
+                tokens = torch.randint(0, V, z.shape[:2], device=DEV)
+                tokens[torch.rand(z.shape[:2], device=DEV) < 0.3] = IGNORE
+                check_scores(z, tokens, k, 0.8, token_logprobs(z, tokens, k, temperature=0.8))
+            for k, alpha, tau, tail in ((33, 0.5, 2.0, False), (20, 1.0, 1.0, True), (100, 0.9, 0.7, True)):
+                index, logprob = teacher(*z.shape[:2], V, k, seed=n)
+                check_distill(z, index, logprob, tokens, alpha=alpha, temperature=tau, tail=tail)
+        for kind in ("neg_inf", "lowest", "all_masked", "equal", "two_values", "rising", "falling", "empty_row"):
+            z = mask_(make_logits(4, 3, 9001, dtype, "behind"), kind)
+            tokens = torch.randint(0, 9001, (4, 3), device=DEV)
+            check_scores(z, tokens, 90, 1.0, token_logprobs(z, tokens, 90))
+            if kind in ("all_masked", "equal"):  # a slot that a mask holds at -3e38 would make a loss of 3e38
+                index, logprob = teacher(4, 3, 9001, 12)
+                check_distill(z, index, logprob, tokens, alpha=0.5, tail=True)
+                check_distill(z, index, logprob, tokens, alpha=0.5, temperature=2.0)
+
+
+@pytest.mark.parametrize("V", [65, 5003, 40007])
+def test_results_do_not_change_from_run_to_run(V):
+    z = make_logits(6, 5, V, torch.bfloat16).requires_grad_(True)
+    index, logprob = teacher(6, 5, V, 30)
+    index[0, 0, 7] = index[0, 0, 3]
+    tokens = torch.randint(0, V, (6, 5), device=DEV)
+
+    def run():
+        r = token_logprobs(z, tokens, 40)
+        loss = distill_loss(z, index, logprob, tokens, alpha=0.5, temperature=2.0, tail=True)
+        (a,) = torch.autograd.grad([r.logprob, r.entropy, r.top_logprob], z,
+                                   [torch.ones_like(t) for t in (r.logprob, r.entropy, r.top_logprob)])
+        (b,) = torch.autograd.grad(loss, z)
+        return (*(t.detach() for t in r), loss.detach(), a, b)
+
+    first = run()
+    for _ in range(4):
+        for x, y in zip(first, run()):
+            assert torch.equal(x, y)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams share nothing."""
+    V = 40007
+    sets = []
+    for seed in range(2):
+        z = make_logits(8, 4, V, torch.float32, seed=seed).requires_grad_(True)
+        index, logprob = teacher(8, 4, V, 20, seed=seed)
+        sets.append((z, index, logprob))
+
+    def run(z, index, logprob):
+        loss = distill_loss(z, index, logprob)
+        return (loss.detach(), torch.autograd.grad(loss, z)[0], *token_logprobs(z.detach(), None, 30)[1:])
+
+    want = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got = []
+        for s, args in zip(streams, sets):
+            with torch.cuda.stream(s):
+                got.append([run(*args) for _ in range(3)])
+        torch.cuda.synchronize()
+        for w, g in zip(want, got):
+            for one in g:
+                for x, y in zip(w, one):
+                    assert torch.equal(x, y)
+
+
+def test_extreme_temperatures_and_logits():
+    for V in (65, 5003):
+        z = make_logits(2, 3, V, torch.float32)
+        tokens = torch.randint(0, V, (2, 3), device=DEV)
+        hot = token_logprobs(z, tokens, 3, temperature=1e30)
+        near(hot.entropy, torch.full((2, 3), V, device=DEV).double().log(), 1e-5, "uniform")
+        cold = token_logprobs(z, tokens, 3, temperature=1e-30)
+        assert torch.equal(cold.top_logprob[..., 0], torch.zeros(2, 3, device=DEV))
+        assert torch.equal(cold.entropy, torch.zeros(2, 3, device=DEV))
+        assert torch.equal(cold.top_index, token_logprobs(z, tokens, 3).top_index)
+        big = z * 1e7  # maxima beyond 2^22
+        r = token_logprobs(big, tokens, 2)
+        assert torch.equal(r.top_logprob[..., 0], torch.zeros(2, 3, device=DEV))
+        leaf = big.requires_grad_(True)
+        best = r.top_index[..., 0]
+        loss = distill_loss(leaf, best[..., None], torch.zeros(2, 3, 1, device=DEV))
+        loss.backward()
+        assert float(loss.detach()) == 0.0 and not leaf.grad.any()
+
+
+def test_logits_that_are_views_of_one_row():
+    """Rows of stride 0: one row's logits for every position, its gradient their sum."""
+    for V in (65, 5003):
+        row = make_logits(1, 1, V, torch.float32)[0, 0].requires_grad_(True)
+        z = row.expand(3, 4, V)
+        tokens = torch.randint(0, V, (3, 4), device=DEV)
+        r = token_logprobs(z, tokens, 2)
+        check_scores(z.detach(), tokens, 2, 1.0, type(r)(*(t.detach() for t in r)))
+        r.logprob.sum().backward()
+        want, size = score_grad64(z.detach(), tokens, 0, 1.0, *(torch.full((3, 4), v, device=DEV) for v in (1.0, 0.0)),
+                                  torch.zeros(3, 4, 0, device=DEV))
+        near(row.grad, want.sum((0, 1)), ((prob_tol(V) + 30 * F32) * size).sum((0, 1)) + F32 * want.abs().sum((0, 1)), V)
+
+
+def test_logits_changed_before_the_backward_are_noticed():
+    z = make_logits(1, 2, 70, torch.float32).requires_grad_(True)
+    index, logprob = teacher(1, 2, 70, 3)
+    for f in (lambda x: distill_loss(x, index, logprob), lambda x: token_logprobs(x, None).entropy.sum()):
+        x = z * 1.0
+        y = f(x)
+        x.mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
