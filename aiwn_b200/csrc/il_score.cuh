@@ -18,6 +18,12 @@
 // bound than the list holds, the k-th largest of those listed is a higher bound
 // for another round; where that is no higher, the list is of the logits above
 // the bound, and of those equal to it the first by index fill it up to k.
+// 4096 x 131072 bf16, 64 alternatives: 260 us, 174 us of them the sums'; a list
+// that every logit above a running bound was put into, with a barrier a step,
+// took 614 us, and reading eighths again instead of thirty-seconds 287 us.
+//
+// 8192 x 65536 bf16 with the gradient of log probability and entropy: 177 us
+// forward, 381 us backward (2.1 GB, 86% of the measured copy rate).
 #pragma once
 #include <type_traits>
 
