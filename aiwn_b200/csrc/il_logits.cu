@@ -46,7 +46,7 @@ int check_rows(int dtype, int64_t B, int64_t T, int64_t V, double temperature) {
 // the row stride of the operands and their element size: natural alignment of the base is all that is asked
 int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_BF16 ? 1u : 3u)) ? IL_ERR_ALIGN : IL_OK; }
 
-// Rows of more than kWarpVocab logits.  An SM holds 512 or 768 threads, in CTAs of 128, 256 or 512: a warp's share
+// Rows of more than kWarpVocab logits.  An SM holds 512 or 768 threads, in CTAs of 64 to 512: a warp's share
 // of what a row costs beside its logits is the same whatever the row's length, so that shorter rows get fewer warps.
 // Where all rows are at work at once and leave SMs idle, a cluster of c CTAs takes a row.  Of these the one that takes
 // the shortest time by a simple count: a CTA has 1/c of a row to load at its share of the SM's rate, and the rest costs
@@ -55,7 +55,7 @@ int check_align(const void* p, int dtype) { return ((uintptr_t)p & (dtype == IL_
 // shared(t, lg): bytes of shared memory of a CTA beside its stream; least: threads that it has at least.
 // AIWN_IL_LOGITS=threads,ctas pins both where they can serve the row (for the tests).
 template <class Shared>
-Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, int passes, int least, Shared shared) {
+Plan plan_rows(int64_t N, int64_t V, int64_t k, int dtype, int sms, int passes, int least, Shared shared) {
     Plan p{0, 256, 0, 0};
     if (V <= kWarpVocab) {
         p.regs = (int)((V + 31) / 32);
@@ -71,7 +71,9 @@ Plan plan_rows(int64_t N, int64_t V, int dtype, int sms, int passes, int least, 
     if (pin && sscanf(pin, "%d,%d", &threads, &ctas) != 2) threads = ctas = 0;
     int lg0 = 0;  // the least that a CTA's part of a row allows
     while ((V >> lg0) > (1 << 18)) ++lg0;
-    for (int t = 128; t <= 512; t *= 2) {
+    const int need = k > 64 ? 128 : 64;  // a slot, or an alternative, a thread
+    if (threads && threads < need) threads = need;
+    for (int t = need; t <= 512; t *= 2) {
         if (threads ? threads != t : t < least) continue;
         for (int lg = lg0; (1 << lg) <= kMaxCluster; ++lg) {
             const int c = 1 << lg;
@@ -144,6 +146,7 @@ int with_dtype(int dtype, F f) {
 }
 template <class F>
 int with_threads(int threads, F f) {
+    if (threads == 64) return f(std::integral_constant<int, 64>());
     if (threads == 128) return f(std::integral_constant<int, 128>());
     if (threads == 256) return f(std::integral_constant<int, 256>());
     return f(std::integral_constant<int, 512>());
@@ -179,7 +182,7 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
     a.top_index = top_index, a.top_logprob = top_logprob;
     // more alternatives than a quarter of the lanes make the bound of their maxima a weak one (4096 x 131072 bf16, 128
     // alternatives: 627 us with 128 threads, 393 us with 256)
-    const Plan p = plan_rows(a.N, V, dtype, sms, 1, a.k > 64 ? 256 : 128, [&](int, int lg) {
+    const Plan p = plan_rows(a.N, V, k, dtype, sms, 1, k > 64 ? 256 : k > 32 ? 128 : 64, [&](int, int lg) {
         return k > 0 ? 9 * 1024 + 8 * (top_list(a.k, lg) + (lg ? a.k : 0)) : 0;
     });
     cudaStream_t s = (cudaStream_t)stream;
@@ -222,7 +225,7 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.stats = reinterpret_cast<const float2*>(stats), a.entropy = entropy, a.top_index = top_index;
     a.g_logprob = g_logprob, a.g_entropy = g_entropy, a.g_top = k > 0 ? g_top : nullptr;
-    const Plan p = plan_rows(a.N, V, dtype, sms, 1, 128, [](int, int) { return 0; });
+    const Plan p = plan_rows(a.N, V, 0, dtype, sms, 1, 64, [](int, int) { return 0; });
     cudaStream_t s = (cudaStream_t)stream;
     return with_dtype(dtype, [&](auto dt) {
         if (p.regs)
@@ -233,7 +236,9 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
         while ((V >> lg) > 32768) ++lg;
         const int64_t grid = (int64_t)a.N << lg;
         if (grid > 0x7fffffff) return (int)IL_ERR_SHAPE;
-        return launch(score_grad_row_kernel<dt.value>, (unsigned)grid, kGradThreads, 0, 0, s, a, lg);
+        // short rows: one round of a few warps
+        if (V <= 8192) return launch(score_grad_row_kernel<dt.value, 128>, (unsigned)grid, 128, 0, 0, s, a, lg);
+        return launch(score_grad_row_kernel<dt.value, 512>, (unsigned)grid, 512, 0, 0, s, a, lg);
     });
 }
 
@@ -281,7 +286,7 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
         if (loss)
             if ((st = launch(distill_begin_kernel, 1, 1024, 0, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
     }
-    const Plan p = N > 0 ? plan_rows(N, V, dtype, sms, dlogits ? 2 : 1, 128, [&](int t, int lg) {
+    const Plan p = N > 0 ? plan_rows(N, V, k, dtype, sms, dlogits ? 2 : 1, 64, [&](int t, int lg) {
         return tail ? distill_bitmap(a.V, 1 << lg, dtype == IL_BF16 ? 8 : 4, 4 * t) : 0;
     }) : Plan{1, 256, 0, 1};
     const bool two = a.hard && a.tau != 1.0f;

@@ -15,7 +15,7 @@
 // with s = 0; NaN or +inf makes s NaN.
 //
 // Rows of up to 1024 logits are a warp's, in its registers.  Longer ones are a
-// CTA's of 128, 256 or 512 threads, or where there are fewer of them than the
+// CTA's of 64 to 512 threads, or where there are fewer of them than the
 // SMs can hold, a cluster's of up to 16.  What bounds these is first the
 // instructions of a logit (bf16, log probability and entropy: 11.5 an element
 // at first, 7.9 now, of about 11 that the SMs could issue at the rate of HBM), then what

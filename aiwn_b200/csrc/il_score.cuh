@@ -8,7 +8,7 @@
 // backward reads it once more and writes its gradient.
 //
 // The k largest.  While a row goes by, each thread keeps the maximum of every
-// sixteenth (or eighth, or thirty-second) of what it reads, rounded up to 16 bits, and
+// sixteenth (an eighth to a 64th) of what it reads, rounded up to 16 bits, and
 // nothing else is done for them.  Then, with W warps and j = k / W rounded up,
 // the least of the warps' j-th largest thread maxima is a bound that at least k
 // logits reach, and of a row in no particular order not many more; the few
@@ -638,11 +638,9 @@ __global__ void __launch_bounds__(256) score_grad_warp_kernel(ScoreGradArgs a) {
     }
 }
 
-constexpr int kGradThreads = 512;
-
 // CTA `part` of 2^lg of a row
-template <int DT>
-__global__ void __launch_bounds__(kGradThreads, 2) score_grad_row_kernel(ScoreGradArgs a, uint32_t lg) {
+template <int DT, int kGradThreads>
+__global__ void __launch_bounds__(kGradThreads, 1024 / kGradThreads) score_grad_row_kernel(ScoreGradArgs a, uint32_t lg) {
     using T = typename Elem<DT>::type;
     constexpr int kVec = Elem<DT>::kVec;
     const int tid = threadIdx.x;

@@ -463,7 +463,7 @@ def test_long_rows_beyond_32_bit_offsets():
     check_distill(every, index, logprob, tokens, alpha=0.5, tail=True)
 
 
-PINS = ["128,1", "256,1", "512,1", "128,4", "256,2", "512,16"]
+PINS = ["64,1", "64,8", "128,1", "256,1", "512,1", "128,4", "256,2", "512,16"]
 
 
 @pytest.mark.parametrize("pin", PINS)
