@@ -232,13 +232,12 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
             return with_regs(p.regs, [&](auto e) {
                 return launch(score_grad_warp_kernel<dt.value, e.value>, p.grid, 256, 0, 0, s, a);
             });
+        // parts of a row of at most 32768 logits, more of them where that leaves SMs idle
         uint32_t lg = 0;
-        while ((V >> lg) > 32768) ++lg;
+        while ((V >> lg) > 32768 || (((int64_t)a.N << lg) < 4 * sms && (V >> lg) > 4096)) ++lg;
         const int64_t grid = (int64_t)a.N << lg;
         if (grid > 0x7fffffff) return (int)IL_ERR_SHAPE;
-        // short rows: one round of a few warps
-        if (V <= 8192) return launch(score_grad_row_kernel<dt.value, 128>, (unsigned)grid, 128, 0, 0, s, a, lg);
-        return launch(score_grad_row_kernel<dt.value, 512>, (unsigned)grid, 512, 0, 0, s, a, lg);
+        return launch(score_grad_row_kernel<dt.value>, (unsigned)grid, kGradThreads, 0, 0, s, a, lg);
     });
 }
 
