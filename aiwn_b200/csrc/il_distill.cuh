@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(256) distill_warp_kernel(DistillArgs a) {
     int* idx = index[warp];
     float sum = 0.0f;
     for (uint32_t row = blockIdx.x * 8 + warp; row < a.N; row += gridDim.x * 8) {
-        const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : 0;
+        const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.tok.T, row)] : 0;
         const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
         T* dr = a.d.p ? reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row) : nullptr;
         float x[E];
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, sm_threads(GRAD ? 2 : 1) / kThreads)
         for (int i = tid; i < distill_bitmap(a.V, ctas, kVec, Stream::kStep) / 4; i += kThreads)
             reinterpret_cast<uint32_t*>(named)[i] = 0;
     }
-    const RowList list(a.tok, a.z.T, a.N, blockIdx.x >> lg, gridDim.x >> lg);
+    const RowList list(a.tok, a.N, blockIdx.x >> lg, gridDim.x >> lg);
     const RowStep step(a.z, gridDim.x >> lg);
     Stream stream(a.z, a.V, list, step, rank, lg, sm);
     // rows of padding
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, sm_threads(GRAD ? 2 : 1) / kThreads)
         if (tid < 64) {
             int64_t t = -1;
             if (a.hard) {
-                t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
+                t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.tok.T, row)];
                 z_t = t >= 0 && t < a.V ? to_float(zr[t]) : NAN;
             }
             if (tid == 0) index[parity][a.k] = t >= 0 && t < a.V ? (int)t : -1;
@@ -693,12 +693,12 @@ __global__ void __launch_bounds__(kThreads, sm_threads(GRAD ? 2 : 1) / kThreads)
 }
 
 // ws[0] = 1 / (rows that are not padding, at least 1), ws[1]: the ticket, 0; one CTA of 1024 threads
-__global__ void __launch_bounds__(1024) distill_begin_kernel(Tokens tok, uint32_t T, uint32_t N, float* ws) {
+__global__ void __launch_bounds__(1024) distill_begin_kernel(Tokens tok, uint32_t N, float* ws) {
     __shared__ int part[32];
     int n = 0;
     if (tok.p)
         for (uint32_t row = threadIdx.x; row < N; row += 1024)
-            n += tok.p[row_offset(tok.sb, tok.st, T, row)] != tok.ignore;
+            n += tok.p[row_offset(tok.sb, tok.st, tok.T, row)] != tok.ignore;
     n = __reduce_add_sync(0xffffffffu, n);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = n;
     __syncthreads();

@@ -26,6 +26,20 @@ constexpr double kRowCost = 32768;
 constexpr double kResident = 62e6;
 constexpr int64_t kMaxGrid = 8192;  // CTAs of a kernel that adds up a whole loss
 
+// two strides as one where that serves all rows, which saves a division a row
+void merge_strides(int64_t& sb, int64_t& st, int64_t B, int64_t& T) {
+    if (T != 1 && (B == 1 || sb == T * st)) sb = st, T = 1;
+}
+template <class R, class P>
+R rows_of(P* p, int64_t sb, int64_t st, int64_t B, int64_t T) {
+    merge_strides(sb, st, B, T);
+    return R{p, sb, st, (uint32_t)T};
+}
+Tokens tokens_of(const int64_t* p, int64_t sb, int64_t st, int64_t ignore, int64_t B, int64_t T) {
+    merge_strides(sb, st, B, T);
+    return Tokens{p, sb, st, ignore, (uint32_t)T};
+}
+
 // how a [B, T, V] operand is cut up
 struct Plan {
     int regs;     // logits a lane holds, rows of one warp; 0: CTAs
@@ -174,8 +188,8 @@ int il_token_logprobs(const void* logits, int dtype, int64_t B, int64_t T, int64
     int sms = 0;
     if ((st = host_check_device(&sms))) return st;
     ScoreArgs a{};
-    a.z = RowsIn{logits, stride_b, stride_t, (uint32_t)T};
-    a.tok = Tokens{tokens, tokens_b, tokens_t, ignore_index};
+    a.z = rows_of<RowsIn>(logits, stride_b, stride_t, B, T);
+    a.tok = tokens_of(tokens, tokens_b, tokens_t, ignore_index, B, T);
     a.N = (uint32_t)(B * T), a.V = (int)V, a.k = (int)k;
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.logprob = tokens ? logprob : nullptr, a.entropy = entropy, a.stats = reinterpret_cast<float2*>(stats);
@@ -218,9 +232,9 @@ int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, int64_t
     int sms = 0;
     if ((st = host_check_device(&sms))) return st;
     ScoreGradArgs a{};
-    a.z = RowsIn{logits, stride_b, stride_t, (uint32_t)T};
-    a.tok = Tokens{tokens, tokens_b, tokens_t, ignore_index};
-    a.d = RowsOut{dlogits, dstride_b, dstride_t, (uint32_t)T};
+    a.z = rows_of<RowsIn>(logits, stride_b, stride_t, B, T);
+    a.tok = tokens_of(tokens, tokens_b, tokens_t, ignore_index, B, T);
+    a.d = rows_of<RowsOut>(dlogits, dstride_b, dstride_t, B, T);
     a.N = (uint32_t)(B * T), a.V = (int)V, a.k = (int)k;
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature);
     a.stats = reinterpret_cast<const float2*>(stats), a.entropy = entropy, a.top_index = top_index;
@@ -266,9 +280,9 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
     cudaStream_t s = (cudaStream_t)stream;
     float* ws = reinterpret_cast<float*>(workspace);
     DistillArgs a{};
-    a.z = RowsIn{logits, stride_b, stride_t, (uint32_t)T};
-    a.tok = Tokens{targets, targets_b, targets_t, ignore_index};
-    a.d = RowsOut{dlogits, dstride_b, dstride_t, (uint32_t)T};
+    a.z = rows_of<RowsIn>(logits, stride_b, stride_t, B, T);
+    a.tok = tokens_of(targets, targets_b, targets_t, ignore_index, B, T);
+    a.d = rows_of<RowsOut>(dlogits, dstride_b, dstride_t, B, T);
     a.N = (uint32_t)N, a.V = (int)V, a.k = (int)k;
     a.index = top_index, a.logprob = top_logprob;
     a.tau = (float)temperature, a.c = (float)(kLog2e64 / temperature), a.alpha = (float)alpha;
@@ -283,7 +297,7 @@ int il_distill(const void* logits, int dtype, int64_t B, int64_t T, int64_t V, i
             else a.scale = 1.0f / (float)(N > 1 ? N : 1);
         }
         if (loss)
-            if ((st = launch(distill_begin_kernel, 1, 1024, 0, 0, s, a.tok, (uint32_t)T, a.N, ws))) return st;
+            if ((st = launch(distill_begin_kernel, 1, 1024, 0, 0, s, a.tok, a.N, ws))) return st;
     }
     const Plan p = N > 0 ? plan_rows(N, V, k, dtype, sms, dlogits ? 2 : 1, 64, [&](int t, int lg) {
         return tail ? distill_bitmap(a.V, 1 << lg, dtype == IL_BF16 ? 8 : 4, 4 * t) : 0;

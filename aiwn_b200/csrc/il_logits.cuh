@@ -44,7 +44,7 @@ constexpr int kMaxCluster = 16;
 constexpr int sm_threads(int passes) { return passes > 1 ? 512 : 768; }
 constexpr float kLog2e = 1.44269504088896341f;
 
-// rows r = b*T + t of a [B, T, V] tensor whose last dimension is contiguous
+// rows r = b*T + t of a [B, T, V] tensor whose last dimension is contiguous; T = 1 where one stride serves all rows
 struct RowsIn {
     const void* p;
     int64_t sb, st;
@@ -58,9 +58,11 @@ struct RowsOut {
 struct Tokens {  // [B, T] int64; p == nullptr: none
     const int64_t* p;
     int64_t sb, st, ignore;
+    uint32_t T;
 };
 
 __device__ __forceinline__ int64_t row_offset(int64_t sb, int64_t st, uint32_t T, uint32_t row) {
+    if (T == 1) return (int64_t)row * sb;
     const uint32_t b = row / T;
     return (int64_t)b * sb + (int64_t)(row - b * T) * st;
 }
@@ -506,10 +508,10 @@ __device__ __forceinline__ Segment segment_of(const void* row, int V, uint32_t r
 // which of 32 consecutive rows of a cluster (or CTA) are not padding: a load of a lane each
 struct RowList {
     Tokens tok;
-    uint32_t T, N, first, step, count;
+    uint32_t N, first, step, count;
 
-    __device__ __forceinline__ RowList(const Tokens& tok_, uint32_t T_, uint32_t N_, uint32_t first_, uint32_t step_)
-        : tok(tok_), T(T_), N(N_), first(first_), step(step_) {
+    __device__ __forceinline__ RowList(const Tokens& tok_, uint32_t N_, uint32_t first_, uint32_t step_)
+        : tok(tok_), N(N_), first(first_), step(step_) {
         count = first < N ? (N - first - 1) / step + 1 : 0;
     }
     __device__ __forceinline__ uint32_t row(uint32_t i) const { return first + i * step; }
@@ -517,7 +519,7 @@ struct RowList {
     __device__ __forceinline__ uint32_t window(uint32_t i) const {
         if (!tok.p) return 0xffffffffu;
         const uint32_t n = i + (threadIdx.x & 31);
-        const bool live = n < count && tok.p[row_offset(tok.sb, tok.st, T, row(n))] != tok.ignore;
+        const bool live = n < count && tok.p[row_offset(tok.sb, tok.st, tok.T, row(n))] != tok.ignore;
         return __ballot_sync(0xffffffffu, live);
     }
 };
@@ -526,12 +528,12 @@ struct RowList {
 struct LiveRows {
     const RowList& list;
     const RowStep& step;
-    uint32_t i, window;
+    uint32_t T, i, window;
     RowAt at;
 
     // whole warps
     __device__ __forceinline__ LiveRows(const RowsIn& z, const RowList& list_, const RowStep& step_)
-        : list(list_), step(step_), i(0), at(z, list_.first) {
+        : list(list_), step(step_), T(z.T), i(0), at(z, list_.first) {
         window = list.window(0);
         seek();
     }
@@ -544,7 +546,7 @@ struct LiveRows {
 
 private:
     __device__ __forceinline__ void step_on() {
-        step.move(at, list.T);
+        step.move(at, T);
         if ((++i & 31) == 0 && i < list.count) window = list.window(i);
     }
     __device__ __forceinline__ void seek() {

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(256) score_warp_kernel(ScoreArgs a) {
     const int lane = threadIdx.x & 31;
     const uint32_t warps = gridDim.x * 8;
     for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < a.N; row += warps) {
-        const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : 0;
+        const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.tok.T, row)] : 0;
         const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
         float x[E];
 #pragma unroll
@@ -110,39 +110,38 @@ __global__ void __launch_bounds__(256) score_warp_kernel(ScoreArgs a) {
         r.u = warp_sum(r.u);
         if (lane == 0) score_write(a, row, a.logprob && t >= 0 && t < a.V ? to_float(zr[t]) : NAN, r);
         if (a.k == 0) continue;
-        // k times the largest of the lanes' largest; what is not left is NaN, which no maximum takes
+        // k times the largest of the lanes' largest; keys are 0 where nothing is left
         const float log_s = logf(r.s);
-        best = NAN;
+        uint32_t key[E], most = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            x[e] = lane + 32 * e >= a.V ? NAN : fmaxf(x[e], -INFINITY);
-            best = fmaxf(best, x[e]);
+            key[e] = lane + 32 * e < a.V ? order_key(x[e]) : 0u;
+            most = max(most, key[e]);
         }
-        float my_value = 0.0f;
-        uint32_t my_index = 0;
+        uint32_t my_key = 0, my_index = 0;
         for (int i = 0; i < a.k; ++i) {
-            const float top = warp_max(best);
+            const uint32_t top = __reduce_max_sync(0xffffffffu, most);
             uint32_t mine = 0xffffffffu;
-            if (best == top) {
+            if (most == top) {
 #pragma unroll
                 for (int e = E - 1; e >= 0; --e)
-                    if (x[e] == top) mine = lane + 32 * e;
+                    if (key[e] == top) mine = lane + 32 * e;
             }
             const uint32_t index = __reduce_min_sync(0xffffffffu, mine);
-            if (lane == (i & 31)) my_value = top, my_index = index;
+            if (lane == (i & 31)) my_key = top, my_index = index;
             if ((i & 31) == 31 || i == a.k - 1) {
                 const int o = (i & ~31) + lane;
                 if (o <= i) {
                     a.top_index[(int64_t)row * a.k + o] = my_index;
-                    a.top_logprob[(int64_t)row * a.k + o] = log_prob(my_value, r.m, r.s, log_s, a.tau);
+                    a.top_logprob[(int64_t)row * a.k + o] = log_prob(key_value(my_key), r.m, r.s, log_s, a.tau);
                 }
             }
             if (mine == index) {
-                best = NAN;
+                most = 0;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    if (lane + 32 * e == index) x[e] = NAN;
-                    best = fmaxf(best, x[e]);
+                    if (lane + 32 * e == index) key[e] = 0;
+                    most = max(most, key[e]);
                 }
             }
         }
@@ -421,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, sm_threads(1) / kThreads) score_row_
     if constexpr (TOP)
         top.sh = &top_shared, top.list = reinterpret_cast<uint64_t*>(sm + Stream::kBytes), top.k = a.k,
         top.cap = top_list(a.k, lg);
-    const RowList list(a.tok, a.z.T, a.N, blockIdx.x >> lg, gridDim.x >> lg);
+    const RowList list(a.tok, a.N, blockIdx.x >> lg, gridDim.x >> lg);
     const RowStep step(a.z, gridDim.x >> lg);
     Stream stream(a.z, a.V, list, step, rank, lg, sm);
     if constexpr (TOP) {
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, sm_threads(1) / kThreads) score_row_
         const float end = tid < ends ? to_float(zr[end_at]) : -INFINITY;
         float z_t = 0.0f;
         if (tid == kThreads - 1 && a.logprob) {
-            const int64_t t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)];
+            const int64_t t = a.tok.p[row_offset(a.tok.sb, a.tok.st, a.tok.T, row)];
             z_t = t >= 0 && t < a.V ? to_float(zr[t]) : NAN;
         }
         int group_lg = 0;  // kGroups groups of 2^group_lg steps are enough
@@ -616,7 +615,7 @@ __global__ void __launch_bounds__(256) score_grad_warp_kernel(ScoreGradArgs a) {
     const uint32_t warps = gridDim.x * 8;
     for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < a.N; row += warps) {
         // everything is asked for before the first use of any of it
-        const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : -1;
+        const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.tok.T, row)] : -1;
         T* dr = reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row);
         const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
         float x[E];
@@ -647,7 +646,7 @@ __global__ void __launch_bounds__(kGradThreads, 1024 / kGradThreads) score_grad_
     constexpr int kVec = Elem<DT>::kVec;
     const int tid = threadIdx.x;
     const uint32_t row = blockIdx.x >> lg;
-    const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.z.T, row)] : -1;
+    const int64_t t = a.tok.p ? a.tok.p[row_offset(a.tok.sb, a.tok.st, a.tok.T, row)] : -1;
     const T* zr = reinterpret_cast<const T*>(a.z.p) + row_offset(a.z.sb, a.z.st, a.z.T, row);
     T* dr = reinterpret_cast<T*>(a.d.p) + row_offset(a.d.sb, a.d.st, a.d.T, row);
     const Segment g = segment_of<DT>(zr, a.V, blockIdx.x & ((1u << lg) - 1u), lg);
