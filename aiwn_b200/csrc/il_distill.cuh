@@ -168,9 +168,9 @@ struct DistillMany {
     bool huge;
     __device__ __forceinline__ explicit DistillMany(const DistillRow& r) : c(r.c) {
         b = -(r.h * c);
-        f = r.coef * fmaf(fmaf(r.h, c, b), -kLn2, 1.0f);
+        f = r.coef * exp2_approx(-fmaf(r.h, c, b));
         b1 = -(r.h1 * kLog2e);
-        f1 = r.coef1 * fmaf(fmaf(r.h1, kLog2e, b1), -kLn2, 1.0f);
+        f1 = r.coef1 * exp2_approx(-fmaf(r.h1, kLog2e, b1));
         huge = !(fabsf(b) < 4194304.0f) || (S1 && !(fabsf(b1) < 4194304.0f));
     }
     template <int n>

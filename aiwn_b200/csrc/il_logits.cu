@@ -82,7 +82,9 @@ Plan plan_rows(int64_t N, int64_t V, int64_t k, int dtype, int sms, int passes, 
     double best = 0.0;
     int threads = 0, ctas = 0;
     const char* pin = getenv("AIWN_IL_LOGITS");
-    if (pin && sscanf(pin, "%d,%d", &threads, &ctas) != 2) threads = ctas = 0;
+    if (pin && (sscanf(pin, "%d,%d", &threads, &ctas) != 2 ||
+                (threads != 64 && threads != 128 && threads != 256 && threads != 512)))
+        threads = ctas = 0;
     int lg0 = 0;  // the least that a CTA's part of a row allows
     while ((V >> lg0) > (1 << 18)) ++lg0;
     const int need = k > 64 ? 128 : 64;  // a slot, or an alternative, a thread

@@ -494,7 +494,7 @@ __device__ __forceinline__ Segment segment_of(const void* row, int V, uint32_t r
     const int nv = (V - g.h0) / kVec;
     g.t0 = g.h0 + nv * kVec;
     const bool last = rank + 1 == 1u << lg;
-    g.v0 = (int)(nv * rank >> lg);  // nv < 2^20, rank <= 16
+    g.v0 = (int)(nv * rank >> lg);  // at most 2^19 vectors, 2^9 parts
     g.v1 = (int)(nv * (rank + 1) >> lg);
     g.head = rank == 0 ? g.h0 : 0;
     g.tail = last ? V - g.t0 : 0;

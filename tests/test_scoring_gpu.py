@@ -562,6 +562,21 @@ def test_extreme_temperatures_and_logits():
         assert float(loss.detach()) == 0.0 and not leaf.grad.any()
 
 
+def test_logits_far_from_zero():
+    """A constant added to a row changes nothing, up to where it leaves the logits no digits: fp32 logits around 7e5
+    (their exponent's whole part has 20 bits) and around -3e6, beyond what is taken against a whole number."""
+    for V in (65, 5003):
+        for add in (7e5, -3e6):
+            z = make_logits(2, 4, V, torch.float32) + add
+            tokens = torch.randint(0, V, (2, 4), device=DEV)
+            r = token_logprobs(z, tokens, 9)
+            check_scores(z, tokens, 9, 1.0, r)
+            index, logprob = teacher(2, 4, V, 12)
+            for tail in (False, True):
+                check_distill(z, index, logprob, tokens, alpha=0.5, temperature=2.0, tail=tail)
+                check_distill(z, index, logprob, tokens, alpha=0.5, tail=tail)
+
+
 def test_logits_that_are_views_of_one_row():
     """Rows of stride 0: one row's logits for every position, its gradient their sum."""
     for V in (65, 5003):
