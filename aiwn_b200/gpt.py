@@ -323,6 +323,9 @@ class GraphedTrainStep:
         step = GraphedTrainStep(model, opt, batch, ctx, teacher_k=8, distill=dict(alpha=0.5, temperature=2.0))
         loss = step(x, y, top_index, top_logprob)   # [batch, ctx, 8], teacher.score(x, None, 8, temperature=2.0)'s
 
+    Construct it while no loss of the model is alive: torch cannot capture the backward of parameters that another
+    graph still refers to on the default stream, and raises.
+
     The optimizer must be capturable.  Gradients live in the graph's memory
     pool and are overwritten (not accumulated) every step.  Construction runs
     ``warmup`` eager steps (on all-zero tokens) so that the optimizer state and

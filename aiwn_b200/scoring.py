@@ -155,19 +155,19 @@ class _Distill(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, rows, index, logprob, targets, opts, lead):
-        loss, d, ws = _distill(rows, index, logprob, targets, opts, lead, opts[4] != 0)
+        loss, d, ctx.ws, ctx.args = _distill(rows, index, logprob, targets, opts, lead, opts[4] != 0)
         ctx.save_for_backward(rows, index, logprob, targets)
-        ctx.opts, ctx.d, ctx.ws = opts, d, ws
+        ctx.d = d
         return loss
 
     @staticmethod
     def _grad(ctx, g):
-        rows, index, logprob, targets = ctx.saved_tensors
+        rows = ctx.saved_tensors[0]  # raises where one of them has been changed
         d, ctx.d = ctx.d, None
         ready = d is not None
         if not ready:
             d = _gradient_like(rows)
-        _lib.run_distill(rows, index, logprob, targets, *ctx.opts, None, d, ctx.ws, g.contiguous(), int(ready))
+        _lib.run_distill_again(ctx.args, d, g.contiguous(), int(ready))
         return d, None, None, None, None, None
 
     _once = staticmethod(torch.autograd.function.once_differentiable(_grad.__func__))
@@ -185,8 +185,7 @@ def _distill(rows, index, logprob, targets, opts, lead, gradient):
     if whole:
         ws = torch.empty(_lib.distill_workspace_bytes(loss.numel()), dtype=torch.uint8, device=rows.device)
     d = _gradient_like(rows) if gradient else None
-    _lib.run_distill(rows, index, logprob, targets, *opts, loss, d, ws)
-    return loss, d, ws
+    return loss, d, ws, _lib.run_distill(rows, index, logprob, targets, *opts, loss, d, ws)
 
 
 def distill_loss(logits, top_index, top_logprob, targets=None, *, alpha: float = 1.0, temperature: float = 1.0,
