@@ -27,10 +27,10 @@
 // measured copy rate): 883 us.  The rows at work are kept to 62 MB, so that the
 // second reading finds them in the L2: 148 rows of 256 KB (a CTA of 512 threads
 // an SM) read 544 MB of 537 from HBM, 296 rows 871 MB and took 1007 us.  Rows of
-// 128 KB take 256 threads, two rows an SM (4096 x 65536: 250 us, of 165).  What is left is
+// 128 KB take 256 threads, two rows an SM (4096 x 65536: 252 us, of 165).  What is left is
 // what a row costs between its two readings (join, factors, two barriers), which
 // one or two CTAs an SM do not hide: DRAM is 64% busy, the issue slots 48%.
-// 4096 x 32768 bf16, 20 slots, the loss alone (0.27 GB): 52 us, 79%.
+// 4096 x 32768 bf16, 20 slots, the loss alone (0.27 GB): 53 us, 78%.
 #pragma once
 #include "il_logits.cuh"
 
