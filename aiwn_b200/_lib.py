@@ -535,31 +535,18 @@ def distill(logits, top_index, top_logprob, targets, ignore_index: int, alpha: f
 
 def run_distill(logits, top_index, top_logprob, targets, ignore_index, alpha, temperature, tail, reduction, loss,
                 dlogits, workspace, g=None, only_if_not_one=0):
-    """distill of operands that have been checked; reduction by its number.  Returns the call's arguments for
-    run_distill_again."""
+    """distill of operands that have been checked; reduction by its number."""
     B, T, V = logits.shape
     sb, st, _ = logits.stride()
     tb, tt = targets.stride() if targets is not None else (0, 0)
     db, dt, _ = dlogits.stride() if dlogits is not None else (0, 0, 0)
-    args = [_p(logits), _DTYPES[logits.dtype], B, T, V, sb, st, _p(top_index), _p(top_logprob), top_index.shape[2],
-            _p(targets), tb, tt, ignore_index, alpha, temperature, tail, reduction, _p(g), only_if_not_one, _p(loss),
-            _p(dlogits), db, dt, _p(workspace), 0 if workspace is None else workspace.numel(), None]
-    _run_distill(args, logits.device)
-    return args
-
-
-def run_distill_again(args, dlogits, g, only_if_not_one):
-    """The gradient alone, into dlogits and times g, of an earlier call whose operands still stand."""
-    args = list(args)
-    args[18:24] = g.data_ptr(), only_if_not_one, None, dlogits.data_ptr(), *dlogits.stride()[:2]
-    _run_distill(args, dlogits.device)
-
-
-def _run_distill(args, dev):
+    dev = logits.device
     lib = _lib or load()
     with _on_device(dev):
-        args[26] = _stream(dev)
-        rc = lib.il_distill(*args)
+        rc = lib.il_distill(_p(logits), _DTYPES[logits.dtype], B, T, V, sb, st, _p(top_index), _p(top_logprob),
+                            top_index.shape[2], _p(targets), tb, tt, ignore_index, alpha, temperature, tail, reduction,
+                            _p(g), only_if_not_one, _p(loss), _p(dlogits), db, dt, _p(workspace),
+                            0 if workspace is None else workspace.numel(), _stream(dev))
     if rc:
         _check(rc, "il_distill")
 

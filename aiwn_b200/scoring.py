@@ -97,6 +97,17 @@ def _score(rows, tokens, k, temperature, ignore_index, lead, with_stats):
     return logprob, entropy, index, top, stats
 
 
+def _saved(ctx, *whole):
+    """The tensors saved by a forward.  Hooks on saved tensors (save_on_cpu, checkpoints) return others of the same
+    values, maybe with other strides: logits of a row side by side and tensors `whole` without gaps are made sure of."""
+    t = list(ctx.saved_tensors)
+    if t[0].shape[2] > 1 and t[0].stride(2) != 1:
+        t[0] = t[0].contiguous()
+    for i in whole:
+        t[i] = t[i].contiguous()
+    return t
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, tokens, k, temperature, ignore_index, lead):
@@ -109,7 +120,7 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def _grad(ctx, g_logprob, g_entropy, _, g_top):
-        rows, tokens, entropy, stats, index = ctx.saved_tensors
+        rows, tokens, entropy, stats, index = _saved(ctx, 2, 3, 4)
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None, None, None, None
         g_logprob, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logprob, g_entropy, g_top))
@@ -155,19 +166,19 @@ class _Distill(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, rows, index, logprob, targets, opts, lead):
-        loss, d, ctx.ws, ctx.args = _distill(rows, index, logprob, targets, opts, lead, opts[4] != 0)
+        loss, d, ws = _distill(rows, index, logprob, targets, opts, lead, opts[4] != 0)
         ctx.save_for_backward(rows, index, logprob, targets)
-        ctx.d = d
+        ctx.opts, ctx.d, ctx.ws = opts, d, ws
         return loss
 
     @staticmethod
     def _grad(ctx, g):
-        rows = ctx.saved_tensors[0]  # raises where one of them has been changed
+        rows, index, logprob, targets = _saved(ctx, 1, 2)
         d, ctx.d = ctx.d, None
         ready = d is not None
         if not ready:
             d = _gradient_like(rows)
-        _lib.run_distill_again(ctx.args, d, g.contiguous(), int(ready))
+        _lib.run_distill(rows, index, logprob, targets, *ctx.opts, None, d, ctx.ws, g.contiguous(), int(ready))
         return d, None, None, None, None, None
 
     _once = staticmethod(torch.autograd.function.once_differentiable(_grad.__func__))
@@ -185,7 +196,8 @@ def _distill(rows, index, logprob, targets, opts, lead, gradient):
     if whole:
         ws = torch.empty(_lib.distill_workspace_bytes(loss.numel()), dtype=torch.uint8, device=rows.device)
     d = _gradient_like(rows) if gradient else None
-    return loss, d, ws, _lib.run_distill(rows, index, logprob, targets, *opts, loss, d, ws)
+    _lib.run_distill(rows, index, logprob, targets, *opts, loss, d, ws)
+    return loss, d, ws
 
 
 def distill_loss(logits, top_index, top_logprob, targets=None, *, alpha: float = 1.0, temperature: float = 1.0,

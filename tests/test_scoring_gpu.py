@@ -1,6 +1,7 @@
 """token_logprobs and distill_loss on the GPU against their definitions in 64
 bits: types, layouts, masks, ties, lengths on both sides of every kernel's
 range, padding, gradients, streams, graphs and repeated calls."""
+import contextlib
 import itertools
 
 import pytest
@@ -600,3 +601,34 @@ def test_logits_changed_before_the_backward_are_noticed():
         x.mul_(2.0)
         with pytest.raises(RuntimeError, match="modified by an inplace"):
             y.backward()
+
+
+@pytest.mark.parametrize("V", [65, 3001])
+def test_saved_tensors_that_hooks_replace(V):
+    """The backward reads what the hooks unpack, not the memory that the forward read."""
+    z = make_logits(2, 3, V + 7, torch.float32)[..., :V]
+    index, logprob = teacher(2, 3, V, 6)
+    targets = torch.randint(0, V, (3, 2), device=DEV).t()
+
+    def gradients(hooks=None):
+        x = z.detach().requires_grad_(True)
+        with hooks or contextlib.nullcontext():
+            y = x * 1.0
+            i, l, t = index.clone(), logprob.clone(), targets.clone()
+            a = distill_loss(y, i, l, t, alpha=0.3)
+            b = distill_loss(y, i, l, t, alpha=0.3, tail=True, reduction="none")
+            s = token_logprobs(y, t, top_k=4)
+        if hooks:  # what the forward read holds other values by now
+            for old in (y, i, l, t):
+                old.detach().data.zero_()
+        return torch.autograd.grad(2.0 * a + b.sum() + s.logprob.sum() + s.entropy.sum() + s.top_logprob.sum(), x)[0]
+
+    def strided(t):  # the same values, those of the last dimension apart
+        t = t.detach()
+        return t if t.dim() == 0 else torch.stack([t, t], -1)[..., 0]
+
+    plain = gradients()
+    for hooks in (torch.autograd.graph.save_on_cpu(),
+                  torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t),
+                  torch.autograd.graph.saved_tensors_hooks(strided, lambda t: t)):
+        assert torch.equal(gradients(hooks), plain)
