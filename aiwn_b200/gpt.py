@@ -378,8 +378,11 @@ class GraphedTrainStep:
         return self.model.distill(self.x, self.top_index, self.top_logprob, self.y, **self.distill)[1]
 
     def __call__(self, x, y, top_index=None, top_logprob=None):
-        if (top_index is None or top_logprob is None) != (self.top_index is None):
-            raise ValueError("a step with teacher_k takes top_index and top_logprob, one without takes neither")
+        for mine, t in ((self.top_index, top_index), (self.top_logprob, top_logprob)):
+            if (t is None) != (mine is None):
+                raise ValueError("a step with teacher_k takes top_index and top_logprob, one without takes neither")
+            if t is not None and t.shape != mine.shape:  # copy_ would repeat a single alternative
+                raise ValueError(f"teacher's alternatives of shape {tuple(t.shape)}, expected {tuple(mine.shape)}")
         self.x.copy_(x, non_blocking=True)
         self.y.copy_(y, non_blocking=True)
         if self.top_index is not None:

@@ -106,3 +106,18 @@ def test_graphed_step_refuses_options_without_teacher():
     opt = torch.optim.AdamW(m.parameters())
     with pytest.raises(ValueError):
         GraphedTrainStep(m, opt, 2, 24, distill=dict(alpha=0.5))
+
+
+def test_graphed_step_refuses_other_alternatives():
+    """Before anything is copied or replayed: alternatives that are missing, not asked for or of another number."""
+    index, logprob = torch.zeros(2, 24, 6, dtype=torch.long), torch.zeros(2, 24, 6)
+    step = GraphedTrainStep.__new__(GraphedTrainStep)
+    step.top_index, step.top_logprob = index, logprob
+    for given in ((None, None), (index, None), (None, logprob), (index[..., :1], logprob[..., :1]),
+                  (index[:1], logprob[:1]), (index, logprob[..., :1])):
+        with pytest.raises(ValueError):
+            step(index[..., 0], index[..., 0], *given)
+    step.top_index = step.top_logprob = None
+    for given in ((index, logprob), (index, None), (None, logprob)):
+        with pytest.raises(ValueError):
+            step(index[..., 0], index[..., 0], *given)
