@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, sm_threads(GRAD ? 2 : 1) / kThreads)
             if (tid == 0) index[parity][a.k] = t >= 0 && t < a.V ? (int)t : -1;
         }
         Running<false, S1> run;
-        run.begin();
+        run.begin(a.c);
         auto use = [&](uint4 (&raw)[kU], int v) {  // v: of the first vector
             if constexpr (TAIL) {
                 const uint8_t* byte = named + (v - g.v0);

@@ -53,7 +53,7 @@ int check_rows(int dtype, int64_t B, int64_t T, int64_t V, double temperature) {
     if (B < 0 || T < 0 || V < 1 || V > kMaxVocab) return IL_ERR_SHAPE;
     if (B > 0 && T > (int64_t(1) << 30) / B) return IL_ERR_SHAPE;
     const float tau = (float)temperature;
-    if (!(tau > 0.0f) || isinf(tau) || isinf(1.0f / tau)) return IL_ERR_VALUE;
+    if (!(tau > 0.0f) || isinf(tau) || isinf((float)(kLog2e64 / temperature))) return IL_ERR_VALUE;
     return IL_OK;
 }
 

@@ -330,24 +330,26 @@ __device__ __noinline__ Sums huge_vector(uint4 r, float m, float c) {
 // m log2(e) / tau: d = z c - H is one fused multiply-add, rounded once, and a new maximum
 // rescales by a power of two, without rounding.  Where |m| c is 2^22 or more (a row of nothing
 // but a mask's huge negative values) such an H has no meaning, and d = (z - m) c; so it is where
-// c is so small (a temperature above 10^20) that floor16's -2^100 would count for something.
-constexpr float kLeastFactor = 1e-20f;
+// c is so small (a temperature above 10^20) that floor16's -2^100 would count for something, or so large (one below
+// 10^-8) that its exponent would not be finite.
+constexpr float kLeastFactor = 1e-20f, kMostFactor = 1e8f;
 
 template <bool U, bool S1>
 struct Running {
     float m, s, u, s1, h, h1;  // h, h1: -H for c and for log2(e)
     bool huge;
 
-    __device__ __forceinline__ void begin() {
+    __device__ __forceinline__ void begin(float c) {
         m = -INFINITY;
         s = u = s1 = h = h1 = 0.0f;
-        huge = false;
+        huge = beyond(c);  // for what comes before the first value above -inf, too
     }
+    __device__ __forceinline__ static bool beyond(float c) { return U && (c < kLeastFactor || c > kMostFactor); }
     __device__ __forceinline__ static bool is_huge(float t) { return !(fabsf(t) < 4194304.0f); }
 
     __device__ __forceinline__ void raise(float top, float c) {
         const float t = top * c;
-        const bool now = is_huge(t) || (S1 && is_huge(top * kLog2e)) || (U && c < kLeastFactor);
+        const bool now = is_huge(t) || (S1 && is_huge(top * kLog2e)) || beyond(c);
         const float g = now ? -t : -rintf(t), g1 = now ? -top * kLog2e : -rintf(top * kLog2e);
         if (m != -INFINITY) {
             const float d = fmaxf(now && huge ? (m - top) * c : g - h, kMinExp), f = exp2_approx(d);
@@ -367,7 +369,7 @@ struct Running {
         if (huge) {
 #pragma unroll
             for (int q = 0; q < kU; ++q) {
-                const Sums x = huge_vector<DT, U, S1>(r[q], m, c);
+                const Sums x = huge_vector<DT, U, S1>(r[q], shift_of(m), c);
                 s += x.s, u += x.u, s1 += x.s1;
             }
         } else {

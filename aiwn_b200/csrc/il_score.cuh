@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, sm_threads(1) / kThreads) score_row_
         if constexpr (TOP)
             while ((Stream::kStep * TopOf::kGroups << group_lg) < g.v1 - g.v0) ++group_lg;
         Running<true, false> run;
-        run.begin();
+        run.begin(a.c);
         float most = -INFINITY;
         int n = 0;
         auto use = [&](const uint4 (&raw)[kU], bool last) {

@@ -112,3 +112,10 @@ def test_c_entry_points_check_their_arguments():
     assert distill(w=None) == 5 and distill(n=ws - 1) == 5
     assert distill(z=odd) == 3 and distill(d=odd) == 3 and distill(w=ctypes.c_void_p(72)) == 3
     assert distill(b=0, red=0) == 0
+
+
+def test_temperature_whose_reciprocal_overflows_is_refused():
+    """1 / tau is finite in fp32 and log2(e) / tau is not."""
+    lib, p = _lib.load(), ctypes.c_void_p(64)
+    for tau in (3e-39, 4.2e-39):
+        assert lib.il_token_logprobs(p, 0, 2, 3, 40, 120, 40, p, 3, 1, -100, 4, tau, p, p, p, p, p, None) == 9

@@ -632,3 +632,22 @@ def test_saved_tensors_that_hooks_replace(V):
                   torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t),
                   torch.autograd.graph.saved_tensors_hooks(strided, lambda t: t)):
         assert torch.equal(gradients(hooks), plain)
+
+
+@pytest.mark.parametrize("V", [65, 1500, 5003])
+def test_scores_of_masked_rows_at_extreme_temperatures(V):
+    """Rows whose largest logit is 0 and whose mask is -inf, or about the type's lowest value: at small temperatures
+    the masked logits' exponents overflow, at large ones only those of -inf do."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for tau in (2.0 ** -120, 2.0 ** -60, 2.0 ** -28, 2.0 ** -20, 2.0 ** 66, 2.0 ** 70, 2.0 ** 100, 2.0 ** 126):
+            for low in (float("-inf"), LOWEST):
+                z = make_logits(2, 3, V, dtype)
+                z -= z.amax(-1, keepdim=True)
+                z[..., 3::2] = low
+                z[..., 0], z[..., 1] = 0.0, -tau  # two that count
+                tokens = torch.zeros(2, 3, dtype=torch.int64, device=DEV)
+                r = token_logprobs(z, tokens, 4, temperature=tau)
+                lp, h, index, _ = scores64(z, tokens, 4, tau)
+                near(r.logprob, lp, sum_tol(V) + 8 * F32 * 12, "logprob")
+                near(r.entropy, h, 4 * sum_tol(V) * (1 + 2 * h) + 8 * F32 * 12, "entropy")
+                assert torch.equal(r.top_index, index)
