@@ -651,3 +651,22 @@ def test_scores_of_masked_rows_at_extreme_temperatures(V):
                 near(r.logprob, lp, sum_tol(V) + 8 * F32 * 12, "logprob")
                 near(r.entropy, h, 4 * sum_tol(V) * (1 + 2 * h) + 8 * F32 * 12, "entropy")
                 assert torch.equal(r.top_index, index)
+
+
+@pytest.mark.parametrize("V", [65, 1500, 5003])
+def test_distill_of_masked_rows_at_extreme_temperatures(V):
+    """The same rows; the slots are the two tokens that count at every temperature, and an empty one."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for tau in (2.0 ** -60, 2.0 ** -28, 2.0 ** -20, 2.0 ** 20, 2.0 ** 60):
+            for low in (float("-inf"), LOWEST):
+                z = make_logits(2, 3, V, dtype)
+                z -= z.amax(-1, keepdim=True)
+                z[..., 3::2] = low
+                z[..., 0], z[..., 1] = 0.0, -min(tau, 1.0)
+                index = torch.tensor([1, -1, 0], device=DEV).expand(2, 3, 3)
+                logprob = torch.tensor([0.6, 0.5, 0.3], device=DEV).log().expand(2, 3, 3)
+                check_distill(z, index, logprob, None, temperature=tau)
+                check_distill(z, index, logprob, torch.zeros(2, 3, dtype=torch.int64, device=DEV), alpha=0.5,
+                              temperature=tau)
+                if tau > 1.0:
+                    check_distill(z, index, logprob, None, temperature=tau, tail=True)
