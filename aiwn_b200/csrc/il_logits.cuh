@@ -336,7 +336,7 @@ constexpr float kLeastFactor = 1e-20f, kMostFactor = 1e8f;
 
 template <bool U, bool S1>
 struct Running {
-    float m, s, u, s1, h, h1;  // h, h1: -H for c and for log2(e)
+    float m, s, u, s1, h, h1;  // h, h1: -H for c and for log2(e), 0 where huge
     bool huge;
 
     __device__ __forceinline__ void begin(float c) {
@@ -347,15 +347,18 @@ struct Running {
     __device__ __forceinline__ static bool beyond(float c) { return U && (c < kLeastFactor || c > kMostFactor); }
     __device__ __forceinline__ static bool is_huge(float t) { return !(fabsf(t) < 4194304.0f); }
 
+    // The sums are next to m c, or (huge: h = h1 = 0) at m itself; the factor between any two of these forms has its
+    // exponent rounded once: a product m c is rounded alone nowhere, beyond 2^22 that is by a quarter and more.
     __device__ __forceinline__ void raise(float top, float c) {
         const float t = top * c;
         const bool now = is_huge(t) || (S1 && is_huge(top * kLog2e)) || beyond(c);
-        const float g = now ? -t : -rintf(t), g1 = now ? -top * kLog2e : -rintf(top * kLog2e);
+        const float g = now ? 0.0f : -rintf(t), g1 = now ? 0.0f : -rintf(top * kLog2e);
         if (m != -INFINITY) {
-            const float d = fmaxf(now && huge ? (m - top) * c : g - h, kMinExp), f = exp2_approx(d);
+            const float step = (huge ? m : 0.0f) - (now ? top : 0.0f);
+            const float d = fmaxf(fmaf(step, c, g - h), kMinExp), f = exp2_approx(d);
             if constexpr (U) u = f * (u + s * d);
             s *= f;
-            if constexpr (S1) s1 *= exp2_approx(fmaxf(now && huge ? (m - top) * kLog2e : g1 - h1, kMinExp));
+            if constexpr (S1) s1 *= exp2_approx(fmaxf(fmaf(step, kLog2e, g1 - h1), kMinExp));
         }
         m = top, h = g, h1 = g1, huge = now;
     }
