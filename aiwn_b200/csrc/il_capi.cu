@@ -356,6 +356,20 @@ namespace il {
 int host_check_device(int* num_sms) { return check_device(num_sms); }
 int host_launch_status(int kernels) { return launch_status(kernels); }
 
+int host_allow_shared(const void* kern, size_t smem) {
+    constexpr int kDefault = 48 * 1024, kMost = 227 * 1024;  // of a CTA, static arrays included
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, kern);
+    if (e == cudaSuccess && smem + at.sharedSizeBytes > kDefault) {
+        const int most = kMost - (int)at.sharedSizeBytes;
+        if (at.maxDynamicSharedSizeBytes < most)
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    }
+    if (e == cudaSuccess) return IL_OK;
+    cudaGetLastError();
+    return IL_ERR_LAUNCH;
+}
+
 }  // namespace il
 
 extern "C" {

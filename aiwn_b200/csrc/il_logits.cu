@@ -119,11 +119,8 @@ Plan plan_rows(int64_t N, int64_t V, int64_t k, int dtype, int sms, int passes, 
 
 template <class... P, class... A>
 int launch(void (*kern)(P...), unsigned grid, int threads, uint32_t lg, size_t smem, cudaStream_t s, A... args) {
-    if (smem > 16 * 1024 &&  // beyond 48 KB with the static arrays
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-        cudaGetLastError();
-        return IL_ERR_LAUNCH;
-    }
+    if (smem > 16 * 1024)  // beyond 48 KB with the static arrays
+        if (const int st = host_allow_shared((const void*)kern, smem)) return st;
     if (lg > 3 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         cudaGetLastError();
         return IL_ERR_LAUNCH;
