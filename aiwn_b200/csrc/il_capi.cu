@@ -260,9 +260,8 @@ uint32_t attn_threshold(double p) {
 
 template <typename Kern, typename... Args>
 int attn_launch(Kern kern, int64_t smem, int64_t B, int64_t T, int64_t H, cudaStream_t s, Args... args) {
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-                                cudaSuccess)
-        return IL_ERR_LAUNCH;
+    if (smem > 48 * 1024)
+        if (const int st = il::host_allow_shared((const void*)kern, (size_t)smem)) return st;
     kern<<<dim3((unsigned)H, (unsigned)B, 1), (unsigned)T, (size_t)smem, s>>>(args...);
     return launch_status();
 }
@@ -504,10 +503,8 @@ int il_cdf_backward(const float* gxn, const float* x, const float* gamma, const 
         return launch_status();
     }
     const size_t smem = (size_t)(2 * IN) * sizeof(float);
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(il::cdf_backward_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-            cudaSuccess)
-        return IL_ERR_LAUNCH;
+    if (smem > 48 * 1024)
+        if (const int st = il::host_allow_shared((const void*)il::cdf_backward_kernel, smem)) return st;
     const unsigned blocks = (unsigned)((N + il::kCdfRowThreads - 1) / il::kCdfRowThreads);
     il::cdf_backward_kernel<<<blocks, il::kCdfRowThreads, smem, s>>>(gxn, x, gamma, beta, mean, rstd, dx, dgamma,
                                                                       dbeta, (int)N, (int)IN);
@@ -756,9 +753,8 @@ int il_bin_counts(const void* x, int x_dtype, int64_t N, int64_t IN, int64_t K, 
     auto* cnt = reinterpret_cast<unsigned long long*>(counts);
     // K > 12288 counters need more than the default 48 KB of dynamic shared memory
     auto run = [&](auto kern) -> int {
-        if (smem > 48 * 1024 &&
-            cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-            return IL_ERR_LAUNCH;
+        if (smem > 48 * 1024)
+            if (const int st = il::host_allow_shared((const void*)kern, smem)) return st;
         kern<<<g, 256, smem, s>>>(x, N * IN, c, cnt);
         return launch_status();
     };

@@ -437,8 +437,7 @@ inline int launch_token_cdf(const CUtensorMap& map, const FwdArgs& a, const CdfA
     // slices + base alignment + mbarriers + gamma, beta
     const int smem = a.IN * pl.slice_bytes + 128 + 8 * ceil_div(a.IN, kTokXB) + 2 * kCdfMaxIn * 4;
     if (smem > kSmemBudget) return kNotApplicable;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return 4;
+    if (host_allow_shared((const void*)kern, smem)) return 4;
     const int jranges = ceil_div(a.OUT, pl.JR);
     const int max_ranges = std::max(1, sms / jranges);
     const int per = std::max(32, round_up(ceil_div(a.N, max_ranges), 32));

@@ -29,6 +29,7 @@
 #include <numeric>
 
 #include "il_common.cuh"
+#include "il_host.h"
 #include "il_sm100.cuh"
 #include "il_dtable.cuh"
 
@@ -504,8 +505,7 @@ template <int DT, int C, int CS>
 inline int launch_fwd(const CUtensorMap& map, const FwdArgs& a, const FwdPlan& pl, int num_sms,
                       cudaStream_t s) {
     auto kern = fwd_cluster_kernel<DT, C, CS>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess)
-        return 4;
+    if (host_allow_shared((const void*)kern, pl.smem)) return 4;
     if (CS > 1 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 0) != cudaSuccess)
         return 4;
     const int jranges = ceil_div(a.OUT, pl.JR);
@@ -927,8 +927,7 @@ template <int DT, int C>
 inline int launch_bwd(const CUtensorMap& map, const BwdArgs& a, const BwdPlan& pl, int sms,
                       cudaStream_t s) {
     auto kern = bwd_fused_kernel<DT, C>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess)
-        return 4;
+    if (host_allow_shared((const void*)kern, pl.smem)) return 4;
     const int per = std::max(1, sms / pl.ngroups);
     dim3 grid((unsigned)std::min(per, a.ntiles), (unsigned)pl.ngroups, 1);
     kern<<<grid, kBwdThreads, pl.smem, s>>>(map, a);
@@ -991,8 +990,7 @@ inline bool plan_dtable(int N, int K, int IN, int OUT, int sms, DtPlan& pl) {
 template <int DT, int C>
 inline int launch_dtable(const DtArgs& a, const DtPlan& pl, cudaStream_t s) {
     auto kern = dtable_kernel<DT, C>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess)
-        return 4;
+    if (host_allow_shared((const void*)kern, pl.smem)) return 4;
     kern<<<dim3((unsigned)pl.R, (unsigned)a.IN, 1), kDtThreads, pl.smem, s>>>(a);
     return 0;
 }

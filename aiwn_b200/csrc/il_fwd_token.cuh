@@ -215,8 +215,7 @@ template <int DT, int C>
 inline int launch_token_fwd(const CUtensorMap& map, const FwdArgs& a, const FwdPlan& pl, int sms,
                             cudaStream_t s) {
     auto kern = a.counts ? fwd_token_kernel<DT, C, true> : fwd_token_kernel<DT, C, false>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess)
-        return 4;
+    if (host_allow_shared((const void*)kern, pl.smem)) return 4;
     const int jranges = ceil_div(a.OUT, pl.JR);
     const int T = tok_threads(C);
     // contiguous token ranges, one per CTA, a multiple of 32 tokens each
@@ -414,8 +413,7 @@ inline bool plan_stream_forward(int K, int IN, int OUT, StrPlan& pl) {
 template <int DT, int C>
 inline int launch_stream_fwd(const CUtensorMap& map, const StrArgs& a, const StrPlan& pl, cudaStream_t s) {
     auto kern = fwd_stream_kernel<DT, C>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess)
-        return 4;
+    if (host_allow_shared((const void*)kern, pl.smem)) return 4;
     kern<<<dim3((unsigned)ceil_div(a.N, kStrThreads), (unsigned)(a.OUT / pl.JR), 1), kStrThreads, pl.smem, s>>>(map,
                                                                                                              a);
     return 0;

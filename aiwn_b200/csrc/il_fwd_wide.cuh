@@ -223,7 +223,7 @@ inline bool plan_wide_forward(int64_t N, int K, int IN, int OUT, int sms, WidePl
 template <int DT, int CB, int JW>
 inline int launch_wide_fwd(const CUtensorMap& map, const WideArgs& a, const WidePlan& pl, cudaStream_t s) {
     auto kern = fwd_wide_kernel<DT, CB, JW>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess) return 4;
+    if (host_allow_shared((const void*)kern, pl.smem)) return 4;
     const dim3 grid((unsigned)ceil_div(a.N, wide_mw(JW) * pl.warps), (unsigned)(a.OUT / JW), 1);
     kern<<<grid, 32 * (pl.warps + 1), pl.smem, s>>>(map, a);
     return 0;

@@ -486,8 +486,7 @@ inline bool plan_sorted(int64_t N, int K, int IN, int OUT, int sms, int G, SrtPl
 template <int DT, int C>
 inline int launch_sorted(const CUtensorMap& map, const SrtArgs& a, const SrtPlan& pl, cudaStream_t s) {
     auto kern = pl.G == kSrtG ? bwd_sorted_kernel<DT, C, kSrtG> : bwd_sorted_kernel<DT, C, 1>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem) != cudaSuccess)
-        return 4;
+    if (host_allow_shared((const void*)kern, pl.smem)) return 4;
     kern<<<dim3((unsigned)pl.R, (unsigned)(a.IN / pl.G), (unsigned)pl.jranges), kSrtThreads, pl.smem, s>>>(map, a);
     return 0;
 }

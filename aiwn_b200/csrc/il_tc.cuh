@@ -395,7 +395,7 @@ inline int tc_forward(const void* x, int x_dtype, const float* table, const floa
     CUtensorMap map;
     if (!make_table_map(&map, table, c.K, (int)IN, (int)OUT, (int)OUT, std::min(c.K, kTcKC))) return kNotApplicable;
     auto kern = x_dtype == kBF16 ? fwd_tc_kernel<kBF16> : fwd_tc_kernel<kF32>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 4;
+    if (host_allow_shared((const void*)kern, smem)) return 4;
     const unsigned grid = (unsigned)((N + kTcM - 1) / kTcM);
     kern<<<grid, kTcThreads + 32, smem, s>>>(map, a);
     return 0;

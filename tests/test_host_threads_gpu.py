@@ -84,3 +84,47 @@ def test_distill_of_two_vocabularies(monkeypatch):
 def test_scores_of_two_numbers_of_alternatives(monkeypatch):
     monkeypatch.setenv("AIWN_IL_LOGITS", "256,8")
     _check(_scores(50021, 128), _scores(50021, 8), _scores(9001, 100), _scores(9001, 3))
+
+
+def _counts(K):
+    def make():
+        lib, s = _lib.load(), torch.cuda.current_stream().cuda_stream
+        x = torch.rand(64, 8, device=DEV) * 2 - 1
+        counts = torch.zeros(K, dtype=torch.int64, device=DEV)
+        args = (x.data_ptr(), 0, 64, 8, K, 2.0 / K, counts.data_ptr(), s)
+        return lambda keep=(x, counts): lib.il_bin_counts(*args), []  # the counts add up
+    return make
+
+
+def _forward(K, IN=20, OUT=20, N=256):
+    def make():
+        lib, s = _lib.load(), torch.cuda.current_stream().cuda_stream
+        x, table = torch.rand(N, IN, device=DEV) * 2 - 1, torch.randn(K, IN, OUT, device=DEV)
+        bias, out = torch.zeros(OUT, device=DEV), torch.zeros(N, OUT, device=DEV)
+        args = (x.data_ptr(), 0, table.data_ptr(), bias.data_ptr(), out.data_ptr(), N, IN, OUT, K, 2.0 / K, s)
+        return lambda keep=(x, table, bias): lib.il_forward(*args), [out]
+    return make
+
+
+def _attention(T, D=8):
+    def make():
+        lib, s = _lib.load(), torch.cuda.current_stream().cuda_stream
+        q, k, v = (torch.randn(1, T, D, device=DEV) for _ in range(3))
+        o, lse = torch.zeros(1, T, D, device=DEV), torch.zeros(1, 1, T, device=DEV)
+        args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 1, T, 1, D, 0.5, 0.0, None, s)
+        return lambda keep=(q, k, v): lib.il_attention_forward(*args), [o, lse]
+    return make
+
+
+def test_bin_counts_of_several_sizes():
+    _check(_counts(13000), _counts(16384), _counts(14000), _counts(15000))
+
+
+@pytest.mark.parametrize("family", ["token", "cluster"])
+def test_layers_of_several_sizes(family, monkeypatch):
+    monkeypatch.setenv("AIWN_IL_FORWARD", family)
+    _check(_forward(512), _forward(64), _forward(256), _forward(16))
+
+
+def test_attention_of_several_lengths():
+    _check(_attention(1024), _attention(800), _attention(900), _attention(820))
