@@ -13,7 +13,8 @@ cross-entropy (transformer_validation.py:365-370).  ``IndexedGPT.score`` and
 Both take fp32 or bf16 CUDA logits [..., V].  Up to two leading dimensions
 may have any strides (the shifted view ``logits[:, :-1]`` or a head padded to
 a round width, ``logits[..., :V]``, are read in place); more are flattened.
-The sums are held in 32 bits whatever the logits' type.
+The sums are held in 32 bits whatever the logits' type.  Gradients are those of
+reverse mode; logits with a forward-mode tangent are refused.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from ._lib import ILError
@@ -40,6 +42,8 @@ def _rows(logits):
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ILError(f"logits must be [..., V] with V >= 1, got shape {tuple(logits.shape)}")
     _lib.x_dtype_code(logits)
+    if unpack_dual(logits).tangent is not None:
+        raise ILError("logits have a forward-mode tangent: these operators have gradients in reverse mode only")
     V = logits.shape[-1]
     if V > _lib.MAX_VOCAB:
         raise ILError(f"logits: {V} logits a row, at most {_lib.MAX_VOCAB}")
