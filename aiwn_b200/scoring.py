@@ -53,11 +53,11 @@ def _rows(logits):
     return logits if d == 3 else logits[None] if d == 2 else logits[None, None] if d == 1 else logits.reshape(1, -1, V)
 
 
-def _per_row(name, t, lead, rows, dtype):
-    """t [*lead, ...] as [B, T, ...] like the rows."""
+def _per_row(name, t, lead, rows, dtype, more=0):
+    """t, of the leading dimensions `lead` and `more` others, as [B, T, ...] like the rows."""
     if t.dtype != dtype:
         raise ILError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if t.shape[:len(lead)] != lead:
+    if t.dim() != len(lead) + more or t.shape[:len(lead)] != lead:
         raise ILError(f"{name}: shape {tuple(t.shape)} for logits over {tuple(lead)}")
     if t.device != rows.device:
         raise ILError(f"tensors on different devices: {name} on {t.device}, the logits on {rows.device}")
@@ -232,8 +232,8 @@ def distill_loss(logits, top_index, top_logprob, targets=None, *, alpha: float =
         raise ILError(f"top_index must be [..., k] with k <= {_lib.MAX_TOP}, got shape {tuple(top_index.shape)}")
     if top_logprob.shape != top_index.shape:
         raise ILError(f"top_logprob: shape {tuple(top_logprob.shape)}, expected {tuple(top_index.shape)}")
-    index = _per_row("top_index", top_index, lead, rows, torch.int64).contiguous()
-    logprob = _per_row("top_logprob", top_logprob, lead, rows, torch.float32).detach().contiguous()
+    index = _per_row("top_index", top_index, lead, rows, torch.int64, 1).contiguous()
+    logprob = _per_row("top_logprob", top_logprob, lead, rows, torch.float32, 1).detach().contiguous()
     tgt = None if targets is None else _per_row("targets", targets, lead, rows, torch.int64)
     opts = (int(ignore_index), alpha, _temperature(temperature), int(bool(tail)), _lib.REDUCTIONS[reduction])
     _need_cuda(rows)

@@ -25,3 +25,19 @@ def test_forward_mode_is_refused():
                     distill_loss(logits, torch.zeros(*lead, K, dtype=torch.long), torch.zeros(*lead, K))
             with pytest.raises(ILError, match="CUDA"):  # no tangent: the next check
                 token_logprobs(torch.randn(B, T, V), None)
+
+
+def test_tensors_of_more_dimensions_than_the_rows_are_refused():
+    z, tokens = torch.randn(B, T, V), torch.zeros(B, T, dtype=torch.long)
+    index, logprob = torch.zeros(B, T, K, dtype=torch.long), torch.zeros(B, T, K)
+    for logits, t in ((z, tokens[..., None]), (z, tokens[..., None].expand(B, T, 2)), (z[0], tokens[0][:, None]),
+                      (z[0, 0], tokens[0, :1]), (z[None], tokens[None, ..., None])):
+        with pytest.raises(ILError, match="shape"):
+            token_logprobs(logits, t)
+        lead = logits.shape[:-1]
+        with pytest.raises(ILError, match="shape"):
+            distill_loss(logits, torch.zeros(*lead, K, dtype=torch.long), torch.zeros(*lead, K), t)
+    with pytest.raises(ILError, match="shape"):
+        distill_loss(z, index[0], logprob[0])
+    with pytest.raises(ILError, match="shape"):
+        distill_loss(z[0], index, logprob)
