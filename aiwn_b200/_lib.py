@@ -529,11 +529,11 @@ def distill(logits, top_index, top_logprob, targets, ignore_index: int, alpha: f
         raise ILError("workspace must be a uint8 tensor")
     _on_cuda(logits, targets, dlogits)
     _need_cuda(top_index, top_logprob, loss, workspace, g)
-    run_distill(logits, top_index, top_logprob, targets, ignore_index, alpha, temperature, int(bool(tail)),
+    run_distill(logits, top_index, top_logprob, k, targets, ignore_index, alpha, temperature, int(bool(tail)),
                 REDUCTIONS[reduction], loss, dlogits, workspace, g, int(bool(only_if_not_one)))
 
 
-def run_distill(logits, top_index, top_logprob, targets, ignore_index, alpha, temperature, tail, reduction, loss,
+def run_distill(logits, top_index, top_logprob, k, targets, ignore_index, alpha, temperature, tail, reduction, loss,
                 dlogits, workspace, g=None, only_if_not_one=0):
     """distill of operands that have been checked; reduction by its number."""
     B, T, V = logits.shape
@@ -544,7 +544,7 @@ def run_distill(logits, top_index, top_logprob, targets, ignore_index, alpha, te
     lib = _lib or load()
     with _on_device(dev):
         rc = lib.il_distill(_p(logits), _DTYPES[logits.dtype], B, T, V, sb, st, _p(top_index), _p(top_logprob),
-                            top_index.shape[2], _p(targets), tb, tt, ignore_index, alpha, temperature, tail, reduction,
+                            k, _p(targets), tb, tt, ignore_index, alpha, temperature, tail, reduction,
                             _p(g), only_if_not_one, _p(loss), _p(dlogits), db, dt, _p(workspace),
                             0 if workspace is None else workspace.numel(), _stream(dev))
     if rc:

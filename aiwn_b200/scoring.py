@@ -22,7 +22,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ILError
@@ -42,7 +42,7 @@ def _rows(logits):
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ILError(f"logits must be [..., V] with V >= 1, got shape {tuple(logits.shape)}")
     _lib.x_dtype_code(logits)
-    if unpack_dual(logits).tangent is not None:
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(logits).tangent is not None:
         raise ILError("logits have a forward-mode tangent: these operators have gradients in reverse mode only")
     V = logits.shape[-1]
     if V > _lib.MAX_VOCAB:
@@ -101,15 +101,26 @@ def _score(rows, tokens, k, temperature, ignore_index, lead, with_stats):
     return logprob, entropy, index, top, stats
 
 
-def _saved(ctx, *whole):
-    """The tensors saved by a forward.  Hooks on saved tensors (save_on_cpu, checkpoints) return others of the same
-    values, maybe with other strides: logits of a row side by side and tensors `whole` without gaps are made sure of."""
-    t = list(ctx.saved_tensors)
-    if t[0].shape[2] > 1 and t[0].stride(2) != 1:
-        t[0] = t[0].contiguous()
-    for i in whole:
-        t[i] = t[i].contiguous()
-    return t
+# Hooks on saved tensors (save_on_cpu, checkpoints) return others of the same values, maybe with other strides: the
+# backward passes make sure of logits of a row side by side and of the rest without gaps.  Others than that, on another
+# device, of another type or size, are refused, for the kernels go by the forward's sizes.  Written out, as every
+# backward pass comes here: 0.9 us, in a loop over the tensors 2.7 us.
+def _like(rows):
+    """Of the forward's logits, for `_saved_rows`."""
+    return rows.shape, rows.dtype, rows.get_device()
+
+
+def _replaced():
+    return ILError("a hook has replaced a saved tensor by one of another device, type or shape")
+
+
+def _saved_rows(rows, tokens, like):
+    """The logits that a forward saved (tokens: checked too), the number of rows and their device's index."""
+    shape, dtype, dev = like
+    if rows.shape != shape or rows.dtype is not dtype or rows.get_device() != dev or tokens is not None and (
+            tokens.shape != shape[:2] or tokens.dtype is not torch.int64 or tokens.get_device() != dev):
+        raise _replaced()
+    return rows if shape[2] == 1 or rows.stride()[2] == 1 else rows.contiguous(), shape[0] * shape[1], dev
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -117,18 +128,24 @@ class _TokenLogprobs(torch.autograd.Function):
     def forward(ctx, rows, tokens, k, temperature, ignore_index, lead):
         logprob, entropy, index, top, stats = _score(rows, tokens, k, temperature, ignore_index, lead, True)
         ctx.save_for_backward(rows, tokens, entropy, stats, index)
-        ctx.opts = k, temperature, ignore_index
+        ctx.opts, ctx.like = (k, temperature, ignore_index), _like(rows)
         ctx.mark_non_differentiable(index)
         ctx.set_materialize_grads(False)
         return logprob, entropy, index, top
 
     @staticmethod
     def _grad(ctx, g_logprob, g_entropy, _, g_top):
-        rows, tokens, entropy, stats, index = _saved(ctx, 2, 3, 4)
+        k, temperature, ignore_index = ctx.opts
+        rows, tokens, entropy, stats, index = ctx.saved_tensors
+        rows, n, dev = _saved_rows(rows, tokens, ctx.like)
+        if (entropy.dtype is not torch.float32 or entropy.numel() != n or entropy.get_device() != dev
+                or stats.dtype is not torch.float32 or stats.numel() != 2 * n or stats.get_device() != dev
+                or index.dtype is not torch.int64 or index.numel() != k * n or index.get_device() != dev):
+            raise _replaced()
+        entropy, stats, index = entropy.contiguous(), stats.contiguous(), index.contiguous()
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None, None, None, None
         g_logprob, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logprob, g_entropy, g_top))
-        k, temperature, ignore_index = ctx.opts
         d = _gradient_like(rows)
         _lib.run_token_logprobs_backward(rows, tokens, ignore_index, temperature, k, entropy, stats, index, g_logprob,
                                          g_entropy, g_top, d)
@@ -171,18 +188,24 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, index, logprob, targets, opts, lead):
         loss, d, ws = _distill(rows, index, logprob, targets, opts, lead, opts[4] != 0)
-        ctx.save_for_backward(rows, index, logprob, targets)
-        ctx.opts, ctx.d, ctx.ws = opts, d, ws
+        ctx.save_for_backward(rows, targets, index, logprob)
+        ctx.opts, ctx.d, ctx.ws, ctx.like, ctx.k = opts, d, ws, _like(rows), index.shape[2]
         return loss
 
     @staticmethod
     def _grad(ctx, g):
-        rows, index, logprob, targets = _saved(ctx, 1, 2)
+        k = ctx.k
+        rows, targets, index, logprob = ctx.saved_tensors
+        rows, n, dev = _saved_rows(rows, targets, ctx.like)
+        if (index.dtype is not torch.int64 or index.numel() != k * n or index.get_device() != dev
+                or logprob.dtype is not torch.float32 or logprob.numel() != k * n or logprob.get_device() != dev):
+            raise _replaced()
+        index, logprob = index.contiguous(), logprob.contiguous()
         d, ctx.d = ctx.d, None
         ready = d is not None
         if not ready:
             d = _gradient_like(rows)
-        _lib.run_distill(rows, index, logprob, targets, *ctx.opts, None, d, ctx.ws, g.contiguous(), int(ready))
+        _lib.run_distill(rows, index, logprob, k, targets, *ctx.opts, None, d, ctx.ws, g.contiguous(), int(ready))
         return d, None, None, None, None, None
 
     _once = staticmethod(torch.autograd.function.once_differentiable(_grad.__func__))
@@ -200,7 +223,7 @@ def _distill(rows, index, logprob, targets, opts, lead, gradient):
     if whole:
         ws = torch.empty(_lib.distill_workspace_bytes(loss.numel()), dtype=torch.uint8, device=rows.device)
     d = _gradient_like(rows) if gradient else None
-    _lib.run_distill(rows, index, logprob, targets, *opts, loss, d, ws)
+    _lib.run_distill(rows, index, logprob, index.shape[2], targets, *opts, loss, d, ws)
     return loss, d, ws
 
 

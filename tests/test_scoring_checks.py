@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from aiwn_b200 import distill_loss, token_logprobs
+from aiwn_b200 import distill_loss, scoring, token_logprobs
 from aiwn_b200._lib import ILError
 
 B, T, V, K = 2, 3, 40, 4
@@ -41,3 +41,48 @@ def test_tensors_of_more_dimensions_than_the_rows_are_refused():
         distill_loss(z, index[0], logprob[0])
     with pytest.raises(ILError, match="shape"):
         distill_loss(z[0], index, logprob)
+
+
+class _Ctx:
+    """What a backward gets, with saved tensors as a hook may have replaced them."""
+
+    def __init__(self, saved, opts, k=K):
+        self.saved_tensors, self.opts, self.k = saved, opts, k
+        self.like = scoring._like(torch.empty(B, T, V))
+        self.d = self.ws = None
+
+
+def test_saved_tensors_that_hooks_replace_by_others_are_refused():
+    """Hooks may return tensors of another device, type or size: their addresses must not reach a kernel.  All are on the
+    CPU here, the forward's and the replaced ones, but for the one on another device."""
+    rows, tokens = torch.randn(B, T, V), torch.zeros(B, T, dtype=torch.long)
+    per_row, stats = torch.empty(B, T), torch.empty(B, T, 2)
+    index, top = torch.zeros(B, T, K, dtype=torch.long), torch.empty(B, T, K)
+
+    scores = (rows, tokens, per_row, stats, index)
+    slots = (rows, tokens, index, top)
+    like = scoring._like(rows)
+    for t in (tokens, None, tokens.t().contiguous().t()):
+        got, n, dev = scoring._saved_rows(rows, t, like)
+        assert got is rows and n == B * T and dev == -1
+    turned = rows.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(scoring._saved_rows(turned, tokens, like)[0], turned)
+    assert scoring._saved_rows(turned, tokens, like)[0].is_contiguous()
+
+    for i, other in [(0, rows.bfloat16()), (0, rows[..., :-1]), (0, rows[0]), (0, rows.transpose(0, 1)), (1, tokens.int()),
+                     (1, tokens.t()), (1, tokens[:1]), (2, per_row.double()), (2, per_row[:1]), (3, stats[..., :1]),
+                     (4, index[..., :1]), (4, index.int())]:
+        ctx = _Ctx([other if n == i else t for n, t in enumerate(scores)], (K, 1.0, -100))
+        with pytest.raises(ILError, match="saved tensor"):
+            scoring._TokenLogprobs._grad(ctx, per_row, None, None, top)
+    for i, other in [(0, rows.bfloat16()), (0, rows[:1]), (1, tokens.int()), (1, tokens[..., None]), (2, index.int()),
+                     (2, index[:, :1]), (3, top.double()), (3, top[..., :2])]:
+        ctx = _Ctx([other if n == i else t for n, t in enumerate(slots)], (-100, 0.5, 1.0, 0, 1))
+        with pytest.raises(ILError, match="saved tensor"):
+            scoring._Distill._grad(ctx, torch.ones(()))
+    for saved, grad in ((scores, lambda c: scoring._TokenLogprobs._grad(c, per_row, None, None, top)),
+                        (slots, lambda c: scoring._Distill._grad(c, torch.ones(())))):
+        ctx = _Ctx(saved, (K, 1.0, -100))
+        ctx.like = (*ctx.like[:2], 0)  # the forward ran on a GPU
+        with pytest.raises(ILError, match="saved tensor"):
+            grad(ctx)

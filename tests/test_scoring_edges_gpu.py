@@ -1,9 +1,10 @@
 """token_logprobs and distill_loss on the GPU where they once went wrong: logits whose exponents change form on the
-way."""
+way, saved tensors that hooks replace."""
 import pytest
 import torch
 
-from aiwn_b200 import token_logprobs
+from aiwn_b200 import distill_loss, token_logprobs
+from aiwn_b200._lib import ILError
 from test_scoring_gpu import DEV, check_distill, check_scores, make_logits, teacher
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +43,18 @@ def test_distill_where_the_exponent_changes_form(V, sign, order):
         for tail in (False, True):
             check_distill(z, index, logprob, tokens, alpha=0.5, temperature=tau, tail=tail)
             check_distill(z, index, logprob, None, temperature=tau, tail=tail)
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t.cpu(), lambda t: t.double() if t.is_floating_point() else t.int(),
+                                    lambda t: t[:1] if t.dim() else t], ids=["host", "types", "sizes"])
+def test_saved_tensors_that_no_kernel_takes(unpack):
+    """A hook's tensors on another device, of another type or size are refused before a launch."""
+    z = make_logits(2, 3, 65, torch.float32).requires_grad_(True)
+    tokens = torch.zeros(2, 3, dtype=torch.int64, device=DEV)
+    index, logprob = teacher(2, 3, 65, 4)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        outs = [token_logprobs(z, tokens, 2).logprob.sum(), distill_loss(z, index, logprob, tokens, alpha=0.5),
+                distill_loss(z, index, logprob, reduction="none").sum()]
+    for out in outs:
+        with pytest.raises(ILError, match="saved tensor"):
+            out.backward()
