@@ -1,8 +1,11 @@
 // il_capi.cu -- the extern "C" entry points declared in include/aiwn_il.h.
 //
-// Argument checking, kernel selection and launch.  All kernels are compiled
-// into this one translation unit (they are included below), so the library
-// needs no relocatable device code.
+// Argument checking, kernel selection and launch.  The kernels are compiled
+// into this translation unit (they are included below) and, those on rows of
+// logits, into il_logits.cu; neither calls device code of the other, so the
+// library needs no relocatable device code.  The error word of kernels whose
+// waits give up is here.
+#define IL_ERROR_WORD
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>

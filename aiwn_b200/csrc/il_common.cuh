@@ -109,13 +109,19 @@ __device__ __forceinline__ void store_gx(void* gx, int64_t idx, float v) {
 }
 
 // Device-side error word: kernels whose bounded waits give up set it, the
-// host reads it back with il_check_device_status().  The library is a single
-// translation unit (il_capi.cu includes every kernel header), so this is the
-// one definition.
-__device__ unsigned int g_il_error = 0;
-
+// host reads it back with il_check_device_status().  Without relocatable
+// device code every translation unit would have a word of its own, so it is
+// in the one that reads it (il_capi.cu, which defines IL_ERROR_WORD); in the
+// others report_error has no definition, and a kernel that calls it does not
+// build.
 constexpr unsigned int kErrTimeout = 1u;
 
+#ifdef IL_ERROR_WORD
+__device__ unsigned int g_il_error = 0;
+
 __device__ __forceinline__ void report_error(unsigned int code) { atomicOr(&g_il_error, code); }
+#else
+__device__ void report_error(unsigned int code);
+#endif
 
 }  // namespace il
