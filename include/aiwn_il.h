@@ -217,8 +217,9 @@ IL_API int il_attention_dropout_mask(uint8_t* keep, int64_t B, int64_t T, int64_
  * entropy [N], stats [N, 2] for the backward (8-byte aligned, or NULL),
  * top_index and top_logprob [N, k] (largest first, equal logits by index).
  * V <= 2^21, k <= 128 and <= V.
- *   A row whose token is ignore_index is padding: its logits are not read,
- * logprob and entropy are 0, its indices -1 and their log probabilities -inf.
+ *   A row whose token is ignore_index is padding: whatever its logits are (they
+ * may be read, but count for nothing), logprob and entropy are 0, its indices
+ * -1 and their log probabilities -inf.
  * A token outside [0, V) gets NaN.  Where every logit is -inf, logprob is
  * -inf and the entropy 0; a NaN or +inf logit makes a row's results NaN (a NaN
  * counts as -inf among the alternatives).

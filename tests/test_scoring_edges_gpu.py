@@ -58,3 +58,36 @@ def test_saved_tensors_that_no_kernel_takes(unpack):
     for out in outs:
         with pytest.raises(ILError, match="saved tensor"):
             out.backward()
+
+
+@pytest.mark.parametrize("V", [65, 1024, 5003, 50021])
+def test_padded_rows_count_for_nothing_whatever_they_hold(V):
+    """NaN and infinite logits, slots beyond the vocabulary and upstream gradients of NaN in rows of padding."""
+    z = make_logits(2, 8, V, torch.float32)
+    tokens = torch.randint(0, V, (2, 8), device=DEV)
+    index, logprob = teacher(2, 8, V, 5)
+    pad = torch.zeros(2, 8, dtype=torch.bool, device=DEV)
+    pad[0, ::3] = pad[1, 4:] = True
+    tokens[pad] = -100
+    plain = z.clone().requires_grad_(True)
+    dirty = z.clone()
+    dirty[pad] = float("nan")
+    dirty[1, 5] = float("inf")
+    dirty = dirty.requires_grad_(True)
+    index2, logprob2 = index.clone(), logprob.clone()
+    index2[pad], logprob2[pad] = V + 3, float("nan")
+    up = torch.ones(2, 8, device=DEV)
+    bad = up.masked_fill(pad, float("nan"))
+
+    def run(x, idx, lp, g):
+        r = token_logprobs(x, tokens, 4)
+        loss = distill_loss(x, idx, lp, tokens, alpha=0.5, temperature=2.0)
+        each = distill_loss(x, idx, lp, tokens, alpha=0.5, reduction="none", tail=True)
+        return (*(t.detach() for t in r), loss.detach(), each.detach(),
+                torch.autograd.grad([r.logprob, r.entropy, r.top_logprob], x, [g, g, g[..., None].expand(2, 8, 4)])[0],
+                torch.autograd.grad(loss, x)[0], torch.autograd.grad(each, x, g)[0])
+
+    for a, b in zip(run(plain, index, logprob, up), run(dirty, index2, logprob2, bad)):
+        assert torch.equal(a, b)
+        if a.dim() and a.dtype != torch.int64:
+            assert not torch.nan_to_num(a[pad], neginf=0.0).any()
