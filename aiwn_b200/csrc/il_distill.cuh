@@ -21,7 +21,8 @@
 // when the student agrees with the teacher: a bitmap of the slots in shared
 // memory keeps their logits out of the running sums, which so become those of
 // the rest, and the slots' own sums are joined to them.  q_r, a small
-// difference of inputs, is taken in 64 bits.
+// difference of inputs, is taken in 64 bits; where it is less than 2^-16 and
+// the student has nothing outside the slots, it is rounding and counts for 0.
 //
 // 8192 x 131072 bf16 with 64 slots and the gradient (4.3 GB, 658 us at the
 // measured copy rate): 883 us.  The rows at work are kept to 62 MB, so that the
@@ -35,6 +36,12 @@
 #include "il_logits.cuh"
 
 namespace il {
+
+// What fp32 log probabilities leave of a mass of one by their own rounding: that of a sum over a long row is a few 2^-20
+// (the largest vocabularies' bound is 2^-12, of which such sums use little).  Less than this is no bucket where the
+// student has nothing outside the slots, that is 2^-150 of its mass or less: the slots then name the whole vocabulary,
+// or all that a mask has left of it, and q_r ln p_r would be 1e-8 times minus infinity, or times a mask's -3e38.
+constexpr double kRounding = 1.0 / 65536;
 
 constexpr int kMean = 1;  // reduction; 2: the sum, 0: each row's loss
 
@@ -222,8 +229,11 @@ struct DistillSums {
             }
         }
         inv_mass = TAIL ? 1.0f : mass != 0.0f ? 1.0f / mass : 0.0f;  // NaN stays
-        q_rest = !TAIL || left < 0.0 ? 0.0f : (float)left;           // NaN stays
-        Q = TAIL ? (left < 0.0 ? mass : 1.0f + 0.0f * q_rest) : mass != 0.0f ? 1.0f + 0.0f * mass : 0.0f;
+        bool none = left < 0.0;  // no bucket
+        if (TAIL && !none && left < kRounding)
+            none = (rest.m - shift_of(s.m)) * a.c + log2f(rest.s) - log2f(s.s) < kMinExp;
+        q_rest = !TAIL || none ? 0.0f : (float)left;  // NaN stays
+        Q = TAIL ? (none ? mass : 1.0f + 0.0f * q_rest) : mass != 0.0f ? 1.0f + 0.0f * mass : 0.0f;
     }
     // of a warp's slots next to the others'
     __device__ __forceinline__ float weight_of(const SlotSums& p) const {

@@ -235,9 +235,11 @@ def distill_loss(logits, top_index, top_logprob, targets=None, *, alpha: float =
     same ``temperature``, as ``token_logprobs(teacher_logits, top_k=k, temperature=temperature)`` returns them; a
     negative index is an empty slot, so rows may hold fewer.  With ``tail=False`` they are normalised to sum to one
     (any constant may be added to a row of them); with ``tail=True`` what they leave of the mass is compared with the
-    student's mass outside the slots, as one bucket.  ``targets`` [...] (int64): the hard labels, needed for
-    ``alpha < 1``; rows whose target is ``ignore_index`` are left out with either alpha.  ``reduction``: "mean" over
-    the rows that are not left out (0 where there are none), "sum", or "none" for the rows' losses [...].
+    student's mass outside the slots, as one bucket (none where less than 2^-16 is left and the student has nothing
+    there: slots of a whole vocabulary, or of all that a mask leaves, whose sum is 1 but for rounding).
+    ``targets`` [...] (int64): the hard labels, needed for ``alpha < 1``; rows whose target is ``ignore_index`` are left
+    out with either alpha.  ``reduction``: "mean" over the rows that are not left out (0 where there are none), "sum", or
+    "none" for the rows' losses [...].
 
     For "mean" and "sum" the gradient of logits that need one is written along with the loss, in the logits' type and
     rounded once; call it under ``torch.no_grad()`` where no gradient is wanted.  An upstream gradient other than 1

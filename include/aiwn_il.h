@@ -250,6 +250,8 @@ IL_API int il_token_logprobs_backward(const void* logits, int dtype, int64_t B, 
  *   tail == 0:  q = softmax(top_logprob) over the slots
  *   tail != 0:  q = exp(top_logprob), the rest q_r = max(0, 1 - sum q) is one
  *               bucket against p_r, the student's mass outside the slots
+ *               (q_r below 2^-16 where p_r is 0 in 32 bits: taken as 0, the
+ *               slots name all that counts and the rest is rounding)
  *   KL = sum q (ln q - ln p) [+ q_r (ln q_r - ln p_r)]
  *   row loss = alpha temperature^2 KL - (1 - alpha) ln softmax(logits)[target]
  * targets [B, T] may be NULL when alpha == 1; rows whose target is

@@ -5,6 +5,7 @@ import torch
 
 from aiwn_b200 import distill_loss, token_logprobs
 from aiwn_b200._lib import ILError
+from logits_oracle import F32, distill64, near, prob_tol
 from test_scoring_gpu import DEV, check_distill, check_scores, make_logits, teacher
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +92,41 @@ def test_padded_rows_count_for_nothing_whatever_they_hold(V):
         assert torch.equal(a, b)
         if a.dim() and a.dtype != torch.int64:
             assert not torch.nan_to_num(a[pad], neginf=0.0).any()
+
+
+@pytest.mark.parametrize("low", [float("-inf"), -3.0e38, -1e9, None], ids=["neg_inf", "lowest", "-1e9", "whole"])
+@pytest.mark.parametrize("V,k", [(65, 65), (128, 128), (1000, 128), (5003, 60), (50021, 128)])
+def test_distill_tail_where_the_slots_name_all_that_counts(V, k, low):
+    """Slots that name the whole vocabulary, or all that a mask leaves to teacher and student.  What their fp32 log
+    probabilities leave of the mass is rounding, and the student has nothing outside: no bucket to compare it with."""
+    if low is None and k < V:
+        pytest.skip("the slots name a part of the vocabulary")
+    z, t = make_logits(4, 8, V, torch.float32, seed=1), make_logits(4, 8, V, torch.float32, seed=2)
+    if low is not None:
+        gone = torch.ones(V, dtype=torch.bool, device=DEV)
+        gone[torch.randperm(V, device=DEV)[:k // 2]] = False
+        z[..., gone] = t[..., gone] = low
+    for tau in (1.0, 2.0):
+        top = token_logprobs(t, None, k, temperature=tau)
+        mass = top.top_logprob.double().exp().sum(-1)
+        assert mass.max() > 1.0 > mass.min()  # rounded to either side
+        leaf = z.clone().requires_grad_(True)
+        loss = distill_loss(leaf, top.top_index, top.top_logprob, temperature=tau, tail=True, reduction="none")
+        (got,) = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+        want, d, err, size = distill64(z, top.top_index, top.top_logprob, None, 1.0, tau, False, "none")
+        # the same but for the slots' sum, which is not 1: a factor of q, and the logarithm of that factor
+        off = (mass - 1).abs()
+        near(loss.detach(), want, err + 2 * off * (want.abs() + tau ** 2), "loss")
+        near(got, d, (2 * prob_tol(V) + (k + 24) * F32 + 2 * off[..., None]) * size + F32 * d.abs() + 1e-37, "grad")
+
+
+def test_distill_tail_of_mass_that_the_student_masks():
+    """More than rounding, where the student has nothing: the divergence is infinite."""
+    for V in (65, 5003):
+        z = make_logits(1, 2, V, torch.float32)
+        index = torch.arange(8, device=DEV).expand(1, 2, 8)
+        logprob = torch.full((1, 2, 8), 1 / 8, device=DEV).log()
+        logprob[0, 0, 7] -= 0.01  # leaves 1e-3
+        z[..., 8:] = float("-inf")
+        loss = distill_loss(z, index, logprob, tail=True, reduction="none")
+        assert torch.isposinf(loss[0, 0]) and torch.isfinite(loss[0, 1])
