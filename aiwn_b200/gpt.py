@@ -387,6 +387,6 @@ class GraphedTrainStep:
         self.y.copy_(y, non_blocking=True)
         if self.top_index is not None:
             self.top_index.copy_(top_index, non_blocking=True)
-            self.top_logprob.copy_(top_logprob, non_blocking=True)
+            self.top_logprob.copy_(top_logprob.detach(), non_blocking=True)  # a teacher scored with gradients on, too
         self.graph.replay()
         return self.loss

@@ -1,11 +1,14 @@
 """token_logprobs and distill_loss refuse, before anything reaches the device (no GPU needed), calls that would give
 wrong results without a word."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from aiwn_b200 import distill_loss, scoring, token_logprobs
 from aiwn_b200._lib import ILError
+from aiwn_b200.gpt import GraphedTrainStep
 
 B, T, V, K = 2, 3, 40, 4
 
@@ -86,3 +89,16 @@ def test_saved_tensors_that_hooks_replace_by_others_are_refused():
         ctx.like = (*ctx.like[:2], 0)  # the forward ran on a GPU
         with pytest.raises(ILError, match="saved tensor"):
             grad(ctx)
+
+
+def test_graphed_step_keeps_nothing_of_the_teachers_graph():
+    """A teacher scored with gradients on: copying its log probabilities must not tie the step's buffer to its graph."""
+    step = GraphedTrainStep.__new__(GraphedTrainStep)
+    step.x, step.y = torch.zeros(B, T, dtype=torch.long), torch.zeros(B, T, dtype=torch.long)
+    step.top_index, step.top_logprob = torch.zeros(B, T, K, dtype=torch.long), torch.zeros(B, T, K)
+    step.graph, step.loss = SimpleNamespace(replay=lambda: None), torch.zeros(())
+    given = torch.randn(B, T, K, requires_grad=True).log_softmax(-1)
+    for _ in range(2):
+        step(step.x, step.y, torch.ones_like(step.top_index), given)
+    assert not step.top_logprob.requires_grad and step.top_logprob.grad_fn is None
+    assert torch.equal(step.top_logprob, given.detach()) and step.top_index.all()
