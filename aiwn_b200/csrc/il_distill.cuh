@@ -25,13 +25,15 @@
 // the student has nothing outside the slots, it is rounding and counts for 0.
 //
 // 8192 x 131072 bf16 with 64 slots and the gradient (4.3 GB, 658 us at the
-// measured copy rate): 883 us.  The rows at work are kept to 62 MB, so that the
+// measured copy rate): 890 us.  The rows at work are kept to 62 MB, so that the
 // second reading finds them in the L2: 148 rows of 256 KB (a CTA of 512 threads
 // an SM) read 544 MB of 537 from HBM, 296 rows 871 MB and took 1007 us.  Rows of
-// 128 KB take 256 threads, two rows an SM (4096 x 65536: 252 us, of 165).  What is left is
+// 128 KB take 256 threads, two rows an SM (4096 x 65536: 254 us, of 165).  What is left is
 // what a row costs between its two readings (join, factors, two barriers), which
 // one or two CTAs an SM do not hide: DRAM is 64% busy, the issue slots 48%.
-// 4096 x 32768 bf16, 20 slots, the loss alone (0.27 GB): 53 us, 78%.
+// 4096 x 32768 bf16, 20 slots, the loss alone: 61 us (0.27 GB, 41 us at the
+// measured copy rate); with 30% of the rows padding, which are not read, 53 us
+// (0.19 GB, 29 us): rows are dealt out beforehand, and some CTAs keep all theirs.
 #pragma once
 #include "il_logits.cuh"
 

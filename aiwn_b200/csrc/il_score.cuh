@@ -22,8 +22,10 @@
 // that every logit above a running bound was put into, with a barrier a step,
 // took 614 us, and reading eighths again instead of thirty-seconds 287 us.
 //
-// 8192 x 65536 bf16 with the gradient of log probability and entropy: 177 us
-// forward, 310 us backward (2.1 GB, the measured copy rate).
+// 8192 x 65536 bf16 with the gradient of log probability and entropy, a fifth
+// of the rows padding (not read): forward 178 us (0.86 GB, 131 us at the
+// measured copy rate), backward 310 us (1.93 GB, 296 us).  Without padding 190
+// us (164) and 355 us (328).
 #pragma once
 #include <type_traits>
 
@@ -637,7 +639,8 @@ __global__ void __launch_bounds__(256) score_grad_warp_kernel(ScoreGradArgs a) {
     }
 }
 
-constexpr int kGradThreads = 128;  // 8192 x 65536 bf16: 310 us; with 512, whose parts of a row end together, 381 us
+// 8192 x 65536 bf16, a fifth of the rows padding: 310 us; with 512, whose parts of a row end together, 381 us
+constexpr int kGradThreads = 128;
 
 // CTA `part` of 2^lg of a row
 template <int DT>

@@ -94,13 +94,11 @@ def test_padded_rows_count_for_nothing_whatever_they_hold(V):
             assert not torch.nan_to_num(a[pad], neginf=0.0).any()
 
 
-@pytest.mark.parametrize("low", [float("-inf"), -3.0e38, -1e9, None], ids=["neg_inf", "lowest", "-1e9", "whole"])
-@pytest.mark.parametrize("V,k", [(65, 65), (128, 128), (1000, 128), (5003, 60), (50021, 128)])
+@pytest.mark.parametrize("V,k,low", [(V, k, low) for V, k in [(65, 65), (128, 128), (1000, 128), (5003, 60), (50021, 128)]
+                                     for low in (float("-inf"), -3.0e38, -1e9, None) if low is not None or k == V])
 def test_distill_tail_where_the_slots_name_all_that_counts(V, k, low):
-    """Slots that name the whole vocabulary, or all that a mask leaves to teacher and student.  What their fp32 log
+    """Slots that name the whole vocabulary (None), or all that a mask leaves to teacher and student.  What their fp32 log
     probabilities leave of the mass is rounding, and the student has nothing outside: no bucket to compare it with."""
-    if low is None and k < V:
-        pytest.skip("the slots name a part of the vocabulary")
     z, t = make_logits(4, 8, V, torch.float32, seed=1), make_logits(4, 8, V, torch.float32, seed=2)
     if low is not None:
         gone = torch.ones(V, dtype=torch.bool, device=DEV)
